@@ -348,6 +348,121 @@ CTTS_API int ctts_op_causal_conv1d(const float* x, int batch, int c_in, int T, c
 CTTS_API int ctts_op_embed_gather(const float* table, int vocab, int H, const int64_t* ids, int n,
                          float* out, int* bad_count, void* stream);
 
+/* ------------------------------------------------ paged KV-cache operators
+ * One serving step over a paged cache is a run of three operators: plan
+ * (request lengths -> block tables, positions, slots), append (QK-Norm, RoPE,
+ * new keys and values into their slots) and attention (the new rows of every
+ * request over its pages).  No counterpart in the reference, whose cache is
+ * one growing vector per utterance (qwen.rs:139-149); ctts_kv_* is the
+ * contiguous form of this framework.  All pointers are device pointers, every
+ * call is asynchronous on `stream`, allocates nothing and can be captured in
+ * a CUDA graph.  Arguments the host can see are checked (CTTS_ERR_ARG,
+ * CTTS_ERR_RANGE); lengths, offsets and page numbers live on the device and
+ * are clamped there, so a bad one never reads or writes out of range. */
+
+/* K and V pools of n_pages pages of page_size token slots (a power of two,
+ * 8..256).  Element d of KV head h of slot t of page p lies at
+ *   p*page_stride + t*token_stride + h*head_stride + d     (in elements)
+ * in both pools: [page, token, head, hd], [page, head, token, hd] and other
+ * orders all fit.  head_dim is 64 or 128; strides are multiples of 16 bytes,
+ * k and v 16-byte aligned.  n_pages * page_size < 2^31. */
+typedef struct {
+  void *k, *v;
+  int64_t page_stride, token_stride, head_stride;
+  int n_pages, page_size, n_kv_heads, head_dim;
+  int dtype; /* CTTS_F32 or CTTS_BF16 */
+} ctts_paged_kv;
+
+/* Block tables, offsets and slots of one step from the request lengths, in
+ * one launch.  Request b holds ceil(ctx_lens[b] / page_size) pages, listed in
+ * row b of block_tables, and asks for new_lens[b] rows: > 0 rows to append,
+ * 0 idle, < 0 finished.  free_pages is a stack of *free_count free pages.
+ *  1. Finished requests give their pages back: pushed on the stack in request
+ *     and page order.
+ *  2. The others are granted in request order, up to the first one that does
+ *     not fit (its new pages exceed what is left, its rows exceed max_rows in
+ *     all, or its pages exceed max_pages).  It and all requests behind it get
+ *     no rows in this step and keep their lengths.  New pages come from the
+ *     top of the stack, in request and page order.
+ * Written: seq_lens [batch] (context + granted rows; 0 for finished ones),
+ * cu_rows [batch+1] (row offsets: request b owns rows cu_rows[b] ..
+ * cu_rows[b+1]), positions and slots [max_rows] (slot = page*page_size +
+ * position % page_size; -1 both in rows behind the last request), state [4]
+ * = {free pages now, rows, requests ahead of the first refused one (batch:
+ * none refused), pages taken}, the taken entries of block_tables and the
+ * pushed entries of free_pages; nothing else.  The inputs are not changed, so
+ * a repeated call gives the same step; the next step passes seq_lens as its
+ * ctx_lens and state as its free_count, with other buffers for its outputs
+ * (an output that is an input too is CTTS_ERR_ARG).  batch <= 4096.  A
+ * negative context counts as 0. */
+typedef struct {
+  const int *ctx_lens, *new_lens, *free_count;
+  int *block_tables, *free_pages;
+  int *seq_lens, *cu_rows, *positions, *slots, *state;
+  int64_t table_ld; /* entries from one row of block_tables to the next, >= max_pages */
+  int batch, page_size, max_pages, free_capacity /* entries of free_pages */, max_rows;
+} ctts_paged_plan;
+CTTS_API int ctts_op_paged_plan(const ctts_paged_plan* p, void* stream);
+
+/* New rows into a paged cache: x [rows, (n_heads + 2*n_kv_heads)*head_dim]
+ * (query, key, value heads, as the fused QKV linear writes them).  Queries
+ * and keys: RMSNorm per head with gain q_norm / k_norm [head_dim] (both NULL:
+ * no norm), then NeoX RoPE at positions[row] (angles in double precision, so
+ * far positions keep theirs).  Queries go to q [rows, n_heads, head_dim],
+ * keys and values to slots[row] of the pools, each rounded once to its type.
+ * A row whose slot lies outside the pools (-1: padding) writes nothing, its
+ * query included.  The slots of one call are distinct.  x_ld and q_ld are row
+ * strides in elements (multiples of 16 bytes; x and q 16-byte aligned). */
+typedef struct {
+  ctts_paged_kv kv;
+  const void* x;
+  void* q;
+  const int *positions, *slots;
+  const float *q_norm, *k_norm;
+  int64_t x_ld, q_ld;
+  double theta;
+  float eps;
+  int rows, n_heads, x_dtype, q_dtype;
+} ctts_paged_append;
+CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
+
+/* Causal attention of each request's new rows over its pages (their own keys
+ * and values included: append first).  Rows cu_rows[b] .. cu_rows[b+1] of q
+ * [rows, n_heads, head_dim] belong to request b and sit at the last positions
+ * of its seq_lens[b] tokens; a row at position p attends to keys 0..p:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j
+ * Query head h reads KV head h / (n_heads / n_kv_heads).  A row that sees no
+ * key (its position is negative, or only pages with numbers outside
+ * 0..n_pages-1, whose keys are hidden) gives zeros; rows behind
+ * cu_rows[batch] are left as they were.  Slots at and behind a request's
+ * length are never read into a result, whatever they hold.
+ * max_new is an upper bound of the requests' new rows (rows beyond it are
+ * left as they were); a length above max_pages*page_size is cut to that.
+ * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
+ * n_heads / n_kv_heads <= 16.  Scores, softmax and sums are float32.  With
+ * bf16 queries the softmax weights enter the product with V in bf16; with
+ * float32 queries every product carries at least 16 significant bits of the
+ * weights and 24 of the scores' operands.
+ * The result depends on the split of the work over the GPU, which follows
+ * from the lengths: the same call gives the same bits.
+ * workspace: ctts_op_paged_attention_workspace bytes, 16-byte aligned, no
+ * initial contents wanted; calls that may overlap need one each. */
+typedef struct {
+  ctts_paged_kv kv;
+  const void* q;
+  void* out;
+  const int *block_tables, *cu_rows, *seq_lens;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t q_ld, out_ld, table_ld;
+  int batch, rows, n_heads, max_pages, max_new, q_dtype;
+  float scale; /* > 0 */
+} ctts_paged_attn;
+CTTS_API int ctts_op_paged_attention(const ctts_paged_attn* p, void* stream);
+/* Workspace bytes a call with these sizes needs on the current device (the
+ * data pointers are not looked at). */
+CTTS_API int ctts_op_paged_attention_workspace(const ctts_paged_attn* p, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,189 @@
+// paged_attn.cuh -- how the work of a paged attention call is cut: the line
+// of key tiles, a CTA's piece of it, and the partial states of divided items.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace ctts {
+
+// A partial state in the workspace.  CTA c has two places: 2c for a piece
+// that enters it (middle or end of an item), 2c + 1 for one that begins in it
+// and leaves it.
+constexpr int kPartStart = 1, kPartMiddle = 2, kPartEnd = 3;
+struct AttnPart {
+  int kind = 0;  // 0: none
+  int row0 = 0;  // the request's first row of q
+  int packed0 = 0, rows = 0, h = 0;  // first packed row, packed rows, KV head
+  int pad[3] = {0, 0, 0};
+};
+
+struct PagedAttnArgs {
+  ctts_paged_attn p;
+  int group = 1, shift = 0;      // query heads per KV head, log2 of the page size
+  int ctas = 0, tile_rows = 0;   // CTAs, packed rows per item
+  int rows_used = 0;             // packed rows an item can have
+  AttnPart* parts = nullptr;     // [2 * ctas]
+  float* acc = nullptr;          // [2 * ctas][tile_rows][hd + 2]: maximum, sum, output
+};
+
+CTTS_DEV float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A request's lengths, cut to what the buffers hold.
+struct AttnReq {
+  int r0, cnt, nn, len;  // first row, rows, rows computed (cnt cut to max_new), tokens
+};
+CTTS_DEV AttnReq attn_req(const PagedAttnArgs& a, int b) {
+  AttnReq r;
+  r.r0 = min(max(a.p.cu_rows[b], 0), a.p.rows);
+  r.cnt = min(max(a.p.cu_rows[b + 1], r.r0), a.p.rows) - r.r0;
+  r.nn = min(r.cnt, a.p.max_new);
+  r.len = (int)min((long)max(a.p.seq_lens[b], 0), (long)a.p.max_pages << a.shift);
+  return r;
+}
+// Key tiles of row tile m: up to the position of its last row; at least one,
+// which also writes the zeros of rows that see nothing.
+template <int R, int C>
+CTTS_DEV int attn_tiles(const AttnReq& r, int m, int group) {
+  const int last = min(r.nn, (int)(((long)(m + 1) * R - 1) / group) + 1);  // rows ahead of the tile's end
+  const int keys = min(r.len, r.len - r.cnt + last);
+  return max(1, (keys + C - 1) / C);
+}
+template <int R, int C>
+CTTS_DEV long attn_units(const PagedAttnArgs& a, int b) {
+  const AttnReq r = attn_req(a, b);
+  const int mt = (int)(((long)r.nn * a.group + R - 1) / R);
+  long n = 0;
+  for (int m = 0; m < mt; m++) n += attn_tiles<R, C>(r, m, a.group);
+  return n * a.p.kv.n_kv_heads;
+}
+
+struct AttnStart {
+  long units;  // this CTA's
+  long skip;   // units of request b ahead of them
+  int b;
+};
+
+// This CTA's piece of the line.  The block sums the requests' units (four
+// requests a thread and turn); a second pass finds the request the piece
+// begins in, from registers when one turn holds the batch.
+template <int R, int C, int NT>
+CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
+  constexpr int PER = 4, W = NT / 32;
+  __shared__ long wsum[2][W];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.p.batch;
+  long u[PER];
+  long total = 0, first = 0, mine_before = 0;
+  int ph = 0;
+  // one turn: units of requests base + tid*PER + j; returns the turn's sum, mine_before = units ahead of the thread's
+  auto turn = [&](int base) {
+    long t = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int b = base + tid * PER + j;
+      u[j] = b < n ? attn_units<R, C>(a, b) : 0;
+      t += u[j];
+    }
+    long inc = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) wsum[ph][warp] = inc;
+    __syncthreads();
+    long all = 0, ahead = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      if (w < warp) ahead += wsum[ph][w];
+      all += wsum[ph][w];
+    }
+    mine_before = ahead + inc - t;
+    ph ^= 1;
+    return all;
+  };
+  for (int base = 0; base < n; base += NT * PER) total += turn(base);
+  // no more pieces than tiles: every piece of a divided item lies in the CTA next to the one before
+  const long ctas = min((long)a.ctas, total), c = blockIdx.x;
+  const long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
+  if (tid == 0) {
+    out->units = u1 - u0;
+    out->b = 0;
+    out->skip = 0;
+  }
+  __syncthreads();
+  if (u1 == u0) return;
+  for (int base = 0; base < n; base += NT * PER) {
+    const long all = n <= NT * PER ? total : turn(base);
+    long at = first + mine_before;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      if (at <= u0 && u0 < at + u[j]) {
+        out->b = base + tid * PER + j;
+        out->skip = u0 - at;
+      }
+      at += u[j];
+    }
+    first += all;
+    if (first > u0) break;
+  }
+  __syncthreads();
+}
+
+// A place on the line: request, row tile, KV head, key tile.
+struct AttnCursor {
+  int b, m, h, kt, nt, mt;
+  int r0, cnt, nn, len;
+
+  CTTS_DEV void load(const PagedAttnArgs& a, int R) {
+    const AttnReq r = attn_req(a, b);
+    r0 = r.r0; cnt = r.cnt; nn = r.nn; len = r.len;
+    mt = (int)(((long)nn * a.group + R - 1) / R);
+  }
+  template <int R, int C>
+  CTTS_DEV void tiles(const PagedAttnArgs& a) {
+    nt = attn_tiles<R, C>(AttnReq{r0, cnt, nn, len}, m, a.group);
+  }
+  template <int R, int C>
+  static CTTS_DEV AttnCursor at(const PagedAttnArgs& a, const AttnStart& s) {
+    AttnCursor c;
+    c.b = s.b;
+    c.load(a, R);
+    long skip = s.skip;
+    for (c.m = 0;; c.m++) {
+      c.tiles<R, C>(a);
+      const long in = (long)c.nt * a.p.kv.n_kv_heads;
+      if (skip < in || c.m + 1 >= c.mt) break;
+      skip -= in;
+    }
+    c.h = (int)(skip / c.nt);
+    c.kt = (int)(skip % c.nt);
+    return c;
+  }
+  // (never called at the end of the line)
+  template <int R, int C>
+  CTTS_DEV void next(const PagedAttnArgs& a) {
+    if (++kt < nt) return;
+    kt = 0;
+    if (++h < a.p.kv.n_kv_heads) return;
+    h = 0;
+    if (++m < mt) {
+      tiles<R, C>(a);
+      return;
+    }
+    m = 0;
+    do {
+      b++;
+      load(a, R);
+    } while (mt == 0 && b + 1 < a.p.batch);
+    tiles<R, C>(a);
+  }
+};
+
+}  // namespace ctts
