@@ -14,7 +14,7 @@ size_t type_size(int dtype) { return dtype == CTTS_BF16 ? 2 : 4; }
 
 // a stride of `ld` elements that keeps rows of at least `width` elements apart and 16-byte aligned
 bool stride_ok(int64_t ld, int64_t width, int dtype) {
-  return ld >= width && ld <= (int64_t)1 << 40 && ld * (int64_t)type_size(dtype) % 16 == 0;
+  return ld >= width && ld <= (int64_t)1 << 36 && ld * (int64_t)type_size(dtype) % 16 == 0;
 }
 
 int check_pool(const ctts_paged_kv& kv) {

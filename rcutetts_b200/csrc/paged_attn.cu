@@ -27,26 +27,6 @@ namespace {
 constexpr int kKeys = 64;  // keys per tile
 constexpr int kNT = 128;   // threads
 
-CTTS_DEV uint32_t pack_bf2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// x in N bf16 terms (packed pairs), each the rounding of what the ones before
-// leave: N = 1, 2, 3 keep 8, 16, 24 bits.  What an infinite x leaves is NaN;
-// the maximum turns that into a large negative number, so the sum of the
-// terms is the infinity again (of a finite x less than 2^120 is left).
-template <int N>
-CTTS_DEV void split_bf2(float x0, float x1, uint32_t* t) {
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    t[i] = pack_bf2(x0, x1);
-    if (i + 1 < N) {
-      x0 = fmaxf(x0 - bf_lo(t[i]), -1.3e36f);
-      x1 = fmaxf(x1 - bf_hi(t[i]), -1.3e36f);
-    }
-  }
-}
 CTTS_DEV void mma_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -79,9 +59,10 @@ CTTS_DEV void cp_wait() {
 template <bool QF, bool KF, int HD, bool CHUNK>
 struct Shape {
   static constexpr int R = CHUNK ? 64 : 16;
-  // bf16 terms of a query and of a softmax weight (a float32 key has three, a value two)
+  // bf16 terms of a float32 operand (queries and softmax weights; keys and
+  // values of a float32 cache): 24 bits, so a float32 call keeps float32
   static constexpr int NQ = QF ? 3 : 1;
-  static constexpr int NP = QF ? 2 : 1;
+  static constexpr int NP = QF ? 3 : 1;
   static constexpr int ES = KF ? 4 : 2;
   static constexpr int ROWB = HD * ES;
   // float32 rows are padded so that the fragment reads (8 keys x 8 bytes of K,
@@ -302,25 +283,28 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       }
 #pragma unroll
       for (int j = 0; j < KT; j += 2) {
-        uint32_t pa[2][4], tmp[2];
-        split_bf2<S::NP>(s[j][0], s[j][1], tmp); pa[0][0] = tmp[0]; pa[1][0] = tmp[1];
-        split_bf2<S::NP>(s[j][2], s[j][3], tmp); pa[0][1] = tmp[0]; pa[1][1] = tmp[1];
-        split_bf2<S::NP>(s[j + 1][0], s[j + 1][1], tmp); pa[0][2] = tmp[0]; pa[1][2] = tmp[1];
-        split_bf2<S::NP>(s[j + 1][2], s[j + 1][3], tmp); pa[0][3] = tmp[0]; pa[1][3] = tmp[1];
+        uint32_t pa[S::NP][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t t[S::NP];
+          split_bf2<S::NP>(s[j + (i >> 1)][2 * (i & 1)], s[j + (i >> 1)][2 * (i & 1) + 1], t);
+#pragma unroll
+          for (int k = 0; k < S::NP; k++) pa[k][i] = t[k];
+        }
         if (KF) {
 #pragma unroll
           for (int t = 0; t < NO; t++) {
             const float* vp = reinterpret_cast<const float*>(smem + buf * S::STAGE + kKeys * S::KROW +
                                                              (wkey + 8 * j + 2 * tq) * S::VROW) + 8 * t + gq;
             constexpr int LD = S::VROW / 4;
-            uint32_t b0[2], b1[2];
-            split_bf2<2>(vp[0], vp[LD], b0);
-            split_bf2<2>(vp[8 * LD], vp[9 * LD], b1);
+            uint32_t b0[3], b1[3];
+            split_bf2<3>(vp[0], vp[LD], b0);
+            split_bf2<3>(vp[8 * LD], vp[9 * LD], b1);
 #pragma unroll
             for (int k = 0; k < S::NP; k++)
 #pragma unroll
-              for (int n = 0; n < 2; n++)
-                if (k + n <= 1) mma_16816(o[t], pa[k], b0[n], b1[n]);
+              for (int n = 0; n < 3; n++)
+                if (k + n <= 2) mma_16816(o[t], pa[k], b0[n], b1[n]);
           }
         } else {
 #pragma unroll
@@ -344,7 +328,8 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       const bool whole = ends && unit0_kt == 0;
       // a piece from the item's start goes to the CTA's second place, one that enters the CTA to its first
       const int slot = 2 * blockIdx.x + (unit0_kt == 0 ? 1 : 0);
-      float* const part = a.acc + (long)slot * a.tile_rows * (HD + 2);
+      float2* const pml = a.ml + (long)slot * a.tile_rows;
+      float* const part = a.acc + (long)slot * a.tile_rows * HD;
       if (!whole && tid == 0) {
         AttnPart d;
         d.kind = unit0_kt == 0 ? kPartStart : (ends ? kPartEnd : kPartMiddle);
@@ -374,11 +359,10 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
                 *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at + 8 * t) = pack_bf2(x, y);
             }
           } else {
-            float* w = part + (long)r * (HD + 2);
-            if (tq == 0) *reinterpret_cast<float2*>(w) = make_float2(m2[e], l2[e]);
+            if (tq == 0) pml[r] = make_float2(m2[e], l2[e]);
 #pragma unroll
             for (int t = 0; t < NO; t++)
-              *reinterpret_cast<float2*>(w + 2 + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+              *reinterpret_cast<float2*>(part + (long)r * HD + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
           }
         }
       } else {
@@ -418,9 +402,8 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
             else
               *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at) = pack_bf2(x * inv, y * inv);
           } else {
-            float* g = part + (long)r * (HD + 2);
-            if (d == 0) *reinterpret_cast<float2*>(g) = make_float2(M, L);
-            *reinterpret_cast<float2*>(g + 2 + d) = make_float2(x, y);
+            if (d == 0) pml[r] = make_float2(M, L);
+            *reinterpret_cast<float2*>(part + (long)r * HD + d) = make_float2(x, y);
           }
         }
       }
@@ -456,10 +439,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
   }
   __syncthreads();
   const int n = min(last - c + 1, a.ctas - c);  // pieces
-  auto piece = [&](int i, int r) { return a.acc + ((long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.tile_rows + r) * (HD + 2); };
+  auto piece = [&](int i, int r) { return (long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.tile_rows + r; };
   for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
     float mx = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, piece(i, r)[0]);
+    for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, a.ml[piece(i, r)].x);
     mx = warp_max(mx);
     __syncthreads();
     if ((tid & 31) == 0) red[tid >> 5] = mx;
@@ -469,7 +452,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
     if (mx == -INFINITY) mx = 0.0f;
     float l = 0.0f;
     for (int i = tid; i < n; i += kJoinThreads) {
-      const float2 ml = *reinterpret_cast<const float2*>(piece(i, r));
+      const float2 ml = a.ml[piece(i, r)];
       wgt[i] = exp2_fast(ml.x - mx);
       l = fmaf(ml.y, wgt[i], l);
     }
@@ -481,7 +464,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll 4
     for (int i = g; i < n; i += GR) {
-      const float2 v = *reinterpret_cast<const float2*>(piece(i, r) + 2 + 2 * col);
+      const float2 v = *reinterpret_cast<const float2*>(a.acc + piece(i, r) * HD + 2 * col);
       s.x = fmaf(v.x, wgt[i], s.x);
       s.y = fmaf(v.y, wgt[i], s.y);
     }
@@ -522,12 +505,10 @@ cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
   static SmemOptIn opt;
   const size_t smem = S::smem(a.rows_used);
   CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, CHUNK>), smem));
-  CTTS_LK(launch_k(paged_attn_kernel<QF, KF, HD, CHUNK>, dim3(a.ctas), dim3(kNT), smem, s, a));
-  const int rows = (int)std::min((long)a.tile_rows, (long)a.p.max_new * a.group);
-  return launch_k(paged_attn_join_kernel<!QF, HD>, dim3(a.ctas, std::min(rows, 16)), dim3(kJoinThreads), 0, s, a);
+  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK>, dim3(a.ctas), dim3(kNT), smem, s, a);
 }
 
-// The call's shape: f(QF, KF, HD, CHUNK as integral constants)
+// The call's mma.sync shape: f(QF, KF, HD, CHUNK as integral constants)
 template <class F>
 auto with_shape(const ctts_paged_attn& p, F f) {
   const bool qf = p.q_dtype == CTTS_F32, kf = p.kv.dtype == CTTS_F32, wide = p.kv.head_dim == 128;
@@ -538,11 +519,17 @@ auto with_shape(const ctts_paged_attn& p, F f) {
   using N = std::false_type;
   using H64 = std::integral_constant<int, 64>;
   using H128 = std::integral_constant<int, 128>;
-  auto g = [&](auto q, auto k) {
-    if (wide) return chunk ? f(q, k, H128{}, T{}) : f(q, k, H128{}, N{});
-    return chunk ? f(q, k, H64{}, T{}) : f(q, k, H64{}, N{});
-  };
-  return qf ? (kf ? g(T{}, T{}) : g(T{}, N{})) : g(N{}, N{});
+  if (kf) {
+    if (wide) return chunk ? f(T{}, T{}, H128{}, T{}) : f(T{}, T{}, H128{}, N{});
+    return chunk ? f(T{}, T{}, H64{}, T{}) : f(T{}, T{}, H64{}, N{});
+  }
+  if (wide) return qf ? f(T{}, N{}, H128{}, N{}) : f(N{}, N{}, H128{}, N{});
+  return qf ? f(T{}, N{}, H64{}, N{}) : f(N{}, N{}, H64{}, N{});
+}
+
+// Chunks over a bf16 cache run on tcgen05 (paged_attn_tc.cu).
+bool use_tc(const ctts_paged_attn& p) {
+  return p.kv.dtype == CTTS_BF16 && (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) > 16;
 }
 
 int rows_used_of(const ctts_paged_attn& p) {
@@ -553,7 +540,11 @@ int rows_used_of(const ctts_paged_attn& p) {
 
 PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
   PagedAttnPlan pl;
-  with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
+  if (use_tc(p)) {
+    const PagedAttnTc t = paged_attn_tc_plan(p);
+    pl.ctas = t.ctas;
+    pl.tile_rows = t.tile_rows;
+  } else with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
     constexpr bool QF = decltype(q)::value, KF = decltype(k)::value, CH = decltype(ch)::value;
     constexpr int HD = decltype(hd)::value;
     pl.ctas = std::min(kJoinMax, attn_ctas<QF, KF, HD, CH>(rows_used_of(p)));
@@ -576,9 +567,19 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   a.rows_used = rows_used_of(p);
   a.parts = static_cast<AttnPart*>(p.workspace);
   a.acc = reinterpret_cast<float*>(a.parts + 2 * pl.ctas);
-  return with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
-    return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value>(a, s);
-  });
+  a.ml = reinterpret_cast<float2*>(a.acc + (size_t)2 * pl.ctas * pl.tile_rows * p.kv.head_dim);
+  if (use_tc(p))
+    CTTS_LK(launch_paged_attn_tc(a, s));
+  else
+    CTTS_LK(with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
+      return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value>(a, s);
+    }));
+  const int rows = (int)std::min((long)a.tile_rows, (long)p.max_new * a.group);
+  const dim3 grid(a.ctas, std::min(rows, 16)), block(kJoinThreads);
+  const bool bf = p.q_dtype == CTTS_BF16;
+  if (p.kv.head_dim == 64)
+    return bf ? launch_k(paged_attn_join_kernel<true, 64>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 64>, grid, block, 0, s, a);
+  return bf ? launch_k(paged_attn_join_kernel<true, 128>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 128>, grid, block, 0, s, a);
 }
 
 }  // namespace ctts

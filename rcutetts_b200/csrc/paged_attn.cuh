@@ -26,8 +26,30 @@ struct PagedAttnArgs {
   int ctas = 0, tile_rows = 0;   // CTAs, packed rows per item
   int rows_used = 0;             // packed rows an item can have
   AttnPart* parts = nullptr;     // [2 * ctas]
-  float* acc = nullptr;          // [2 * ctas][tile_rows][hd + 2]: maximum, sum, output
+  float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum (in powers of two), sum
+  float* acc = nullptr;          // [2 * ctas][tile_rows][hd]: unnormalised output
 };
+
+CTTS_DEV uint32_t pack_bf2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// x in N bf16 terms (packed pairs), each the rounding of what the ones before
+// leave: N = 1, 2, 3 keep 8, 16, 24 bits.  What an infinite x leaves is NaN;
+// the maximum turns that into a large negative number, so the sum of the
+// terms is the infinity again (of a finite x less than 2^120 is left).
+template <int N>
+CTTS_DEV void split_bf2(float x0, float x1, uint32_t* t) {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    t[i] = pack_bf2(x0, x1);
+    if (i + 1 < N) {
+      x0 = fmaxf(x0 - bf_lo(t[i]), -1.3e36f);
+      x1 = fmaxf(x1 - bf_hi(t[i]), -1.3e36f);
+    }
+  }
+}
 
 CTTS_DEV float exp2_fast(float x) {
   float r;
@@ -185,5 +207,12 @@ struct AttnCursor {
     tiles<R, C>(a);
   }
 };
+
+// tcgen05 form (paged_attn_tc.cu): chunks over a bf16 cache.
+struct PagedAttnTc {
+  int tile_rows = 0, ctas = 0;
+};
+PagedAttnTc paged_attn_tc_plan(const ctts_paged_attn& p);
+cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, cudaStream_t s);
 
 }  // namespace ctts

@@ -1,0 +1,539 @@
+// paged_attn_tc.cu -- attention of chunks of new rows over a bf16 paged cache
+// on the 5th-generation tensor cores (tcgen05).
+//
+// An item is up to two sub-tiles of 128 packed rows (one row per TMEM lane)
+// of one request and KV head.  Per key tile and sub-tile:
+//   S = Q . K^T   both operands in shared memory (K-major, 128-byte swizzle),
+//   softmax       one thread per row: S read from TMEM, the weights written
+//                 back over it in bf16,
+//   O += P . V    P read from TMEM, V from shared memory as it lies in the
+//                 pages ([key][dim]: the MN-major form of the B operand).
+// Warps 0-3 and 4-7 run the softmax of the two sub-tiles, so one computes
+// exponentials while the tensor core multiplies for the other; warp 8 issues
+// the MMAs, warp 9 the TMA copies: one box per page and 64 dims (a 4D map over
+// the pool), K and V in rings of their own.  Missing pages are boxes
+// outside the map, which arrive as zeros.
+//
+// The output is rescaled only when a row's maximum has grown by more than
+// 2^8 since the last time: weights up to 256 lose nothing in floating point,
+// and the pass over O in TMEM becomes rare.  S(j+1) of a sub-tile is issued
+// behind P.V(j), so O is at rest while its softmax threads hold S.
+//
+// float32 queries: queries and weights enter as three bf16 terms (24 bits),
+// key tiles are 64 wide so that three terms of the weights fit over S.
+//
+// Every wait is bounded; one that gives up raises a flag that ends all roles.
+#include <algorithm>
+
+#include "common.cuh"
+#include "launch_state.h"
+#include "paged.cuh"
+#include "paged_attn.cuh"
+#include "tc_ptx.cuh"
+
+namespace ctts {
+
+namespace {
+
+constexpr int kTcThreads = 320;
+
+template <bool QF, int HD>
+struct TcShape {
+  static constexpr int KT = QF ? 64 : 128;                // keys per tile
+  static constexpr int NSUB = QF && HD == 128 ? 1 : 2;    // three terms of 256 wide queries would not fit
+  static constexpr int R = 128 * NSUB;                    // packed rows per item
+  static constexpr int NT = QF ? 3 : 1;                   // terms of queries and weights
+  static constexpr int NC = HD / 64;                      // 128-byte column blocks
+  static constexpr uint32_t QTERM = NC * 128 * 128;       // bytes of one term of one sub-tile
+  static constexpr uint32_t TILE = NC * KT * 128;         // bytes of a K or V tile
+  static constexpr int NS = QF ? (HD == 64 ? 6 : 3) : (HD == 64 ? 4 : 2);
+  static constexpr size_t SMEM = (size_t)NSUB * NT * QTERM + (size_t)2 * NS * TILE + 1024;
+};
+
+// Shared-memory descriptor of a 128-byte swizzled operand.  K-major: lbo
+// unused (1).  MN-major: rows of 64 dims per key, `lbo` bytes between blocks
+// of 64 dims, 1024 bytes between groups of 8 keys.
+CTTS_DEV uint64_t tc_desc(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(lbo >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+// D f32, A and B bf16, M = 128, N = n; B K-major or MN-major
+CTTS_DEV constexpr uint32_t tc_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+CTTS_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {  // A from TMEM
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+CTTS_DEV void tma_4d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+CTTS_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+CTTS_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+CTTS_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+CTTS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+CTTS_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// uses of r[0..31] stay behind this point
+CTTS_DEV void pin32(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 16)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]),
+                 "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]), "+r"(r[i + 12]), "+r"(r[i + 13]),
+                 "+r"(r[i + 14]), "+r"(r[i + 15]));
+}
+CTTS_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+CTTS_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  tmem_st16(taddr, r);
+  tmem_st16(taddr + 16, r + 16);
+}
+
+struct TcBars {
+  uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+};
+
+template <bool QF, int HD>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                                      const __grid_constant__ CUtensorMap tmV, const PagedAttnArgs a,
+                                                                      int box, int order) {
+  using S = TcShape<QF, HD>;
+  constexpr int KT = S::KT, R = S::R, NS = S::NS, NT = S::NT, NC = S::NC;
+  extern __shared__ uint8_t tc_smem[];
+  __shared__ AttnStart start;
+  __shared__ __align__(8) TcBars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int gave_up;
+  const uint32_t sbase = (smem_u32(tc_smem) + 1023u) & ~1023u;
+  const uint32_t qs = sbase, ks = qs + S::NSUB * NT * S::QTERM, vs = ks + NS * S::TILE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) {
+      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&bars.q_full[i], 128);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 128);
+      mbar_init(&bars.o_full[i], 1);
+    }
+    mbar_init(&bars.drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    gave_up = 0;
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  grid_dep_enter();
+  attn_find_start<R, KT, kTcThreads>(a, &start);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;  // S and P of sub-tile s at column 128 s, O at 256 + 128 s
+  const long units = start.units;
+  if (tid < 2) a.parts[2 * blockIdx.x + tid].kind = 0;  // no partial state yet
+  __syncthreads();
+
+  if (units > 0 && warp == 9) {
+    // ---- producer: lane i copies page box i of each tile
+    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    const int nbox = KT / box;
+    long u = 0;
+    for (; u < units; u++) {
+      const int st = (int)(u % NS);
+      const uint32_t par = (uint32_t)((u / NS) & 1);
+      const int kk = cu.kt * KT + lane * box;
+      int page = -1;
+      if (lane < nbox && kk < cu.len) page = a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)];
+      if ((unsigned)page >= (unsigned)a.p.kv.n_pages) page = a.p.kv.n_pages;  // outside the map: zeros
+      const int slot = kk & (a.p.kv.page_size - 1);
+      auto coord = [&](int i) {
+        const int what = (order >> (2 * i)) & 3;
+        return what == 0 ? slot : (what == 1 ? cu.h : page);
+      };
+      const int y = coord(0), z = coord(1), w = coord(2);
+#pragma unroll
+      for (int kv = 0; kv < 2; kv++) {
+        uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
+        if (u >= NS && !mbar_wait(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1)) gave_up = 1;
+        if (__any_sync(0xffffffffu, gave_up)) goto produced;
+        if (lane == 0) mbar_expect_tx(full, S::TILE);
+        __syncwarp();
+        if (lane < nbox) {
+          const uint32_t dst = (kv ? vs : ks) + st * S::TILE + (uint32_t)(lane * box) * 128u;
+#pragma unroll
+          for (int c = 0; c < NC; c++) tma_4d(dst + c * KT * 128, kv ? &tmV : &tmK, c * 64, y, z, w, full);
+        }
+      }
+      if (u + 1 < units) cu.next<R, KT>(a);
+    }
+  produced:
+    __syncwarp();
+    if (gave_up)  // copies in flight land before the block may leave
+      for (long w = u > NS ? u - NS : 0; w <= u && w < units; w++) {
+        mbar_wait(&bars.k_full[w % NS], (uint32_t)((w / NS) & 1));
+        mbar_wait(&bars.v_full[w % NS], (uint32_t)((w / NS) & 1));
+      }
+  } else if (units > 0 && warp == 8) {
+    // ---- MMA issue (one thread)
+    if (lane == 0) {
+      AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+      uint32_t q_par = 0, p_par = 0;  // one bit per sub-tile
+      auto wait = [&](uint64_t* bar, uint32_t par) {
+        if (gave_up || !mbar_wait(bar, par)) gave_up = 1;
+        fence_after();
+        return !gave_up;
+      };
+      auto scores = [&](int s, int st) {
+        const uint32_t kb = ks + st * S::TILE;
+        uint32_t acc = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              umma_bf16(tmem + 128 * s, tc_desc(qs + (s * NT + t) * S::QTERM + c * 16384 + k * 32, 16),
+                        tc_desc(kb + c * KT * 128 + k * 32, 16), tc_idesc(KT, false), acc);
+              acc = 1;
+            }
+        umma_commit(&bars.s_full[s]);
+      };
+      auto values = [&](int s, int st, uint32_t acc) {
+        const uint32_t vb = vs + st * S::TILE;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int k = 0; k < KT / 16; k++) {
+            mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + t * (KT / 2) + k * 8, tc_desc(vb + k * 2048, KT * 128), tc_idesc(HD, true), acc);
+            acc = 1;
+          }
+      };
+      bool fresh = true, ok = true;
+      int nsub = 1;
+      for (long u = 0; u < units && ok; u++) {
+        const int st = (int)(u % NS);
+        if (fresh) {  // a piece begins: its first scores
+          nsub = min(R, cu.nn * a.group - cu.m * R) > 128 ? 2 : 1;
+          ok = wait(&bars.k_full[st], (uint32_t)((u / NS) & 1));
+          for (int s = 0; s < nsub && ok; s++) {
+            ok = wait(&bars.q_full[s], (q_par >> s) & 1);
+            q_par ^= 1u << s;
+            if (ok) scores(s, st);
+          }
+          if (!ok) break;
+          umma_commit(&bars.k_empty[st]);
+        }
+        const bool last = cu.kt + 1 == cu.nt || u + 1 == units;
+        ok = wait(&bars.v_full[st], (uint32_t)((u / NS) & 1));
+        const int sn = (int)((u + 1) % NS);
+        if (ok && !last) ok = wait(&bars.k_full[sn], (uint32_t)(((u + 1) / NS) & 1));
+        for (int s = 0; s < nsub && ok; s++) {
+          ok = wait(&bars.p_full[s], (p_par >> s) & 1);
+          p_par ^= 1u << s;
+          if (!ok) break;
+          values(s, st, fresh ? 0u : 1u);
+          if (last)
+            umma_commit(&bars.o_full[s]);
+          else
+            scores(s, sn);
+        }
+        if (!ok) break;
+        umma_commit(&bars.v_empty[st]);
+        if (!last) umma_commit(&bars.k_empty[sn]);
+        fresh = last;
+        if (u + 1 < units) cu.next<R, KT>(a);
+      }
+      if (!ok) {  // MMAs in flight end before TMEM is given back
+        umma_commit(&bars.drain);
+        mbar_wait(&bars.drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (units > 0 && (warp >> 2) < S::NSUB) {
+    // ---- softmax: one thread per packed row
+    const int s = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 128 * s + lane_base, tO = tmem + 256 + 128 * s + lane_base;
+    const float c2 = a.p.scale * 1.44269504088896340736f;  // scores in powers of two
+    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    uint32_t s_par = 0, o_par = 0;
+    bool fresh = true, ok = true;
+    int kt0 = 0, nrows = 0, pk = 0, pos = 0, pos_lo = 0;
+    bool mine = false, warp_on = false, on = false;
+    float m = -INFINITY, l = 0.0f;
+    for (long u = 0; u < units && ok; u++) {
+      if (fresh) {
+        fresh = false;
+        kt0 = cu.kt;
+        nrows = min(R, cu.nn * a.group - cu.m * R);
+        on = s * 128 < nrows;  // the sub-tile has rows
+        mine = s * 128 + row < nrows;
+        warp_on = s * 128 + (warp & 3) * 32 < nrows;
+        pk = cu.m * R + s * 128 + row;
+        pos = cu.len - cu.cnt + pk / a.group;
+        pos_lo = cu.len - cu.cnt + (pk - lane) / a.group;
+        m = -INFINITY;
+        l = 0.0f;
+        if (on) {
+          // the row's query, as bf16 terms; rows behind the item are zero
+          const long at = mine ? (long)(cu.r0 + pk / a.group) * a.p.q_ld + (long)(cu.h * a.group + pk % a.group) * HD : 0;
+          const uint32_t qrow = qs + s * NT * S::QTERM + row * 128;
+#pragma unroll 4
+          for (int ch = 0; ch < HD / 8; ch++) {
+            uint32_t t[4][NT];
+            if (QF) {
+              float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+              if (mine) {
+                x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + ch * 8);
+                y = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + ch * 8 + 4);
+              }
+              split_bf2<NT>(x.x, x.y, t[0]);
+              split_bf2<NT>(x.z, x.w, t[1]);
+              split_bf2<NT>(y.x, y.y, t[2]);
+              split_bf2<NT>(y.z, y.w, t[3]);
+            } else {
+              uint4 x = make_uint4(0u, 0u, 0u, 0u);
+              if (mine) x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at + ch * 8);
+              t[0][0] = x.x; t[1][0] = x.y; t[2][0] = x.z; t[3][0] = x.w;
+            }
+            const uint32_t dst = qrow + (ch >> 3) * 16384 + (uint32_t)(((ch & 7) ^ (row & 7)) << 4);
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + k * S::QTERM), "r"(t[0][k]), "r"(t[1][k]), "r"(t[2][k]),
+                           "r"(t[3][k])
+                           : "memory");
+          }
+          fence_async();
+          mbar_arrive(&bars.q_full[s]);
+        }
+      }
+      const bool ends = cu.kt + 1 == cu.nt, last = ends || u + 1 == units;
+      if (on) {
+        const int key0 = cu.kt * KT;
+        // 8-key groups whose page does not exist
+        uint32_t dead = 0;
+        {
+          const int kk = key0 + lane * 8;
+          bool d = false;
+          if (lane < KT / 8 && kk < cu.len)
+            d = (unsigned)a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] >= (unsigned)a.p.kv.n_pages;
+          dead = __ballot_sync(0xffffffffu, d);
+        }
+        if (s == 0 && key0 + KT > cu.len) {
+          // slots behind the length may hold anything, and 0 * NaN is NaN:
+          // their values become zeros (both sub-tiles' products come after
+          // this sub-tile's arrival at p_full)
+          const int st = (int)(u % NS);
+          if (!mbar_wait(&bars.v_full[st], (uint32_t)((u / NS) & 1))) gave_up = 1;
+          if (row < KT && key0 + row >= cu.len) {
+#pragma unroll
+            for (int c = 0; c < NC * 8; c++)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + st * S::TILE + (c >> 3) * KT * 128 + row * 128 + (c & 7) * 16), "r"(0)
+                           : "memory");
+          }
+          fence_async();
+        }
+        if (!mbar_wait(&bars.s_full[s], s_par)) gave_up = 1;
+        s_par ^= 1;
+        if (__any_sync(0xffffffffu, gave_up)) {
+          ok = false;
+          break;
+        }
+        if (warp_on) {
+          fence_after();
+          uint32_t x[KT];
+#pragma unroll
+          for (int c = 0; c < KT; c += 32) tmem_ld32_nowait(tS + c, x + c);
+          tmem_wait();
+#pragma unroll
+          for (int c = 0; c < KT; c += 32) pin32(x + c);
+          if (key0 + KT - 1 > pos_lo || dead) {
+            const int lim = pos - key0;
+#pragma unroll
+            for (int c = 0; c < KT; c++)
+              if (c > lim || ((dead >> (c >> 3)) & 1)) x[c] = 0xff800000u;  // -inf
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < KT; c += 4)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx[j] = fmaxf(mx[j], __uint_as_float(x[c + j]));
+          const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+          if (cu.kt == kt0) {
+            m = mn;  // O is overwritten by the first product
+          } else {
+            const bool grow = mn > m + 8.0f;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? exp2_fast(m - mn) : 1.0f;
+              if (grow) m = mn;
+              l *= f;
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                tmem_ld32_nowait(tO + c, o);
+                tmem_wait();
+                pin32(o);
+#pragma unroll
+                for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tmem_st32(tO + c, o);
+              }
+              tmem_st_wait();
+            }
+          }
+          const float mz = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KT; c += 32) {
+            uint32_t p[NT][16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float e0 = exp2_fast(fmaf(__uint_as_float(x[c + j]), c2, -mz));
+              const float e1 = exp2_fast(fmaf(__uint_as_float(x[c + j + 1]), c2, -mz));
+              sum[j & 2] += e0;
+              sum[(j & 2) + 1] += e1;
+              uint32_t t[NT];
+              split_bf2<NT>(e0, e1, t);
+#pragma unroll
+              for (int k = 0; k < NT; k++) p[k][j >> 1] = t[k];
+            }
+#pragma unroll
+            for (int k = 0; k < NT; k++) tmem_st16(tS + k * (KT / 2) + (c >> 1), p[k]);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+          fence_before();
+        }
+        mbar_arrive(&bars.p_full[s]);
+
+        if (last) {
+          const bool whole = ends && kt0 == 0;
+          const int slot = 2 * blockIdx.x + (kt0 == 0 ? 1 : 0);
+          if (!whole && s == 0 && row == 0) {
+            AttnPart d;
+            d.kind = kt0 == 0 ? kPartStart : (ends ? kPartEnd : kPartMiddle);
+            d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
+            a.parts[slot] = d;
+          }
+          if (!mbar_wait(&bars.o_full[s], o_par)) gave_up = 1;
+          o_par ^= 1;
+          if (__any_sync(0xffffffffu, gave_up)) {
+            ok = false;
+            break;
+          }
+          if (warp_on) {
+            fence_after();
+            const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+            const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD;
+            const long pr = (long)slot * a.tile_rows + s * 128 + row;
+            if (!whole && mine) a.ml[pr] = make_float2(m, l);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32_nowait(tO + c, o);
+              tmem_wait();
+              pin32(o);
+              if (mine) {
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = l == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
+                if (whole && !QF) {
+                  uint16_t* w = static_cast<uint16_t*>(a.p.out) + at + c;
+#pragma unroll
+                  for (int j = 0; j < 32; j += 8)
+                    *reinterpret_cast<uint4*>(w + j) = make_uint4(pack_bf2(v[j], v[j + 1]), pack_bf2(v[j + 2], v[j + 3]),
+                                                                  pack_bf2(v[j + 4], v[j + 5]), pack_bf2(v[j + 6], v[j + 7]));
+                } else {
+                  float* w = whole ? static_cast<float*>(a.p.out) + at + c : a.acc + pr * HD + c;
+#pragma unroll
+                  for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                }
+              }
+            }
+            fence_before();
+          }
+        }
+      }
+      if (last) fresh = true;
+      if (u + 1 < units) cu.next<R, KT>(a);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// The pool as a 4D map, boxes of 64 dims x `box` slots: the head's dims, then
+// slot, head and page by ascending stride, as a map wants them.  order: what
+// dimensions 1, 2 and 3 are (0 slot, 1 head, 2 page), two bits each.
+bool pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, int box, int* order) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  struct Dim {
+    int64_t stride;
+    int size, box, what;
+  } d[3] = {{kv.token_stride, kv.page_size, box, 0}, {kv.head_stride, kv.n_kv_heads, 1, 1}, {kv.page_stride, kv.n_pages, 1, 2}};
+  std::stable_sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim}, strides[3];
+  cuuint32_t boxes[4] = {64}, estr[4] = {1, 1, 1, 1};
+  *order = 0;
+  for (int i = 0; i < 3; i++) {
+    dims[i + 1] = (cuuint64_t)d[i].size;
+    strides[i] = (cuuint64_t)d[i].stride * 2;
+    boxes[i + 1] = (cuuint32_t)d[i].box;
+    *order |= d[i].what << (2 * i);
+  }
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool QF, int HD>
+cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
+  using S = TcShape<QF, HD>;
+  static SmemOptIn opt;
+  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_tc_kernel<QF, HD>), S::SMEM));
+  const int box = std::min(a.p.kv.page_size, S::KT);
+  CUtensorMap mk, mv;
+  int order = 0;
+  if (!pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
+  return launch_k(paged_attn_tc_kernel<QF, HD>, dim3(a.ctas), dim3(kTcThreads), S::SMEM, s, mk, mv, a, box, order);
+}
+
+}  // namespace
+
+PagedAttnTc paged_attn_tc_plan(const ctts_paged_attn& p) {
+  PagedAttnTc t;
+  t.ctas = device_sms();
+  t.tile_rows = p.q_dtype == CTTS_F32 && p.kv.head_dim == 128 ? 128 : 256;
+  return t;
+}
+
+cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, cudaStream_t s) {
+  const bool qf = a.p.q_dtype == CTTS_F32;
+  if (a.p.kv.head_dim == 64) return qf ? launch_tc<true, 64>(a, s) : launch_tc<false, 64>(a, s);
+  return qf ? launch_tc<true, 128>(a, s) : launch_tc<false, 128>(a, s);
+}
+
+}  // namespace ctts
