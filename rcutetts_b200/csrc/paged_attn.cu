@@ -14,6 +14,7 @@
 // once.  Which CTA does what follows from the lengths on the device alone, so
 // the host knows no lengths and a captured call follows them.
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "launch_state.h"
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
 
   attn_find_start<R, kKeys, kNT>(a, &start);
   const long units = start.units;
-  if (tid < 2) a.parts[2 * blockIdx.x + tid].kind = 0;  // no partial state yet
+  if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   if (units == 0) return;
   AttnCursor ld = AttnCursor::at<R, kKeys>(a, start), cu = ld;
   long to_load = units;
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
   for (int i = 0; i < NS - 1; i++) issue();
 
-  const float c2 = a.p.scale * 1.44269504088896340736f;  // scores in powers of two
+  const float c2 = a.c2_hi;
   float o[NO][4], m2[2], l2[2];
   bool fresh = true;  // the unit begins a piece
   int unit0_kt = 0;   // the piece's first key tile
@@ -204,9 +205,14 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
     const int plast = wrow < nrows ? pos0 + (row_base + min(nrows, wrow + 16) - 1) / a.group : -1;
     if (key0 <= plast) {
       const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + kKeys * S::KROW;
-      float s[KT][4];
+      // The tensor core cuts what it adds to the accumulator's precision, so
+      // the small products of a float32 call (all but the leading terms') are
+      // summed apart and added once.
+      float s[KT][4], lo[QF ? KT : 1][4];
 #pragma unroll
       for (int j = 0; j < KT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < (QF ? KT : 1); j++) lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
         uint32_t qa[S::NQ][4];
@@ -222,10 +228,9 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
             split_bf2<3>(y.x, y.y, b1);
             // products of terms whose orders add up to less than 2^-24 of the whole are left out
 #pragma unroll
-            for (int k = 0; k < S::NQ; k++)
+            for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-              for (int n = 0; n < 3; n++)
-                if (k + n <= 2) mma_16816(s[j], qa[k], b0[n], b1[n]);
+              for (int k = 0; k <= sum; k++) mma_16816(sum ? lo[QF ? j : 0] : s[j], qa[QF ? k : 0], b0[sum - k], b1[sum - k]);
           }
         } else {
 #pragma unroll
@@ -234,12 +239,18 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
             uint32_t kb[4];
             ldsm4(kt_s + sw(wkey + 8 * j + 8 * (mi >> 1) + (lane & 7), 2 * ks + (mi & 1)), kb);
 #pragma unroll
-            for (int k = 0; k < S::NQ; k++) {
-              mma_16816(s[j], qa[k], kb[0], kb[1]);
-              mma_16816(s[j + 1], qa[k], kb[2], kb[3]);
+            for (int k = S::NQ - 1; k >= 0; k--) {
+              mma_16816(k ? lo[QF ? j : 0] : s[j], qa[k], kb[0], kb[1]);
+              mma_16816(k ? lo[QF ? j + 1 : 0] : s[j + 1], qa[k], kb[2], kb[3]);
             }
           }
         }
+      }
+      if (QF) {
+#pragma unroll
+        for (int j = 0; j < KT; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[j][e] += lo[QF ? j : 0][e];
       }
       // causal mask and missing pages; a tile that every row sees whole needs none
       const int pfirst = pos0 + (row_base + wrow) / a.group;
@@ -268,8 +279,8 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < KT; j++) {
-          s[j][2 * e] = exp2_fast(fmaf(s[j][2 * e], c2, -mm[e]));
-          s[j][2 * e + 1] = exp2_fast(fmaf(s[j][2 * e + 1], c2, -mm[e]));
+          s[j][2 * e] = exp2_fast(attn_arg<QF>(a, s[j][2 * e], mm[e]));
+          s[j][2 * e + 1] = exp2_fast(attn_arg<QF>(a, s[j][2 * e + 1], mm[e]));
           sum += s[j][2 * e] + s[j][2 * e + 1];
         }
         l2[e] = l2[e] * f[e] + sum;  // this thread's share of the row sum
@@ -291,6 +302,8 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
           for (int k = 0; k < S::NP; k++) pa[k][i] = t[k];
         }
+        // float32 calls: 16 keys at a time in an accumulator of their own,
+        // small products first, added to the output in float32
         if (KF) {
 #pragma unroll
           for (int t = 0; t < NO; t++) {
@@ -300,11 +313,13 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
             uint32_t b0[3], b1[3];
             split_bf2<3>(vp[0], vp[LD], b0);
             split_bf2<3>(vp[8 * LD], vp[9 * LD], b1);
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < S::NP; k++)
+            for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-              for (int n = 0; n < 3; n++)
-                if (k + n <= 2) mma_16816(o[t], pa[k], b0[n], b1[n]);
+              for (int k = 0; k <= sum; k++) mma_16816(x, pa[QF ? k : 0], b0[sum - k], b1[sum - k]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[t][e] += x[e];
           }
         } else {
 #pragma unroll
@@ -312,10 +327,21 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
             // matrices: (keys 0-7, dims 8t..), (keys 8-15, 8t..), (keys 0-7, 8t+8..), (keys 8-15, 8t+8..)
             uint32_t vb[4];
             ldsm4_t(vt_s + sw(wkey + 8 * j + 8 * (mi & 1) + (lane & 7), t + (mi >> 1)), vb);
+            if (QF) {
+              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < S::NP; k++) {
-              mma_16816(o[t], pa[k], vb[0], vb[1]);
-              mma_16816(o[t + 1], pa[k], vb[2], vb[3]);
+              for (int k = S::NP - 1; k >= 0; k--) {
+                mma_16816(x, pa[k], vb[0], vb[1]);
+                mma_16816(y, pa[k], vb[2], vb[3]);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                o[t][e] += x[e];
+                o[t + 1][e] += y[e];
+              }
+            } else {
+              mma_16816(o[t], pa[0], vb[0], vb[1]);
+              mma_16816(o[t + 1], pa[0], vb[2], vb[3]);
             }
           }
         }
@@ -330,11 +356,11 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       const int slot = 2 * blockIdx.x + (unit0_kt == 0 ? 1 : 0);
       float2* const pml = a.ml + (long)slot * a.tile_rows;
       float* const part = a.acc + (long)slot * a.tile_rows * HD;
-      if (!whole && tid == 0) {
+      if (!ends && unit0_kt == 0 && tid == 0) {
         AttnPart d;
-        d.kind = unit0_kt == 0 ? kPartStart : (ends ? kPartEnd : kPartMiddle);
+        d.pieces = attn_pieces(a, start, cu.nt - 1 - cu.kt);
         d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
-        a.parts[slot] = d;
+        a.parts[blockIdx.x] = d;
       }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
@@ -413,81 +439,79 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
   }
 }
 
-// Merges the pieces of the items that cuts divide: block (c, y) takes rows y,
-// y + gridDim.y, ... of the item that begins in CTA c and runs into CTA c + 1
-// and on, if there is one.  The weights of the pieces are computed once per
-// row; 256 threads = HD/4 columns of four x pieces in parallel, summed in a
-// fixed order.
-constexpr int kJoinThreads = 256, kJoinMax = 1024;
+// Merges the pieces of the items that cuts divide: the blocks (c, *) take the
+// item that leaves CTA c, if there is one.  HD/4 lanes hold a row (four
+// columns each).  Few pieces (chunks; the usual case): each group of lanes
+// takes a row of its own and walks its pieces.  Many (one long request): the
+// block takes a row at a time, its groups share the pieces, and their states
+// merge in shared memory in group order.
+constexpr int kJoinThreads = 256;
 template <bool BF, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PagedAttnArgs a) {
-  constexpr int COLS = HD / 2, GR = kJoinThreads / COLS;
-  __shared__ float wgt[kJoinMax];
-  __shared__ float red[kJoinThreads / 32];
-  __shared__ float2 acc[GR][COLS];
-  __shared__ int last;
-  const int tid = threadIdx.x, c = blockIdx.x;
+  constexpr int COLS = HD / 4, G = kJoinThreads / COLS, FEW = 8;
+  __shared__ float4 gv[G][COLS];
+  __shared__ float2 gml[G];
+  const int tid = threadIdx.x, c = blockIdx.x, col = tid % COLS, grp = tid / COLS;
   grid_dep_enter();
-  const AttnPart d = a.parts[2 * c + 1];
-  if (d.kind != kPartStart) return;
-  if (tid == 0) last = a.ctas;
-  __syncthreads();
-  // pieces: CTA c's second place, then the first places of c + 1, ... up to the one that ends the item
-  for (int k = c + 1 + tid; k < a.ctas; k += kJoinThreads) {
-    if (a.parts[2 * k].kind != kPartMiddle) atomicMin(&last, k);
-    if (last <= k) break;
-  }
-  __syncthreads();
-  const int n = min(last - c + 1, a.ctas - c);  // pieces
-  auto piece = [&](int i, int r) { return (long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.tile_rows + r; };
-  for (int r = blockIdx.y; r < d.rows; r += gridDim.y) {
-    float mx = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, a.ml[piece(i, r)].x);
-    mx = warp_max(mx);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; w++) mx = fmaxf(mx, red[w]);
-    if (mx == -INFINITY) mx = 0.0f;
-    float l = 0.0f;
-    for (int i = tid; i < n; i += kJoinThreads) {
-      const float2 ml = a.ml[piece(i, r)];
-      wgt[i] = exp2_fast(ml.x - mx);
-      l = fmaf(ml.y, wgt[i], l);
-    }
-    l = warp_sum(l);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = l;
-    const int col = tid % COLS, g = tid / COLS;
-    __syncthreads();
-    float2 s = make_float2(0.0f, 0.0f);
+  const AttnPart d = a.parts[c];
+  if (d.pieces == 0) return;
+  const bool shared_row = d.pieces > FEW;
+  const int i0 = shared_row ? grp : 0, di = shared_row ? G : 1;
+  const int rows_at_once = shared_row ? 1 : G;
+  for (int base = blockIdx.y * rows_at_once; base < d.rows; base += gridDim.y * rows_at_once) {
+    const int r = base + (shared_row ? 0 : grp);
+    const bool on = r < d.rows;
+    float m = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
 #pragma unroll 4
-    for (int i = g; i < n; i += GR) {
-      const float2 v = *reinterpret_cast<const float2*>(a.acc + piece(i, r) * HD + 2 * col);
-      s.x = fmaf(v.x, wgt[i], s.x);
-      s.y = fmaf(v.y, wgt[i], s.y);
-    }
-    acc[g][col] = s;
-    __syncthreads();
-    if (g == 0) {
-      float L = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kJoinThreads / 32; w++) L += red[w];
-#pragma unroll
-      for (int k = 1; k < GR; k++) {
-        s.x += acc[k][col].x;
-        s.y += acc[k][col].y;
+      for (int i = i0; i < d.pieces; i += di) {
+        const long at = (long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.tile_rows + r;
+        const float2 ml = a.ml[at];
+        const float4 w = *reinterpret_cast<const float4*>(a.acc + at * HD + 4 * col);
+        const float mn = fmaxf(m, ml.x), mz = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2_fast(m - mz), g = exp2_fast(ml.x - mz);
+        m = mn;
+        l = fmaf(ml.y, g, l * f);
+        v.x = fmaf(w.x, g, v.x * f);
+        v.y = fmaf(w.y, g, v.y * f);
+        v.z = fmaf(w.z, g, v.z * f);
+        v.w = fmaf(w.w, g, v.w * f);
       }
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const int pk = d.packed0 + r;
-      const long at = (long)(d.row0 + pk / a.group) * a.p.out_ld + (long)(d.h * a.group + pk % a.group) * HD + 2 * col;
-      if (BF)
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at) = pack_bf2(s.x * inv, s.y * inv);
-      else
-        *reinterpret_cast<float2*>(static_cast<float*>(a.p.out) + at) = make_float2(s.x * inv, s.y * inv);
     }
-    __syncthreads();
+    if (shared_row) {
+      gv[grp][col] = v;
+      if (col == 0) gml[grp] = make_float2(m, l);
+      __syncthreads();
+      if (grp == 0) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < G; k++) M = fmaxf(M, gml[k].x);
+        if (M == -INFINITY) M = 0.0f;
+        l = 0.0f;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < G; k++) {
+          const float g = exp2_fast(gml[k].x - M);
+          const float4 w = gv[k][col];
+          l = fmaf(gml[k].y, g, l);
+          v.x = fmaf(w.x, g, v.x);
+          v.y = fmaf(w.y, g, v.y);
+          v.z = fmaf(w.z, g, v.z);
+          v.w = fmaf(w.w, g, v.w);
+        }
+      }
+      __syncthreads();
+    }
+    if (on && (!shared_row || grp == 0)) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int pk = d.packed0 + r;
+      const long at = (long)(d.row0 + pk / a.group) * a.p.out_ld + (long)(d.h * a.group + pk % a.group) * HD + 4 * col;
+      if (BF)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.p.out) + at) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+      else
+        *reinterpret_cast<float4*>(static_cast<float*>(a.p.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    }
   }
 }
 
@@ -547,11 +571,11 @@ PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
   } else with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
     constexpr bool QF = decltype(q)::value, KF = decltype(k)::value, CH = decltype(ch)::value;
     constexpr int HD = decltype(hd)::value;
-    pl.ctas = std::min(kJoinMax, attn_ctas<QF, KF, HD, CH>(rows_used_of(p)));
+    pl.ctas = attn_ctas<QF, KF, HD, CH>(rows_used_of(p));
     pl.tile_rows = Shape<QF, KF, HD, CH>::R;
     return 0;
   });
-  pl.ws_bytes = (size_t)2 * pl.ctas * (sizeof(AttnPart) + (size_t)pl.tile_rows * (p.kv.head_dim + 2) * sizeof(float));
+  pl.ws_bytes = pl.ctas * (sizeof(AttnPart) + (size_t)2 * pl.tile_rows * (p.kv.head_dim + 2) * sizeof(float));
   return pl;
 }
 
@@ -565,8 +589,13 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   a.ctas = pl.ctas;
   a.tile_rows = pl.tile_rows;
   a.rows_used = rows_used_of(p);
+  const double c2 = (double)p.scale * 1.4426950408889634;
+  a.c2_hi = (float)c2;
+  // the first part below the factor, so that the second is positive: -inf times either is -inf
+  if ((double)a.c2_hi >= c2) a.c2_hi = std::nextafter(a.c2_hi, 0.0f);
+  a.c2_lo = (float)(c2 - (double)a.c2_hi);
   a.parts = static_cast<AttnPart*>(p.workspace);
-  a.acc = reinterpret_cast<float*>(a.parts + 2 * pl.ctas);
+  a.acc = reinterpret_cast<float*>(a.parts + pl.ctas);
   a.ml = reinterpret_cast<float2*>(a.acc + (size_t)2 * pl.ctas * pl.tile_rows * p.kv.head_dim);
   if (use_tc(p))
     CTTS_LK(launch_paged_attn_tc(a, s));
@@ -575,7 +604,7 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
       return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value>(a, s);
     }));
   const int rows = (int)std::min((long)a.tile_rows, (long)p.max_new * a.group);
-  const dim3 grid(a.ctas, std::min(rows, 16)), block(kJoinThreads);
+  const dim3 grid(a.ctas, rows > 16 ? 16 : std::min(rows, 4)), block(kJoinThreads);
   const bool bf = p.q_dtype == CTTS_BF16;
   if (p.kv.head_dim == 64)
     return bf ? launch_k(paged_attn_join_kernel<true, 64>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 64>, grid, block, 0, s, a);

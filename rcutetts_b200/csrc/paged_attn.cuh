@@ -9,13 +9,13 @@
 
 namespace ctts {
 
-// A partial state in the workspace.  CTA c has two places: 2c for a piece
-// that enters it (middle or end of an item), 2c + 1 for one that begins in it
-// and leaves it.
-constexpr int kPartStart = 1, kPartMiddle = 2, kPartEnd = 3;
+// Partial states in the workspace: CTA c has two places, 2c for a piece that
+// enters it (the middle or the end of an item) and 2c + 1 for one that begins
+// in it and leaves it.  An item that leaves CTA c is described by parts[c]:
+// its pieces lie in places 2c + 1, 2(c + 1), 2(c + 2), ...
 struct AttnPart {
-  int kind = 0;  // 0: none
-  int row0 = 0;  // the request's first row of q
+  int pieces = 0;  // 0: no item leaves this CTA
+  int row0 = 0;    // the request's first row of q
   int packed0 = 0, rows = 0, h = 0;  // first packed row, packed rows, KV head
   int pad[3] = {0, 0, 0};
 };
@@ -25,7 +25,8 @@ struct PagedAttnArgs {
   int group = 1, shift = 0;      // query heads per KV head, log2 of the page size
   int ctas = 0, tile_rows = 0;   // CTAs, packed rows per item
   int rows_used = 0;             // packed rows an item can have
-  AttnPart* parts = nullptr;     // [2 * ctas]
+  float c2_hi = 0, c2_lo = 0;    // scale * log2(e): scores in powers of two
+  AttnPart* parts = nullptr;     // [ctas]
   float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum (in powers of two), sum
   float* acc = nullptr;          // [2 * ctas][tile_rows][hd]: unnormalised output
 };
@@ -55,6 +56,14 @@ CTTS_DEV float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// score s and maximum m (in powers of two) to the exponential's argument; a
+// float32 call takes the factor in two parts, or its rounding would cost
+// 2^-24 of the argument
+template <bool QF>
+CTTS_DEV float attn_arg(const PagedAttnArgs& a, float s, float m) {
+  return QF ? fmaf(s, a.c2_hi, fmaf(s, a.c2_lo, -m)) : fmaf(s, a.c2_hi, -m);
 }
 
 // A request's lengths, cut to what the buffers hold.
@@ -88,6 +97,7 @@ CTTS_DEV long attn_units(const PagedAttnArgs& a, int b) {
 
 struct AttnStart {
   long units;  // this CTA's
+  long end, total;  // where they end on the line, and its length
   long skip;   // units of request b ahead of them
   int b;
 };
@@ -136,6 +146,8 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
   const long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
   if (tid == 0) {
     out->units = u1 - u0;
+    out->end = u1;
+    out->total = total;
     out->b = 0;
     out->skip = 0;
   }
@@ -156,6 +168,13 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
     if (first > u0) break;
   }
   __syncthreads();
+}
+
+// CTAs from this one to the one that holds tile `more` behind this CTA's end
+// (unit e lies in the last CTA c with total * c / ctas <= e).
+CTTS_DEV int attn_pieces(const PagedAttnArgs& a, const AttnStart& s, int more) {
+  const long ctas = min((long)a.ctas, s.total), e = s.end + more - 1;
+  return (int)(((e + 1) * ctas + s.total - 1) / s.total) - (int)blockIdx.x;
 }
 
 // A place on the line: request, row tile, KV head, key tile.
