@@ -26,7 +26,7 @@ namespace ctts {
 namespace {
 
 constexpr int kKeys = 64;  // keys per tile
-constexpr int kNT = 128;   // threads
+constexpr int kNT = 128;   // threads that compute; a warp behind them issues the copies
 
 CTTS_DEV void mma_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -43,122 +43,129 @@ CTTS_DEV void ldsm4_t(uint32_t addr, uint32_t* r) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// 16 bytes to shared memory, zeros when `bytes` is 0
-CTTS_DEV void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-CTTS_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-CTTS_DEV void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // One kernel shape.  CHUNK = false: 16 packed rows per item (single tokens and
 // short runs), the four warps share the rows and split each key tile, 16 keys
-// each, with their own softmax states.  CHUNK = true: 64 packed rows, 16 per
-// warp, every warp takes all keys.
-template <bool QF, bool KF, int HD, bool CHUNK>
+// each, with their own softmax states; RH = 1 when no item has more than 8
+// rows (the upper half of the MMA's rows stays zero and unread).  CHUNK =
+// true: 64 packed rows, 16 per warp, every warp takes all keys.
+template <bool QF, bool KF, int HD, bool CHUNK, int RH>
 struct Shape {
-  static constexpr int R = CHUNK ? 64 : 16;
+  static constexpr int R = CHUNK ? 64 : 8 * RH;
+  static constexpr int RQ = CHUNK ? 64 : 16;  // query rows held
   // bf16 terms of a float32 operand (queries and softmax weights; keys and
   // values of a float32 cache): 24 bits, so a float32 call keeps float32
   static constexpr int NQ = QF ? 3 : 1;
   static constexpr int NP = QF ? 3 : 1;
   static constexpr int ES = KF ? 4 : 2;
-  static constexpr int ROWB = HD * ES;
-  // float32 rows are padded so that the fragment reads (8 keys x 8 bytes of K,
-  // 8 keys x 8 words of V) fall in distinct banks; bf16 rows are swizzled
-  static constexpr int KROW = ROWB + (KF ? 32 : 0), VROW = ROWB + (KF ? 16 : 0);
-  static constexpr int STAGE = kKeys * (KROW + VROW);
-  // stages: 48 KB in flight per CTA or more
-  static constexpr int NS = STAGE <= 16384 ? 4 : (STAGE <= 36864 ? 3 : 2);
-  static constexpr int QBYTES = NQ * R * HD * 2;
+  static constexpr int NB = HD * ES / 128;           // 128-byte blocks of a row
+  static constexpr uint32_t TILE = NB * kKeys * 128;  // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
+  static constexpr uint32_t STAGE = 2 * TILE;
+  static constexpr int NS = STAGE <= 16384 ? 4 : (STAGE <= 32768 ? 3 : 2);
+  static constexpr int QBYTES = NQ * RQ * HD * 2;
   static constexpr int KT = CHUNK ? 8 : 2;  // 8-key column tiles per warp and key tile
   static size_t smem(int rows_used) {
-    return (size_t)NS * STAGE + QBYTES + (CHUNK ? 0 : (size_t)4 * rows_used * (HD + 2) * 4);
+    return 1024 + (size_t)NS * STAGE + QBYTES + (CHUNK ? 0 : (size_t)4 * rows_used * (HD + 2) * 4);
   }
 };
 
-template <bool QF, bool KF, int HD, bool CHUNK>
-__global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) {
-  using S = Shape<QF, KF, HD, CHUNK>;
+template <bool QF, bool KF, int HD, bool CHUNK, int RH>
+__global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                                                              const __grid_constant__ PagedAttnArgs a, int box, int order) {
+  using S = Shape<QF, KF, HD, CHUNK, RH>;
   constexpr int R = S::R, KT = S::KT, NO = HD / 8, KS = HD / 16, NS = S::NS;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
   __shared__ AttnStart start;
-  __shared__ uint8_t dead[NS][8];  // 8-key groups of a stage whose page does not exist
-  const uint32_t sbase = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ uint32_t dead_keys[NS];  // 8-key groups of a stage whose page does not exist
+  __shared__ volatile int gave_up;
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (sbase - smem_u32(smem_raw));
   const uint32_t qbase = sbase + NS * S::STAGE;
   float* const wst = reinterpret_cast<float*>(smem + NS * S::STAGE + S::QBYTES);  // [warp][row][HD + 2]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tq = lane & 3, mi = lane >> 3;
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    gave_up = 0;
+  }
   grid_dep_enter();
-
-  attn_find_start<R, kKeys, kNT>(a, &start);
+  attn_find_start<R, kKeys, kNT + 32>(a, &start);
   const long units = start.units;
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   if (units == 0) return;
-  AttnCursor ld = AttnCursor::at<R, kKeys>(a, start), cu = ld;
-  long to_load = units;
+  AttnCursor cu = AttnCursor::at<R, kKeys>(a, start);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // (after one that gave up nobody waits: the block runs to its end)
+    if (!gave_up && !mbar_wait(bar, parity)) gave_up = 1;
+  };
+
+  if (warp == 4) {
+    // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile; the
+    // lanes at the boxes' starts copy them.  Pages that do not exist are
+    // outside the map and arrive as zeros.
+    auto page_of = [&]() {
+      const int kk = cu.kt * kKeys + 8 * lane;
+      return lane < 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
+    };
+    int page = page_of();
+    for (long u = 0; u < units; u++) {
+      const int st = (int)(u % NS), kk = cu.kt * kKeys + 8 * lane, h = cu.h;
+      const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
+      const uint32_t dead = __ballot_sync(0xffffffffu, lane < 8 && kk < cu.len && none);
+      const int mine = none ? a.p.kv.n_pages : page;
+      if (u + 1 < units) {  // the next tile's pages, over the wait
+        cu.next<R, kKeys>(a);
+        page = page_of();
+      }
+      if (u >= NS) wait(&empty[st], (uint32_t)((u / NS) & 1) ^ 1);
+      if (__any_sync(0xffffffffu, gave_up)) break;
+      if (lane == 0) {
+        dead_keys[st] = dead;
+        mbar_expect_tx(&full[st], S::STAGE);
+      }
+      __syncwarp();
+      if (lane < 8 && (8 * lane & (box - 1)) == 0) {
+        const uint32_t dst = sbase + st * S::STAGE + (uint32_t)lane * 1024u;
+        const int slot = kk & (a.p.kv.page_size - 1);
+#pragma unroll
+        for (int b = 0; b < S::NB; b++) {
+          copy_box(dst + b * kKeys * 128, &tmK, order, b * (128 / S::ES), slot, h, mine, &full[st]);
+          copy_box(dst + S::TILE + b * kKeys * 128, &tmV, order, b * (128 / S::ES), slot, h, mine, &full[st]);
+        }
+      }
+    }
+    if (gave_up)  // copies in flight land before the block may leave
+      for (int i = 0; i < NS; i++) {
+        mbar_wait(&full[i], 0);
+        mbar_wait(&full[i], 1);
+      }
+    return;
+  }
+  auto sync_rows = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // the four computing warps
 
   auto q_addr = [&](int term, int row, int chunk) {  // 16-byte chunk of a query row, swizzled
-    return qbase + (uint32_t)(term * R + row) * (HD * 2) + (uint32_t)((chunk & ~7) | ((chunk ^ row) & 7)) * 16u;
+    return qbase + (uint32_t)(term * S::RQ + row) * (HD * 2) + (uint32_t)((chunk & ~7) | ((chunk ^ row) & 7)) * 16u;
   };
-  auto sw = [&](int key, int chunk) { return (uint32_t)key * (HD * 2) + (uint32_t)((chunk & ~7) | ((chunk ^ key) & 7)) * 16u; };
-
-  int ld_buf = 0;
-  auto issue = [&]() {  // the next unit's K and V rows into stage ld_buf (an empty group when there is none)
-    if (to_load > 0) {
-      constexpr int CH = S::ROWB / 16;  // chunks per row
-      const int* tab = a.p.block_tables + (long)ld.b * a.p.table_ld;
-      const int key0 = ld.kt * kKeys;
-      const uint32_t kd = sbase + ld_buf * S::STAGE, vd = kd + kKeys * S::KROW;
-#pragma unroll
-      for (int i = 0; i < kKeys * CH / kNT; i++) {
-        const int c = tid + i * kNT, key = c / CH, ch = c % CH;
-        const int kk = key0 + key;
-        long off = 0;
-        bool ok = kk < ld.len;
-        if (ok) {
-          const int page = tab[kk >> a.shift];
-          ok = (unsigned)page < (unsigned)a.p.kv.n_pages;
-          if (ok)
-            off = ((long)page * a.p.kv.page_stride + (long)(kk & (a.p.kv.page_size - 1)) * a.p.kv.token_stride +
-                   (long)ld.h * a.p.kv.head_stride) * S::ES + ch * 16;
-        }
-        const uint32_t dk = KF ? (uint32_t)key * S::KROW + ch * 16u : sw(key, ch);
-        const uint32_t dv = KF ? (uint32_t)key * S::VROW + ch * 16u : dk;
-        cp_async16(kd + dk, static_cast<const uint8_t*>(a.p.kv.k) + off, ok ? 16 : 0);
-        cp_async16(vd + dv, static_cast<const uint8_t*>(a.p.kv.v) + off, ok ? 16 : 0);
-      }
-      if (tid < 8) {
-        const int kk = key0 + tid * 8;
-        dead[ld_buf][tid] = kk < ld.len && (unsigned)tab[kk >> a.shift] >= (unsigned)a.p.kv.n_pages;
-      }
-      if (--to_load > 0) ld.next<R, kKeys>(a);
-    }
-    cp_commit();
-    ld_buf = ld_buf + 1 == NS ? 0 : ld_buf + 1;
-  };
-#pragma unroll
-  for (int i = 0; i < NS - 1; i++) issue();
-
+  // 16-byte chunk of a key's row in a tile
+  auto sw = [](int key, int chunk) { return (uint32_t)(chunk >> 3) * (kKeys * 128) + (uint32_t)key * 128 + (uint32_t)((chunk ^ key) & 7) * 16u; };
   const float c2 = a.c2_hi;
   float o[NO][4], m2[2], l2[2];
   bool fresh = true;  // the unit begins a piece
   int unit0_kt = 0;   // the piece's first key tile
   int buf = 0;
   for (long u = 0; u < units; u++) {
-    cp_wait<NS - 2>();
-    __syncthreads();  // the stage has landed for everyone; the one before is consumed
-    issue();
     const int row_base = cu.m * R;               // first packed row of the tile
     const int nrows = min(R, cu.nn * a.group - row_base);
     const int pos0 = cu.len - cu.cnt;            // position of the request's first new row
     if (fresh) {
       unit0_kt = cu.kt;
+      if (CHUNK) sync_rows();  // the queries of the item before are read (short runs: their merge has synchronised)
       // queries of the tile as bf16 terms; rows behind nrows are zero
       constexpr int CH = HD / 8;
-      for (int i = tid; i < R * CH; i += kNT) {
+      for (int i = tid; i < S::RQ * CH; i += kNT) {
         const int r = i / CH, ch = i % CH;
         float v[8];
 #pragma unroll
@@ -189,7 +196,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       for (int t = 0; t < NO; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
       m2[0] = m2[1] = -INFINITY;
       l2[0] = l2[1] = 0.0f;
-      __syncthreads();
+      sync_rows();
       fresh = false;
     }
     const int wrow = CHUNK ? warp * 16 : 0;      // the warp's rows and keys
@@ -202,9 +209,21 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       const int r = wrow + gq + 8 * e;
       pr[e] = r < nrows ? pos0 + (row_base + r) / a.group : -1;
     }
+    wait(&full[buf], (uint32_t)((u / NS) & 1));
     const int plast = wrow < nrows ? pos0 + (row_base + min(nrows, wrow + 16) - 1) / a.group : -1;
     if (key0 <= plast) {
-      const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + kKeys * S::KROW;
+      const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + S::TILE;
+      const uint8_t* const kt_p = smem + buf * S::STAGE;
+      const bool tail = key0 + 8 * KT > cu.len;  // slots behind the length: their values may be anything, and 0 * NaN is NaN
+      if (!KF && tail) {
+        for (int i = lane; i < 8 * KT * (HD / 8); i += 32) {
+          const int key = wkey + i / (HD / 8);
+          if (cu.kt * kKeys + key >= cu.len)
+            *reinterpret_cast<uint4*>(smem + buf * S::STAGE + S::TILE + sw(key, i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+        fence_async();  // before the next copy into the stage
+      }
       // The tensor core cuts what it adds to the accumulator's precision, so
       // the small products of a float32 call (all but the leading terms') are
       // summed apart and added once.
@@ -221,8 +240,9 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
         if (KF) {
 #pragma unroll
           for (int j = 0; j < KT; j++) {
-            const uint8_t* kp = smem + buf * S::STAGE + (wkey + 8 * j + gq) * S::KROW + (ks * 16 + 2 * tq) * 4;
-            const float2 x = *reinterpret_cast<const float2*>(kp), y = *reinterpret_cast<const float2*>(kp + 32);
+            const int key = wkey + 8 * j + gq, ch = 4 * ks + (tq >> 1);
+            const float2 x = *reinterpret_cast<const float2*>(kt_p + sw(key, ch) + (tq & 1) * 8);
+            const float2 y = *reinterpret_cast<const float2*>(kt_p + sw(key, ch + 2) + (tq & 1) * 8);
             uint32_t b0[3], b1[3];
             split_bf2<3>(x.x, x.y, b0);
             split_bf2<3>(y.x, y.y, b1);
@@ -250,23 +270,21 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
         for (int j = 0; j < KT; j++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[j][e] += lo[QF ? j : 0][e];
+          for (int e = 0; e < 2 * RH; e++) s[j][e] += lo[QF ? j : 0][e];
       }
       // causal mask and missing pages; a tile that every row sees whole needs none
       const int pfirst = pos0 + (row_base + wrow) / a.group;
-      uint32_t gone = 0;
-#pragma unroll
-      for (int j = 0; j < KT; j++) gone |= (uint32_t)(dead[buf][(wkey >> 3) + j] != 0) << j;
+      const uint32_t gone = (dead_keys[buf] >> (wkey >> 3)) & ((1u << KT) - 1);
       if (key0 + 8 * KT - 1 > pfirst || gone) {
 #pragma unroll
         for (int j = 0; j < KT; j++)
 #pragma unroll
-          for (int e = 0; e < 4; e++)
+          for (int e = 0; e < 2 * RH; e++)
             if (key0 + 8 * j + 2 * tq + (e & 1) > pr[e >> 1] || ((gone >> j) & 1)) s[j][e] = -INFINITY;
       }
-      float f[2], mm[2];
+      float f[2] = {0.0f, 0.0f}, mm[2];
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
+      for (int e = 0; e < RH; e++) {
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < KT; j++) mx = fmaxf(mx, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
@@ -289,16 +307,18 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       for (int t = 0; t < NO; t++) {
         o[t][0] *= f[0];
         o[t][1] *= f[0];
-        o[t][2] *= f[1];
-        o[t][3] *= f[1];
+        if (RH == 2) {
+          o[t][2] *= f[1];
+          o[t][3] *= f[1];
+        }
       }
 #pragma unroll
       for (int j = 0; j < KT; j += 2) {
         uint32_t pa[S::NP][4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          uint32_t t[S::NP];
-          split_bf2<S::NP>(s[j + (i >> 1)][2 * (i & 1)], s[j + (i >> 1)][2 * (i & 1) + 1], t);
+          uint32_t t[S::NP] = {};
+          if (RH == 2 || (i & 1) == 0) split_bf2<S::NP>(s[j + (i >> 1)][2 * (i & 1)], s[j + (i >> 1)][2 * (i & 1) + 1], t);
 #pragma unroll
           for (int k = 0; k < S::NP; k++) pa[k][i] = t[k];
         }
@@ -307,19 +327,24 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
         if (KF) {
 #pragma unroll
           for (int t = 0; t < NO; t++) {
-            const float* vp = reinterpret_cast<const float*>(smem + buf * S::STAGE + kKeys * S::KROW +
-                                                             (wkey + 8 * j + 2 * tq) * S::VROW) + 8 * t + gq;
-            constexpr int LD = S::VROW / 4;
+            const int key = wkey + 8 * j + 2 * tq;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int kk = key + (i & 1) + 8 * (i >> 1);
+              v[i] = *reinterpret_cast<const float*>(kt_p + S::TILE + sw(kk, 2 * t + (gq >> 2)) + (gq & 3) * 4);
+              if (tail && cu.kt * kKeys + kk >= cu.len) v[i] = 0.0f;
+            }
             uint32_t b0[3], b1[3];
-            split_bf2<3>(vp[0], vp[LD], b0);
-            split_bf2<3>(vp[8 * LD], vp[9 * LD], b1);
+            split_bf2<3>(v[0], v[1], b0);
+            split_bf2<3>(v[2], v[3], b1);
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
               for (int k = 0; k <= sum; k++) mma_16816(x, pa[QF ? k : 0], b0[sum - k], b1[sum - k]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[t][e] += x[e];
+            for (int e = 0; e < 2 * RH; e++) o[t][e] += x[e];
           }
         } else {
 #pragma unroll
@@ -335,7 +360,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
                 mma_16816(y, pa[k], vb[2], vb[3]);
               }
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
+              for (int e = 0; e < 2 * RH; e++) {
                 o[t][e] += x[e];
                 o[t + 1][e] += y[e];
               }
@@ -347,6 +372,8 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
         }
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[buf]);  // the stage is consumed
     buf = buf + 1 == NS ? 0 : buf + 1;
 
     const bool ends = cu.kt + 1 == cu.nt;
@@ -363,7 +390,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
         a.parts[blockIdx.x] = d;
       }
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
+      for (int e = 0; e < RH; e++) {
         l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 1);
         l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 2);
       }
@@ -394,7 +421,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
       } else {
         // the four warps' states, merged in warp order
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < RH; e++) {
           const int r = gq + 8 * e;
           if (r >= nrows) continue;
           float* w = wst + (warp * a.rows_used + r) * (HD + 2);
@@ -403,7 +430,7 @@ __global__ void __launch_bounds__(kNT) paged_attn_kernel(const PagedAttnArgs a) 
           for (int t = 0; t < NO; t++)
             *reinterpret_cast<float2*>(w + 2 + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
         }
-        __syncthreads();
+        sync_rows();
         for (int i = tid; i < nrows * (HD / 2); i += kNT) {
           const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
           const float* w = wst + r * (HD + 2);
@@ -515,40 +542,46 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
   }
 }
 
-template <bool QF, bool KF, int HD, bool CHUNK>
+template <bool QF, bool KF, int HD, bool CHUNK, int RH>
 int attn_ctas(int rows_used) {
-  using S = Shape<QF, KF, HD, CHUNK>;
+  using S = Shape<QF, KF, HD, CHUNK, RH>;
   // shared memory per SM: 227 KB for blocks, 1 KB kept per block
   const int occ = std::max(1, std::min(4, (int)((227 * 1024) / (S::smem(rows_used) + 2048))));
   return device_sms() * occ;
 }
 
-template <bool QF, bool KF, int HD, bool CHUNK>
+template <bool QF, bool KF, int HD, bool CHUNK, int RH>
 cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
-  using S = Shape<QF, KF, HD, CHUNK>;
+  using S = Shape<QF, KF, HD, CHUNK, RH>;
   static SmemOptIn opt;
   const size_t smem = S::smem(a.rows_used);
-  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, CHUNK>), smem));
-  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK>, dim3(a.ctas), dim3(kNT), smem, s, a);
+  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, CHUNK, RH>), smem));
+  CUtensorMap mk, mv;
+  const int box = std::min(a.p.kv.page_size, kKeys);
+  int order = 0;
+  if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
+  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK, RH>, dim3(a.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);
 }
 
-// The call's mma.sync shape: f(QF, KF, HD, CHUNK as integral constants)
+// The call's mma.sync shape: f(QF, KF, HD, CHUNK, RH as integral constants).
+// Short runs share the key tile between the warps; beyond 16 packed rows
+// every warp has rows of its own (a float32 cache; over a bf16 one those
+// calls run on tcgen05).
 template <class F>
 auto with_shape(const ctts_paged_attn& p, F f) {
-  const bool qf = p.q_dtype == CTTS_F32, kf = p.kv.dtype == CTTS_F32, wide = p.kv.head_dim == 128;
-  // short runs share the key tile between the warps; beyond 16 packed rows
-  // every warp has rows of its own
-  const bool chunk = (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) > 16;
+  const bool qf = p.q_dtype == CTTS_F32, kf = p.kv.dtype == CTTS_F32;
+  const long rows = (long)p.max_new * (p.n_heads / p.kv.n_kv_heads);
   using T = std::true_type;
   using N = std::false_type;
-  using H64 = std::integral_constant<int, 64>;
-  using H128 = std::integral_constant<int, 128>;
-  if (kf) {
-    if (wide) return chunk ? f(T{}, T{}, H128{}, T{}) : f(T{}, T{}, H128{}, N{});
-    return chunk ? f(T{}, T{}, H64{}, T{}) : f(T{}, T{}, H64{}, N{});
-  }
-  if (wide) return qf ? f(T{}, N{}, H128{}, N{}) : f(N{}, N{}, H128{}, N{});
-  return qf ? f(T{}, N{}, H64{}, N{}) : f(N{}, N{}, H64{}, N{});
+  using R1 = std::integral_constant<int, 1>;
+  using R2 = std::integral_constant<int, 2>;
+  auto g = [&](auto hd) {
+    if (kf && rows > 16) return f(T{}, T{}, hd, T{}, R2{});
+    if (kf) return rows > 8 ? f(T{}, T{}, hd, N{}, R2{}) : f(T{}, T{}, hd, N{}, R1{});
+    if (qf) return rows > 8 ? f(T{}, N{}, hd, N{}, R2{}) : f(T{}, N{}, hd, N{}, R1{});
+    return rows > 8 ? f(N{}, N{}, hd, N{}, R2{}) : f(N{}, N{}, hd, N{}, R1{});
+  };
+  return p.kv.head_dim == 128 ? g(std::integral_constant<int, 128>{}) : g(std::integral_constant<int, 64>{});
 }
 
 // Chunks over a bf16 cache run on tcgen05 (paged_attn_tc.cu).
@@ -562,19 +595,44 @@ int rows_used_of(const ctts_paged_attn& p) {
 
 }  // namespace
 
+bool paged_pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, int box, int* order) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const int es = kv.dtype == CTTS_F32 ? 4 : 2;
+  struct Dim {
+    int64_t stride;
+    int size, box, what;
+  } d[3] = {{kv.token_stride, kv.page_size, box, 0}, {kv.head_stride, kv.n_kv_heads, 1, 1}, {kv.page_stride, kv.n_pages, 1, 2}};
+  std::stable_sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim}, strides[3];
+  cuuint32_t boxes[4] = {(cuuint32_t)(128 / es)}, estr[4] = {1, 1, 1, 1};
+  *order = 0;
+  for (int i = 0; i < 3; i++) {
+    dims[i + 1] = (cuuint64_t)d[i].size;
+    strides[i] = (cuuint64_t)d[i].stride * es;
+    boxes[i + 1] = (cuuint32_t)d[i].box;
+    *order |= d[i].what << (2 * i);
+  }
+  return fn(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
   PagedAttnPlan pl;
   if (use_tc(p)) {
     const PagedAttnTc t = paged_attn_tc_plan(p);
     pl.ctas = t.ctas;
     pl.tile_rows = t.tile_rows;
-  } else with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
-    constexpr bool QF = decltype(q)::value, KF = decltype(k)::value, CH = decltype(ch)::value;
-    constexpr int HD = decltype(hd)::value;
-    pl.ctas = attn_ctas<QF, KF, HD, CH>(rows_used_of(p));
-    pl.tile_rows = Shape<QF, KF, HD, CH>::R;
-    return 0;
-  });
+  } else {
+    with_shape(p, [&](auto q, auto k, auto hd, auto ch, auto rh) {
+      constexpr bool QF = decltype(q)::value, KF = decltype(k)::value, CH = decltype(ch)::value;
+      constexpr int HD = decltype(hd)::value, RH = decltype(rh)::value;
+      pl.ctas = attn_ctas<QF, KF, HD, CH, RH>(rows_used_of(p));
+      pl.tile_rows = Shape<QF, KF, HD, CH, RH>::R;
+      return 0;
+    });
+  }
   pl.ws_bytes = pl.ctas * (sizeof(AttnPart) + (size_t)2 * pl.tile_rows * (p.kv.head_dim + 2) * sizeof(float));
   return pl;
 }
@@ -600,8 +658,8 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   if (use_tc(p))
     CTTS_LK(launch_paged_attn_tc(a, s));
   else
-    CTTS_LK(with_shape(p, [&](auto q, auto k, auto hd, auto ch) {
-      return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value>(a, s);
+    CTTS_LK(with_shape(p, [&](auto q, auto k, auto hd, auto ch, auto rh) {
+      return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value, decltype(rh)::value>(a, s);
     }));
   const int rows = (int)std::min((long)a.tile_rows, (long)p.max_new * a.group);
   const dim3 grid(a.ctas, rows > 16 ? 16 : std::min(rows, 4)), block(kJoinThreads);

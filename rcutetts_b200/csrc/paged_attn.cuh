@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "tc_ptx.cuh"
 
 namespace ctts {
 
@@ -100,6 +101,7 @@ struct AttnStart {
   long end, total;  // where they end on the line, and its length
   long skip;   // units of request b ahead of them
   int b;
+  AttnReq req;
 };
 
 // This CTA's piece of the line.  The block sums the requests' units (four
@@ -161,6 +163,7 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
       if (at <= u0 && u0 < at + u[j]) {
         out->b = base + tid * PER + j;
         out->skip = u0 - at;
+        out->req = attn_req(a, base + tid * PER + j);
       }
       at += u[j];
     }
@@ -182,8 +185,7 @@ struct AttnCursor {
   int b, m, h, kt, nt, mt;
   int r0, cnt, nn, len;
 
-  CTTS_DEV void load(const PagedAttnArgs& a, int R) {
-    const AttnReq r = attn_req(a, b);
+  CTTS_DEV void set(const PagedAttnArgs& a, int R, const AttnReq& r) {
     r0 = r.r0; cnt = r.cnt; nn = r.nn; len = r.len;
     mt = (int)(((long)nn * a.group + R - 1) / R);
   }
@@ -195,7 +197,7 @@ struct AttnCursor {
   static CTTS_DEV AttnCursor at(const PagedAttnArgs& a, const AttnStart& s) {
     AttnCursor c;
     c.b = s.b;
-    c.load(a, R);
+    c.set(a, R, s.req);
     long skip = s.skip;
     for (c.m = 0;; c.m++) {
       c.tiles<R, C>(a);
@@ -221,11 +223,32 @@ struct AttnCursor {
     m = 0;
     do {
       b++;
-      load(a, R);
+      set(a, R, attn_req(a, b));
     } while (mt == 0 && b + 1 < a.p.batch);
     tiles<R, C>(a);
   }
 };
+
+// The pool as a 4D tensor map: 128 bytes of a head by `box` slots a copy, the
+// slot, head and page dimensions by ascending stride.  order: what dimensions
+// 1, 2 and 3 are (0 slot, 1 head, 2 page), two bits each.
+bool paged_pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, int box, int* order);
+
+// One box: `block` 128-byte blocks into the head's row.
+CTTS_DEV void copy_box(uint32_t dst, const CUtensorMap* m, int order, int x, int slot, int head, int page, uint64_t* bar) {
+  const int c[3] = {slot, head, page};
+  const int y = c[0] * ((order & 3) == 0) + c[1] * ((order & 3) == 1) + c[2] * ((order & 3) == 2);
+  const int z = c[0] * ((order >> 2 & 3) == 0) + c[1] * ((order >> 2 & 3) == 1) + c[2] * ((order >> 2 & 3) == 2);
+  const int w = c[0] * ((order >> 4) == 0) + c[1] * ((order >> 4) == 1) + c[2] * ((order >> 4) == 2);
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+CTTS_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+CTTS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // tcgen05 form (paged_attn_tc.cu): chunks over a bf16 cache.
 struct PagedAttnTc {

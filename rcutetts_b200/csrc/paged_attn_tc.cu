@@ -78,18 +78,8 @@ CTTS_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
-CTTS_DEV void tma_4d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
-CTTS_DEV void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 CTTS_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 CTTS_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-CTTS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 CTTS_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // uses of r[0..31] stay behind this point
 CTTS_DEV void pin32(uint32_t* r) {
@@ -178,12 +168,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         if (lane < nbox && kk < cu.len) page = a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)];
         if ((unsigned)page >= (unsigned)a.p.kv.n_pages) page = a.p.kv.n_pages;  // outside the map: zeros
         const int slot = kk & (a.p.kv.page_size - 1);
-        auto coord = [&](int i) {
-          const int what = (order >> (2 * i)) & 3;
-          return what == 0 ? slot : (what == 1 ? cu.h : page);
-        };
-        const int y = coord(0), z = coord(1), w = coord(2);
-  #pragma unroll
+#pragma unroll
         for (int kv = 0; kv < 2; kv++) {
           uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
           if (u >= NS && !mbar_wait(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1)) gave_up = 1;
@@ -193,7 +178,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           if (lane < nbox) {
             const uint32_t dst = (kv ? vs : ks) + st * S::TILE + (uint32_t)(lane * box) * 128u;
   #pragma unroll
-            for (int c = 0; c < NC; c++) tma_4d(dst + c * KT * 128, kv ? &tmV : &tmK, c * 64, y, z, w, full);
+            for (int c = 0; c < NC; c++) copy_box(dst + c * KT * 128, kv ? &tmV : &tmK, order, c * 64, slot, cu.h, page, full);
           }
         }
         if (u + 1 < units) cu.next<R, KT>(a);
@@ -532,30 +517,6 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// The pool as a 4D map, boxes of 64 dims x `box` slots: the head's dims, then
-// slot, head and page by ascending stride, as a map wants them.  order: what
-// dimensions 1, 2 and 3 are (0 slot, 1 head, 2 page), two bits each.
-bool pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, int box, int* order) {
-  auto fn = encode_fn();
-  if (!fn) return false;
-  struct Dim {
-    int64_t stride;
-    int size, box, what;
-  } d[3] = {{kv.token_stride, kv.page_size, box, 0}, {kv.head_stride, kv.n_kv_heads, 1, 1}, {kv.page_stride, kv.n_pages, 1, 2}};
-  std::stable_sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
-  cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim}, strides[3];
-  cuuint32_t boxes[4] = {64}, estr[4] = {1, 1, 1, 1};
-  *order = 0;
-  for (int i = 0; i < 3; i++) {
-    dims[i + 1] = (cuuint64_t)d[i].size;
-    strides[i] = (cuuint64_t)d[i].stride * 2;
-    boxes[i + 1] = (cuuint32_t)d[i].box;
-    *order |= d[i].what << (2 * i);
-  }
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool QF, int HD>
 cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
   using S = TcShape<QF, HD>;
@@ -573,7 +534,7 @@ cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
   }
   CUtensorMap mk, mv;
   int order = 0;
-  if (!pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
+  if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
   return launch_k(paged_attn_tc_kernel<QF, HD>, dim3(a.ctas), dim3(S::THREADS), S::SMEM, s, mk, mv, a, box, order);
 }
 

@@ -605,3 +605,37 @@ def test_serving_steps_match_the_contiguous_cache(dtype):
             assert got.shape == want.shape
             if want.size:
                 assert rel_err(got, want) < 1e-4 if dtype == "f32" else min(cosine(g, x) for g, x in zip(got, want)) >= 0.999
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_other_orders_in_memory(q_t, kv_t, new):
+    """Pools as views: keys and values of a page side by side, heads outermost, rows inside wider ones, one page, one head."""
+    c = Case([30, 100, 77], [new] * 3, 4, 2, 64, 16, q_t, kv_t, seed=5)
+    want = c.run()
+    c.check(want)
+    n, p, h, d = c.k.shape
+    side = torch.stack([c.k, c.v], 1)  # [pages, 2, page, heads, dim]
+    heads_out = torch.stack([c.k, c.v]).permute(0, 3, 1, 2, 4).contiguous().permute(0, 2, 3, 1, 4)
+    page_in = torch.stack([c.k, c.v]).permute(0, 2, 1, 3, 4).contiguous().permute(0, 2, 1, 3, 4)  # [page slot, pages, ...]
+    wide = torch.full((2, n, p, h, d + 8), float("nan"), dtype=kv_t, device="cuda")
+    wide[..., 8:] = torch.stack([c.k, c.v])
+    for k, v in ((side[:, 0], side[:, 1]), heads_out, page_in, wide[..., 8:]):
+        c.k, c.v = k, v
+        assert torch.equal(c.run(), want)
+    one = Case([5], [new], 2, 1, 64, 256, q_t, kv_t, seed=6, spare_cols=0)
+    pg = int(one.tables[0, 0])
+    one.k, one.v, one.tables = one.k[pg: pg + 1], one.v[pg: pg + 1], one.tables * 0
+    one.check(one.run())
+
+
+def test_append_other_orders_in_memory():
+    torch.manual_seed(9)
+    x = torch.randn(20, 8 * 64, device="cuda")
+    pos, slots = torch.arange(20, device="cuda").int(), torch.randperm(48, device="cuda")[:20].int()
+    k, v = torch.zeros(3, 16, 2, 64, device="cuda"), torch.zeros(3, 16, 2, 64, device="cuda")
+    paged.paged_append(x, k, v, pos, slots, 4)
+    side, outer = torch.zeros(3, 2, 16, 2, 64, device="cuda"), torch.zeros(2, 2, 3, 16, 64, device="cuda").permute(0, 2, 3, 1, 4)
+    for kk, vv in ((side[:, 0], side[:, 1]), outer):
+        paged.paged_append(x, kk, vv, pos, slots, 4)
+        assert torch.equal(kk, k) and torch.equal(vv, v)
