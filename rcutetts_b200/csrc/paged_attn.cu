@@ -25,7 +25,6 @@ namespace ctts {
 
 namespace {
 
-constexpr int kKeys = 64;  // keys per tile
 constexpr int kNT = 128;   // threads that compute; a warp behind them issues the copies
 
 CTTS_DEV void mma_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -44,8 +43,8 @@ CTTS_DEV void ldsm4_t(uint32_t addr, uint32_t* r) {
                : "r"(addr));
 }
 // One kernel shape.  CHUNK = false: 16 packed rows per item (single tokens and
-// short runs), the four warps share the rows and split each key tile, 16 keys
-// each, with their own softmax states; RH = 1 when no item has more than 8
+// short runs), the four warps share the rows and split each key tile's keys,
+// each with their own softmax states; RH = 1 when no item has more than 8
 // rows (the upper half of the MMA's rows stays zero and unread).  CHUNK =
 // true: 64 packed rows, 16 per warp, every warp takes all keys.
 template <bool QF, bool KF, int HD, bool CHUNK, int RH>
@@ -57,22 +56,26 @@ struct Shape {
   static constexpr int NQ = QF ? 3 : 1;
   static constexpr int NP = QF ? 3 : 1;
   static constexpr int ES = KF ? 4 : 2;
+  static constexpr int C = !KF && HD == 64 ? 128 : 64;  // keys per tile: 16 KB of K, and as much of V
   static constexpr int NB = HD * ES / 128;           // 128-byte blocks of a row
-  static constexpr uint32_t TILE = NB * kKeys * 128;  // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
+  static constexpr uint32_t TILE = NB * C * 128;  // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
   static constexpr uint32_t STAGE = 2 * TILE;
-  static constexpr int NS = STAGE <= 16384 ? 4 : (STAGE <= 32768 ? 3 : 2);
+  static constexpr int NS = STAGE <= 32768 ? 3 : 2;
   static constexpr int QBYTES = NQ * RQ * HD * 2;
-  static constexpr int KT = CHUNK ? 8 : 2;  // 8-key column tiles per warp and key tile
+  static constexpr int KT = CHUNK ? C / 8 : C / 32;  // 8-key column tiles per warp and key tile
+  // short runs keep their query fragments in registers where they are few
+  static constexpr bool QREG = !CHUNK && NQ * (HD / 16) * 2 * RH <= 24;
+  static constexpr int CTAS = STAGE <= 32768 ? 2 : 1;  // an SM holds at least this many blocks
   static size_t smem(int rows_used) {
     return 1024 + (size_t)NS * STAGE + QBYTES + (CHUNK ? 0 : (size_t)4 * rows_used * (HD + 2) * 4);
   }
 };
 
 template <bool QF, bool KF, int HD, bool CHUNK, int RH>
-__global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+__global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                               const __grid_constant__ PagedAttnArgs a, int box, int order) {
   using S = Shape<QF, KF, HD, CHUNK, RH>;
-  constexpr int R = S::R, KT = S::KT, NO = HD / 8, KS = HD / 16, NS = S::NS;
+  constexpr int R = S::R, C = S::C, KT = S::KT, NO = HD / 8, KS = HD / 16, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnStart start;
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
@@ -93,31 +96,31 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
     gave_up = 0;
   }
   grid_dep_enter();
-  attn_find_start<R, kKeys, kNT + 32>(a, &start);
+  attn_find_start<R, C, kNT + 32>(a, &start);
   const long units = start.units;
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   if (units == 0) return;
-  AttnCursor cu = AttnCursor::at<R, kKeys>(a, start);
+  AttnCursor cu = AttnCursor::at<R, C>(a, start);
   auto wait = [&](uint64_t* bar, uint32_t parity) {  // (after one that gave up nobody waits: the block runs to its end)
     if (!gave_up && !mbar_wait(bar, parity)) gave_up = 1;
   };
 
   if (warp == 4) {
-    // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile; the
+    // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them.  Pages that do not exist are
     // outside the map and arrive as zeros.
     auto page_of = [&]() {
-      const int kk = cu.kt * kKeys + 8 * lane;
-      return lane < 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
+      const int kk = cu.kt * C + 8 * lane;
+      return lane < C / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
     };
     int page = page_of();
     for (long u = 0; u < units; u++) {
-      const int st = (int)(u % NS), kk = cu.kt * kKeys + 8 * lane, h = cu.h;
+      const int st = (int)(u % NS), kk = cu.kt * C + 8 * lane, h = cu.h;
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
-      const uint32_t dead = __ballot_sync(0xffffffffu, lane < 8 && kk < cu.len && none);
+      const uint32_t dead = __ballot_sync(0xffffffffu, lane < C / 8 && kk < cu.len && none);
       const int mine = none ? a.p.kv.n_pages : page;
       if (u + 1 < units) {  // the next tile's pages, over the wait
-        cu.next<R, kKeys>(a);
+        cu.next<R, C>(a);
         page = page_of();
       }
       if (u >= NS) wait(&empty[st], (uint32_t)((u / NS) & 1) ^ 1);
@@ -127,13 +130,13 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
         mbar_expect_tx(&full[st], S::STAGE);
       }
       __syncwarp();
-      if (lane < 8 && (8 * lane & (box - 1)) == 0) {
+      if (lane < C / 8 && (8 * lane & (box - 1)) == 0) {
         const uint32_t dst = sbase + st * S::STAGE + (uint32_t)lane * 1024u;
         const int slot = kk & (a.p.kv.page_size - 1);
 #pragma unroll
         for (int b = 0; b < S::NB; b++) {
-          copy_box(dst + b * kKeys * 128, &tmK, order, b * (128 / S::ES), slot, h, mine, &full[st]);
-          copy_box(dst + S::TILE + b * kKeys * 128, &tmV, order, b * (128 / S::ES), slot, h, mine, &full[st]);
+          copy_box(dst + b * C * 128, &tmK, order, b * (128 / S::ES), slot, h, mine, &full[st]);
+          copy_box(dst + S::TILE + b * C * 128, &tmV, order, b * (128 / S::ES), slot, h, mine, &full[st]);
         }
       }
     }
@@ -150,8 +153,9 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
     return qbase + (uint32_t)(term * S::RQ + row) * (HD * 2) + (uint32_t)((chunk & ~7) | ((chunk ^ row) & 7)) * 16u;
   };
   // 16-byte chunk of a key's row in a tile
-  auto sw = [](int key, int chunk) { return (uint32_t)(chunk >> 3) * (kKeys * 128) + (uint32_t)key * 128 + (uint32_t)((chunk ^ key) & 7) * 16u; };
+  auto sw = [](int key, int chunk) { return (uint32_t)(chunk >> 3) * (C * 128) + (uint32_t)key * 128 + (uint32_t)((chunk ^ key) & 7) * 16u; };
   const float c2 = a.c2_hi;
+  uint32_t qr[S::QREG ? KS : 1][S::NQ][2 * RH];  // QREG: fragments of the item's queries
   float o[NO][4], m2[2], l2[2];
   bool fresh = true;  // the unit begins a piece
   int unit0_kt = 0;   // the piece's first key tile
@@ -197,11 +201,22 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
       m2[0] = m2[1] = -INFINITY;
       l2[0] = l2[1] = 0.0f;
       sync_rows();
+      if (S::QREG) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+          for (int k = 0; k < S::NQ; k++) {
+            uint32_t t[4];
+            ldsm4(q_addr(k, lane & 15, 2 * ks + (lane >> 4)), t);
+#pragma unroll
+            for (int i = 0; i < 2 * RH; i++) qr[S::QREG ? ks : 0][k][i] = t[RH == 2 ? i : 2 * i];  // rows 8..15 (t[1], t[3]) are zero when RH = 1
+          }
+      }
       fresh = false;
     }
     const int wrow = CHUNK ? warp * 16 : 0;      // the warp's rows and keys
-    const int wkey = CHUNK ? 0 : warp * 16;
-    const int key0 = cu.kt * kKeys + wkey;
+    const int wkey = CHUNK ? 0 : warp * (C / 4);
+    const int key0 = cu.kt * C + wkey;
     // positions of the thread's two rows; rows behind the tile see nothing (their queries are zero, their states unused)
     int pr[2];
 #pragma unroll
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
       if (!KF && tail) {
         for (int i = lane; i < 8 * KT * (HD / 8); i += 32) {
           const int key = wkey + i / (HD / 8);
-          if (cu.kt * kKeys + key >= cu.len)
+          if (cu.kt * C + key >= cu.len)
             *reinterpret_cast<uint4*>(smem + buf * S::STAGE + S::TILE + sw(key, i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
@@ -236,7 +251,17 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
       for (int ks = 0; ks < KS; ks++) {
         uint32_t qa[S::NQ][4];
 #pragma unroll
-        for (int k = 0; k < S::NQ; k++) ldsm4(q_addr(k, wrow + (lane & 15), 2 * ks + (lane >> 4)), qa[k]);
+        for (int k = 0; k < S::NQ; k++) {
+          if (S::QREG) {
+            const uint32_t* q = qr[S::QREG ? ks : 0][k];
+            qa[k][0] = q[0];
+            qa[k][1] = RH == 2 ? q[1] : 0u;
+            qa[k][2] = q[RH];
+            qa[k][3] = RH == 2 ? q[3 % (2 * RH)] : 0u;
+          } else {
+            ldsm4(q_addr(k, wrow + (lane & 15), 2 * ks + (lane >> 4)), qa[k]);
+          }
+        }
         if (KF) {
 #pragma unroll
           for (int j = 0; j < KT; j++) {
@@ -333,7 +358,7 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
             for (int i = 0; i < 4; i++) {
               const int kk = key + (i & 1) + 8 * (i >> 1);
               v[i] = *reinterpret_cast<const float*>(kt_p + S::TILE + sw(kk, 2 * t + (gq >> 2)) + (gq & 3) * 4);
-              if (tail && cu.kt * kKeys + kk >= cu.len) v[i] = 0.0f;
+              if (tail && cu.kt * C + kk >= cu.len) v[i] = 0.0f;
             }
             uint32_t b0[3], b1[3];
             split_bf2<3>(v[0], v[1], b0);
@@ -462,7 +487,7 @@ __global__ void __launch_bounds__(kNT + 32) paged_attn_kernel(const __grid_const
       }
       fresh = true;
     }
-    if (u + 1 < units) cu.next<R, kKeys>(a);
+    if (u + 1 < units) cu.next<R, C>(a);
   }
 }
 
@@ -545,8 +570,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
 template <bool QF, bool KF, int HD, bool CHUNK, int RH>
 int attn_ctas(int rows_used) {
   using S = Shape<QF, KF, HD, CHUNK, RH>;
-  // shared memory per SM: 227 KB for blocks, 1 KB kept per block
-  const int occ = std::max(1, std::min(4, (int)((227 * 1024) / (S::smem(rows_used) + 2048))));
+  // shared memory: 228 KB an SM, of which each block takes 1 KB beside its own
+  const int occ = std::max(1, std::min(4, (int)(228 * 1024 / (S::smem(rows_used) + 1024 + 512))));
   return device_sms() * occ;
 }
 
@@ -557,7 +582,7 @@ cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
   const size_t smem = S::smem(a.rows_used);
   CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, CHUNK, RH>), smem));
   CUtensorMap mk, mv;
-  const int box = std::min(a.p.kv.page_size, kKeys);
+  const int box = std::min(a.p.kv.page_size, (int)S::C);
   int order = 0;
   if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
   return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK, RH>, dim3(a.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);

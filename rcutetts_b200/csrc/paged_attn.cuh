@@ -79,22 +79,71 @@ CTTS_DEV AttnReq attn_req(const PagedAttnArgs& a, int b) {
   r.len = (int)min((long)max(a.p.seq_lens[b], 0), (long)a.p.max_pages << a.shift);
   return r;
 }
+// Row tiles of a request (packed rows fit 31 bits: the host checks).
+template <int R>
+CTTS_DEV int attn_row_tiles(const AttnReq& r, int group) {
+  return (r.nn * group + R - 1) / R;
+}
 // Key tiles of row tile m: up to the position of its last row; at least one,
 // which also writes the zeros of rows that see nothing.
 template <int R, int C>
 CTTS_DEV int attn_tiles(const AttnReq& r, int m, int group) {
-  const int last = min(r.nn, (int)(((long)(m + 1) * R - 1) / group) + 1);  // rows ahead of the tile's end
-  const int keys = min(r.len, r.len - r.cnt + last);
-  return max(1, (keys + C - 1) / C);
+  const int packed = (m + 1) * R;  // packed rows up to the tile's end
+  const int ahead = packed >= r.nn * group ? r.nn : (packed - 1) / group + 1;
+  return max(1, (min(r.len, r.len - r.cnt + ahead) + C - 1) / C);
 }
+// The row tiles of a request in order: the rows ahead of each one's end by
+// running quotient and remainder, without a division a tile.
 template <int R, int C>
-CTTS_DEV long attn_units(const PagedAttnArgs& a, int b) {
-  const AttnReq r = attn_req(a, b);
-  const int mt = (int)(((long)r.nn * a.group + R - 1) / R);
+struct AttnRowWalk {
+  const AttnReq& r;
+  int group, per, over, ahead, rem;  // ahead = ((m + 1) R - 1) / group, rem its remainder
+  CTTS_DEV AttnRowWalk(const AttnReq& req, int g) : r(req), group(g) {
+    per = R / g;
+    over = R - per * g;
+    ahead = per;
+    rem = over - 1;
+    if (rem < 0) {
+      rem += g;
+      ahead--;
+    }
+  }
+  CTTS_DEV int tiles() const { return max(1, (min(r.len, r.len - r.cnt + min(r.nn, ahead + 1)) + C - 1) / C); }
+  CTTS_DEV void next() {
+    ahead += per;
+    rem += over;
+    if (rem >= group) {
+      rem -= group;
+      ahead++;
+    }
+  }
+};
+template <int R, int C>
+CTTS_DEV long attn_units(const PagedAttnArgs& a, const AttnReq& r) {
+  const int mt = attn_row_tiles<R>(r, a.group);
+  AttnRowWalk<R, C> w(r, a.group);
   long n = 0;
-  for (int m = 0; m < mt; m++) n += attn_tiles<R, C>(r, m, a.group);
+  for (int m = 0; m < mt; m++, w.next()) n += w.tiles();
   return n * a.p.kv.n_kv_heads;
 }
+// The line is cut into `ctas` pieces of `base` tiles, the first `rest` of them
+// one longer; no more pieces than tiles, so that the pieces of a divided item
+// lie in neighbouring CTAs.
+struct AttnCut {
+  int ctas;
+  long base, rest;
+  CTTS_DEV AttnCut(int n, long total) {
+    ctas = total < n ? (int)total : n;
+    if (ctas == 0) ctas = 1;
+    base = total >> 32 ? total / ctas : (long)((unsigned)total / (unsigned)ctas);  // (a 64-bit division is ten times the latency)
+    rest = total - base * ctas;
+  }
+  CTTS_DEV long begin(int c) const { return c < ctas ? c * base + min((long)c, rest) : base * ctas + rest; }
+  CTTS_DEV int owner(long unit) const {  // the CTA that has a tile
+    const long longer = rest * (base + 1);
+    return (int)(unit < longer ? unit / (base + 1) : rest + (unit - longer) / base);
+  }
+};
 
 struct AttnStart {
   long units;  // this CTA's
@@ -104,24 +153,32 @@ struct AttnStart {
   AttnReq req;
 };
 
-// This CTA's piece of the line.  The block sums the requests' units (four
-// requests a thread and turn); a second pass finds the request the piece
-// begins in, from registers when one turn holds the batch.
+// This CTA's piece of the line.  The block sums the requests' units, one
+// request a thread while the batch fits (else four a thread and turn); a
+// second pass finds the request the piece begins in, from registers when one
+// turn holds the batch.
 template <int R, int C, int NT>
 CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
   constexpr int PER = 4, W = NT / 32;
   __shared__ long wsum[2][W];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.p.batch;
+  const int per = n <= NT ? 1 : PER;
   long u[PER];
+  AttnReq rq[PER];
   long total = 0, first = 0, mine_before = 0;
   int ph = 0;
-  // one turn: units of requests base + tid*PER + j; returns the turn's sum, mine_before = units ahead of the thread's
+  // one turn: units of requests base + tid*per + j; returns the turn's sum, mine_before = units ahead of the thread's
   auto turn = [&](int base) {
     long t = 0;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-      const int b = base + tid * PER + j;
-      u[j] = b < n ? attn_units<R, C>(a, b) : 0;
+      const int b = base + tid * per + j;
+      u[j] = 0;
+      if (j < per && b < n) rq[j] = attn_req(a, b);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      if (j < per && base + tid * per + j < n) u[j] = attn_units<R, C>(a, rq[j]);
       t += u[j];
     }
     long inc = t;
@@ -142,42 +199,37 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
     ph ^= 1;
     return all;
   };
-  for (int base = 0; base < n; base += NT * PER) total += turn(base);
-  // no more pieces than tiles: every piece of a divided item lies in the CTA next to the one before
-  const long ctas = min((long)a.ctas, total), c = blockIdx.x;
-  const long u0 = c < ctas ? total * c / ctas : 0, u1 = c < ctas ? total * (c + 1) / ctas : 0;
+  for (int base = 0; base < n; base += NT * per) total += turn(base);
+  const AttnCut cut(a.ctas, total);
+  const long u0 = cut.begin(blockIdx.x), u1 = cut.begin(blockIdx.x + 1);
   if (tid == 0) {
     out->units = u1 - u0;
     out->end = u1;
     out->total = total;
-    out->b = 0;
-    out->skip = 0;
   }
-  __syncthreads();
-  if (u1 == u0) return;
-  for (int base = 0; base < n; base += NT * PER) {
-    const long all = n <= NT * PER ? total : turn(base);
-    long at = first + mine_before;
+  if (u1 > u0) {
+    for (int base = 0; base < n; base += NT * per) {
+      const long all = n <= NT * per ? total : turn(base);
+      long at = first + mine_before;
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-      if (at <= u0 && u0 < at + u[j]) {
-        out->b = base + tid * PER + j;
-        out->skip = u0 - at;
-        out->req = attn_req(a, base + tid * PER + j);
+      for (int j = 0; j < PER; j++) {
+        if (at <= u0 && u0 < at + u[j]) {
+          out->b = base + tid * per + j;
+          out->skip = u0 - at;
+          out->req = rq[j];
+        }
+        at += u[j];
       }
-      at += u[j];
+      first += all;
+      if (first > u0) break;
     }
-    first += all;
-    if (first > u0) break;
   }
   __syncthreads();
 }
 
-// CTAs from this one to the one that holds tile `more` behind this CTA's end
-// (unit e lies in the last CTA c with total * c / ctas <= e).
+// CTAs from this one to the one that holds tile `more` behind this CTA's end.
 CTTS_DEV int attn_pieces(const PagedAttnArgs& a, const AttnStart& s, int more) {
-  const long ctas = min((long)a.ctas, s.total), e = s.end + more - 1;
-  return (int)(((e + 1) * ctas + s.total - 1) / s.total) - (int)blockIdx.x;
+  return AttnCut(a.ctas, s.total).owner(s.end + more - 1) - (int)blockIdx.x + 1;
 }
 
 // A place on the line: request, row tile, KV head, key tile.
@@ -187,7 +239,7 @@ struct AttnCursor {
 
   CTTS_DEV void set(const PagedAttnArgs& a, int R, const AttnReq& r) {
     r0 = r.r0; cnt = r.cnt; nn = r.nn; len = r.len;
-    mt = (int)(((long)nn * a.group + R - 1) / R);
+    mt = (nn * a.group + R - 1) / R;
   }
   template <int R, int C>
   CTTS_DEV void tiles(const PagedAttnArgs& a) {
@@ -199,14 +251,15 @@ struct AttnCursor {
     c.b = s.b;
     c.set(a, R, s.req);
     long skip = s.skip;
-    for (c.m = 0;; c.m++) {
-      c.tiles<R, C>(a);
+    AttnRowWalk<R, C> w(s.req, a.group);
+    for (c.m = 0;; c.m++, w.next()) {
+      c.nt = w.tiles();
       const long in = (long)c.nt * a.p.kv.n_kv_heads;
       if (skip < in || c.m + 1 >= c.mt) break;
       skip -= in;
     }
-    c.h = (int)(skip / c.nt);
-    c.kt = (int)(skip % c.nt);
+    c.h = (unsigned)skip / (unsigned)c.nt;  // (skip is inside one row tile's heads: 31 bits)
+    c.kt = (unsigned)skip % (unsigned)c.nt;
     return c;
   }
   // (never called at the end of the line)

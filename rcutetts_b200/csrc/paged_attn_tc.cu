@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           __syncwarp();
           if (lane < nbox) {
             const uint32_t dst = (kv ? vs : ks) + st * S::TILE + (uint32_t)(lane * box) * 128u;
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < NC; c++) copy_box(dst + c * KT * 128, kv ? &tmV : &tmK, order, c * 64, slot, cu.h, page, full);
           }
         }
@@ -207,11 +207,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           asm volatile("" : "+r"(kb), "+r"(qb));
           // small terms first: the tensor core cuts what it adds to the
           // accumulator's precision
-  #pragma unroll
+#pragma unroll
           for (int t = NT - 1; t >= 0; t--)
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < NC; c++)
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < 4; k++) {
                 umma_bf16(tmem + 128 * s, tc_desc(qb + t * S::QTERM + c * 16384 + k * 32, 16),
                           tc_desc(kb + c * KT * 128 + k * 32, 16), tc_idesc(KT, false), acc);
@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         auto values = [&](int s, int st, uint32_t acc) {
           uint32_t vb = vs + st * S::TILE;
           asm volatile("" : "+r"(vb));
-  #pragma unroll
+#pragma unroll
           for (int t = NT - 1; t >= 0; t--)
-  #pragma unroll
+#pragma unroll
             for (int k = 0; k < KT / 16; k++) {
               mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + t * (KT / 2) + k * 8, tc_desc(vb + k * 2048, KT * 128), tc_idesc(HD, true), acc);
               acc = 1;
@@ -289,13 +289,13 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
       float o_row[QF ? HD : 1];  // float32 calls: the output row so far
       // adds the product of the last tile to it
       auto gather = [&]() {
-  #pragma unroll
+#pragma unroll
         for (int c = 0; c < HD; c += 32) {
           uint32_t o[32];
           tmem_ld32_nowait(tO + c, o);
           tmem_wait();
           pin32(o);
-  #pragma unroll
+#pragma unroll
           for (int j = 0; j < 32; j++) o_row[QF ? c + j : 0] += __uint_as_float(o[j]);
         }
       };
@@ -312,36 +312,53 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           pos_lo = cu.len - cu.cnt + (pk - lane) / a.group;
           m = -INFINITY;
           l = 0.0f;
-  #pragma unroll
+#pragma unroll
           for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] = 0.0f;
           if (on) {
-            // the row's query, as bf16 terms; rows behind the item are zero
-            const long at = mine ? (long)(cu.r0 + pk / a.group) * a.p.q_ld + (long)(cu.h * a.group + pk % a.group) * HD : 0;
-            const uint32_t qrow = qs + s * NT * S::QTERM + row * 128;
-  #pragma unroll 4
-            for (int ch = 0; ch < HD / 8; ch++) {
-              uint32_t t[4][NT];
-              if (QF) {
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                if (mine) {
-                  x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + ch * 8);
-                  y = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + ch * 8 + 4);
+            // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes
+            // of a row (as bf16), four rows at a time, all loads in flight
+            // before the first is used; rows behind the item are zero
+            const int r0 = (warp & 3) * 32, p0 = cu.m * R + s * 128 + r0;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+              constexpr int RP = 8;  // rows a lane reads: 4 i + lane / 8
+              uint4 x[RP], y[QF ? RP : 1];
+#pragma unroll
+              for (int i = 0; i < RP; i++) {
+                const int r = 4 * i + (lane >> 3), p = p0 + r;
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (QF) y[QF ? i : 0] = x[i];
+                if (s * 128 + r0 + r < nrows) {
+                  const int tok = p / a.group;
+                  const long at = (long)(cu.r0 + tok) * a.p.q_ld + (cu.h * a.group + p - tok * a.group) * HD + c * 64 + (lane & 7) * 8;
+                  if (QF) {
+                    x[i] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at);
+                    y[QF ? i : 0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at + 4);
+                  } else {
+                    x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
+                  }
                 }
-                split_bf2<NT>(x.x, x.y, t[0]);
-                split_bf2<NT>(x.z, x.w, t[1]);
-                split_bf2<NT>(y.x, y.y, t[2]);
-                split_bf2<NT>(y.z, y.w, t[3]);
-              } else {
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (mine) x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at + ch * 8);
-                t[0][0] = x.x; t[1][0] = x.y; t[2][0] = x.z; t[3][0] = x.w;
               }
-              const uint32_t dst = qrow + (ch >> 3) * 16384 + (uint32_t)(((ch & 7) ^ (row & 7)) << 4);
-  #pragma unroll
-              for (int k = 0; k < NT; k++)
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + k * S::QTERM), "r"(t[0][k]), "r"(t[1][k]), "r"(t[2][k]),
-                             "r"(t[3][k])
-                             : "memory");
+#pragma unroll
+              for (int i = 0; i < RP; i++) {
+                const int r = r0 + 4 * i + (lane >> 3);
+                uint32_t t[4][NT];
+                if (QF) {
+                  const uint4 z = y[QF ? i : 0];
+                  split_bf2<NT>(__uint_as_float(x[i].x), __uint_as_float(x[i].y), t[0]);
+                  split_bf2<NT>(__uint_as_float(x[i].z), __uint_as_float(x[i].w), t[1]);
+                  split_bf2<NT>(__uint_as_float(z.x), __uint_as_float(z.y), t[2]);
+                  split_bf2<NT>(__uint_as_float(z.z), __uint_as_float(z.w), t[3]);
+                } else {
+                  t[0][0] = x[i].x; t[1][0] = x[i].y; t[2][0] = x[i].z; t[3][0] = x[i].w;
+                }
+                const uint32_t dst = qs + s * NT * S::QTERM + c * 16384 + r * 128 + (uint32_t)(((lane ^ r) & 7) << 4);
+#pragma unroll
+                for (int k = 0; k < NT; k++)
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + k * S::QTERM), "r"(t[0][k]), "r"(t[1][k]), "r"(t[2][k]),
+                               "r"(t[3][k])
+                               : "memory");
+              }
             }
             fence_async();
             mbar_arrive(&bars.q_full[s]);
@@ -366,7 +383,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
             const int st = (int)(u % NS);
             if (!mbar_wait(&bars.v_full[st], (uint32_t)((u / NS) & 1))) gave_up = 1;
             if (row < KT && key0 + row >= cu.len) {
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < NC * 8; c++)
                 asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + st * S::TILE + (c >> 3) * KT * 128 + row * 128 + (c & 7) * 16), "r"(0)
                              : "memory");
@@ -382,21 +399,21 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           if (warp_on) {
             fence_after();
             uint32_t x[KT];
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < KT; c += 32) tmem_ld32_nowait(tS + c, x + c);
             tmem_wait();
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < KT; c += 32) pin32(x + c);
             if (key0 + KT - 1 > pos_lo || dead) {
               const int lim = pos - key0;
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < KT; c++)
                 if (c > lim || ((dead >> (c >> 3)) & 1)) x[c] = 0xff800000u;  // -inf
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < KT; c += 4)
-  #pragma unroll
+#pragma unroll
               for (int j = 0; j < 4; j++) mx[j] = fmaxf(mx[j], __uint_as_float(x[c + j]));
             const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
             if (QF) {
@@ -404,7 +421,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
               const float mm = fmaxf(m, mn), f = mm == -INFINITY ? 0.0f : exp2_fast(m - mm);
               m = mm;
               l *= f;
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] *= f;
             } else if (cu.kt == kt0) {
               m = mn;  // O is overwritten by the first product
@@ -414,13 +431,13 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
                 const float f = grow ? exp2_fast(m - mn) : 1.0f;
                 if (grow) m = mn;
                 l *= f;
-  #pragma unroll 1
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                   uint32_t o[32];
                   tmem_ld32_nowait(tO + c, o);
                   tmem_wait();
                   pin32(o);
-  #pragma unroll
+#pragma unroll
                   for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
                   tmem_st32(tO + c, o);
                 }
@@ -429,10 +446,10 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
             }
             const float mz = m == -INFINITY ? 0.0f : m;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < KT; c += 32) {
               uint32_t p[NT][16];
-  #pragma unroll
+#pragma unroll
               for (int j = 0; j < 32; j += 2) {
                 const float e0 = exp2_fast(attn_arg<QF>(a, __uint_as_float(x[c + j]), mz));
                 const float e1 = exp2_fast(attn_arg<QF>(a, __uint_as_float(x[c + j + 1]), mz));
@@ -440,10 +457,10 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
                 sum[(j & 2) + 1] += e1;
                 uint32_t t[NT];
                 split_bf2<NT>(e0, e1, t);
-  #pragma unroll
+#pragma unroll
                 for (int k = 0; k < NT; k++) p[k][j >> 1] = t[k];
               }
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < NT; k++) tmem_st16(tS + k * (KT / 2) + (c >> 1), p[k]);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -474,11 +491,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
               const long pr = (long)slot * a.tile_rows + s * 128 + row;
               if (!whole && mine) a.ml[pr] = make_float2(m, l);
               if (QF) gather();
-  #pragma unroll
+#pragma unroll
               for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 if (QF) {
-  #pragma unroll
+#pragma unroll
                   for (int j = 0; j < 32; j++) o[j] = __float_as_uint(o_row[QF ? c + j : 0]);
                 } else {
                   tmem_ld32_nowait(tO + c, o);
@@ -487,17 +504,17 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
                 }
                 if (mine) {
                   float v[32];
-  #pragma unroll
+#pragma unroll
                   for (int j = 0; j < 32; j++) v[j] = l == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
                   if (whole && !QF) {
                     uint16_t* w = static_cast<uint16_t*>(a.p.out) + at + c;
-  #pragma unroll
+#pragma unroll
                     for (int j = 0; j < 32; j += 8)
                       *reinterpret_cast<uint4*>(w + j) = make_uint4(pack_bf2(v[j], v[j + 1]), pack_bf2(v[j + 2], v[j + 3]),
                                                                     pack_bf2(v[j + 4], v[j + 5]), pack_bf2(v[j + 6], v[j + 7]));
                   } else {
                     float* w = whole ? static_cast<float*>(a.p.out) + at + c : a.acc + pr * HD + c;
-  #pragma unroll
+#pragma unroll
                     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                   }
                 }
