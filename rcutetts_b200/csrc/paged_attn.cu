@@ -97,34 +97,36 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
   }
   grid_dep_enter();
   attn_find_start<R, C, kNT + 32>(a, &start);
-  const long units = start.units;
+  const int units = (int)start.units;  // (of one CTA: 31 bits, the host checks)
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   if (units == 0) return;
   AttnCursor cu = AttnCursor::at<R, C>(a, start);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {  // (after one that gave up nobody waits: the block runs to its end)
-    if (!gave_up && !mbar_wait(bar, parity)) gave_up = 1;
-  };
 
   if (warp == 4) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them.  Pages that do not exist are
     // outside the map and arrive as zeros.
+    int kt = cu.kt;
     auto page_of = [&]() {
-      const int kk = cu.kt * C + 8 * lane;
+      const int kk = kt * C + 8 * lane;
       return lane < C / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
     };
-    int page = page_of();
-    for (long u = 0; u < units; u++) {
-      const int st = (int)(u % NS), kk = cu.kt * C + 8 * lane, h = cu.h;
+    int page = page_of(), st = 0;
+    uint32_t par = 0;
+#pragma unroll 1
+    for (int u = 0; u < units && !gave_up; u++) {
+      const int kk = kt * C + 8 * lane, h = cu.h;
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < C / 8 && kk < cu.len && none);
       const int mine = none ? a.p.kv.n_pages : page;
       if (u + 1 < units) {  // the next tile's pages, over the wait
-        cu.next<R, C>(a);
+        if (++kt == cu.nt) {
+          cu = AttnCursor::next<R, C>(a, cu);
+          kt = 0;
+        }
         page = page_of();
       }
-      if (u >= NS) wait(&empty[st], (uint32_t)((u / NS) & 1) ^ 1);
-      if (__any_sync(0xffffffffu, gave_up)) break;
+      if (u >= NS) mbar_wait_or(&empty[st], par ^ 1, &gave_up);
       if (lane == 0) {
         dead_keys[st] = dead;
         mbar_expect_tx(&full[st], S::STAGE);
@@ -133,11 +135,15 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
       if (lane < C / 8 && (8 * lane & (box - 1)) == 0) {
         const uint32_t dst = sbase + st * S::STAGE + (uint32_t)lane * 1024u;
         const int slot = kk & (a.p.kv.page_size - 1);
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < S::NB; b++) {
           copy_box(dst + b * C * 128, &tmK, order, b * (128 / S::ES), slot, h, mine, &full[st]);
           copy_box(dst + S::TILE + b * C * 128, &tmV, order, b * (128 / S::ES), slot, h, mine, &full[st]);
         }
+      }
+      if (++st == NS) {
+        st = 0;
+        par ^= 1;
       }
     }
     if (gave_up)  // copies in flight land before the block may leave
@@ -157,15 +163,16 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
   const float c2 = a.c2_hi;
   uint32_t qr[S::QREG ? KS : 1][S::NQ][2 * RH];  // QREG: fragments of the item's queries
   float o[NO][4], m2[2], l2[2];
-  bool fresh = true;  // the unit begins a piece
-  int unit0_kt = 0;   // the piece's first key tile
-  int buf = 0;
-  for (long u = 0; u < units; u++) {
-    const int row_base = cu.m * R;               // first packed row of the tile
-    const int nrows = min(R, cu.nn * a.group - row_base);
-    const int pos0 = cu.len - cu.cnt;            // position of the request's first new row
-    if (fresh) {
-      unit0_kt = cu.kt;
+  int buf = 0, u = 0;
+  uint32_t par = 0;
+#pragma unroll 1
+  while (true) {
+    // ---- a piece: tiles cu.kt .. end of an item
+    const int end = min(cu.nt, cu.kt + units - u);
+    const int row_base = cu.m * R;  // first packed row of the item
+    const int nrows = cu.rows(a, R);
+    const int pos0 = cu.pos0();
+    {
       if (CHUNK) sync_rows();  // the queries of the item before are read (short runs: their merge has synchronised)
       // queries of the tile as bf16 terms; rows behind nrows are zero
       constexpr int CH = HD / 8;
@@ -212,11 +219,9 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
             for (int i = 0; i < 2 * RH; i++) qr[S::QREG ? ks : 0][k][i] = t[RH == 2 ? i : 2 * i];  // rows 8..15 (t[1], t[3]) are zero when RH = 1
           }
       }
-      fresh = false;
     }
     const int wrow = CHUNK ? warp * 16 : 0;      // the warp's rows and keys
     const int wkey = CHUNK ? 0 : warp * (C / 4);
-    const int key0 = cu.kt * C + wkey;
     // positions of the thread's two rows; rows behind the tile see nothing (their queries are zero, their states unused)
     int pr[2];
 #pragma unroll
@@ -224,8 +229,12 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
       const int r = wrow + gq + 8 * e;
       pr[e] = r < nrows ? pos0 + (row_base + r) / a.group : -1;
     }
-    wait(&full[buf], (uint32_t)((u / NS) & 1));
     const int plast = wrow < nrows ? pos0 + (row_base + min(nrows, wrow + 16) - 1) / a.group : -1;
+    const int pfirst = pos0 + (row_base + wrow) / a.group;
+#pragma unroll 1
+    for (int kt = cu.kt; kt < end; kt++) {
+    const int key0 = kt * C + wkey;
+    mbar_wait_or(&full[buf], par, &gave_up);
     if (key0 <= plast) {
       const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + S::TILE;
       const uint8_t* const kt_p = smem + buf * S::STAGE;
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
       if (!KF && tail) {
         for (int i = lane; i < 8 * KT * (HD / 8); i += 32) {
           const int key = wkey + i / (HD / 8);
-          if (cu.kt * C + key >= cu.len)
+          if (kt * C + key >= cu.len)
             *reinterpret_cast<uint4*>(smem + buf * S::STAGE + S::TILE + sw(key, i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
@@ -298,7 +307,6 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
           for (int e = 0; e < 2 * RH; e++) s[j][e] += lo[QF ? j : 0][e];
       }
       // causal mask and missing pages; a tile that every row sees whole needs none
-      const int pfirst = pos0 + (row_base + wrow) / a.group;
       const uint32_t gone = (dead_keys[buf] >> (wkey >> 3)) & ((1u << KT) - 1);
       if (key0 + 8 * KT - 1 > pfirst || gone) {
 #pragma unroll
@@ -358,7 +366,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
             for (int i = 0; i < 4; i++) {
               const int kk = key + (i & 1) + 8 * (i >> 1);
               v[i] = *reinterpret_cast<const float*>(kt_p + S::TILE + sw(kk, 2 * t + (gq >> 2)) + (gq & 3) * 4);
-              if (tail && cu.kt * C + kk >= cu.len) v[i] = 0.0f;
+              if (tail && kt * C + kk >= cu.len) v[i] = 0.0f;
             }
             uint32_t b0[3], b1[3];
             split_bf2<3>(v[0], v[1], b0);
@@ -399,18 +407,21 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[buf]);  // the stage is consumed
-    buf = buf + 1 == NS ? 0 : buf + 1;
+    if (++buf == NS) {
+      buf = 0;
+      par ^= 1;
+    }
+    }
 
-    const bool ends = cu.kt + 1 == cu.nt;
-    if (ends || u + 1 == units) {  // the piece is done: to the output when it is the whole item, else to the workspace
-      const bool whole = ends && unit0_kt == 0;
+    {  // the piece is done: to the output when it is the whole item, else to the workspace
+      const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
       // a piece from the item's start goes to the CTA's second place, one that enters the CTA to its first
-      const int slot = 2 * blockIdx.x + (unit0_kt == 0 ? 1 : 0);
+      const int slot = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
       float2* const pml = a.ml + (long)slot * a.tile_rows;
       float* const part = a.acc + (long)slot * a.tile_rows * HD;
-      if (!ends && unit0_kt == 0 && tid == 0) {
+      if (!ends && cu.kt == 0 && tid == 0) {
         AttnPart d;
-        d.pieces = attn_pieces(a, start, cu.nt - 1 - cu.kt);
+        d.pieces = attn_pieces(a, start, cu.nt - end);
         d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
         a.parts[blockIdx.x] = d;
       }
@@ -485,9 +496,10 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
           }
         }
       }
-      fresh = true;
     }
-    if (u + 1 < units) cu.next<R, C>(a);
+    u += end - cu.kt;
+    if (u == units) break;
+    cu = AttnCursor::next<R, C>(a, cu);
   }
 }
 

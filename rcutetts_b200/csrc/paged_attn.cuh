@@ -123,6 +123,7 @@ CTTS_DEV long attn_units(const PagedAttnArgs& a, const AttnReq& r) {
   const int mt = attn_row_tiles<R>(r, a.group);
   AttnRowWalk<R, C> w(r, a.group);
   long n = 0;
+#pragma unroll 1
   for (int m = 0; m < mt; m++, w.next()) n += w.tiles();
   return n * a.p.kv.n_kv_heads;
 }
@@ -153,36 +154,29 @@ struct AttnStart {
   AttnReq req;
 };
 
-// This CTA's piece of the line.  The block sums the requests' units, one
-// request a thread while the batch fits (else four a thread and turn); a
-// second pass finds the request the piece begins in, from registers when one
-// turn holds the batch.
+// This CTA's piece of the line.  The block sums the requests' units, a request
+// a thread and turn; a second pass finds the request the piece begins in (from
+// registers when one turn holds the batch).  (Code that runs once a launch is
+// kept small throughout these kernels: what does not fit the instruction cache
+// beside the main loop costs more than a rolled loop.)
 template <int R, int C, int NT>
 CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
-  constexpr int PER = 4, W = NT / 32;
+  constexpr int W = NT / 32;
   __shared__ long wsum[2][W];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.p.batch;
-  const int per = n <= NT ? 1 : PER;
-  long u[PER];
-  AttnReq rq[PER];
-  long total = 0, first = 0, mine_before = 0;
-  int ph = 0;
-  // one turn: units of requests base + tid*per + j; returns the turn's sum, mine_before = units ahead of the thread's
-  auto turn = [&](int base) {
-    long t = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int b = base + tid * per + j;
-      u[j] = 0;
-      if (j < per && b < n) rq[j] = attn_req(a, b);
+  long total = 0, first = 0, u0 = 0, u1 = 0;
+  AttnReq rq = {0, 0, 0, 0};
+  int ph = 0, pass = 0, base = 0;
+  while (true) {
+    // units of request base + tid, and those ahead of it in this turn
+    const int b = base + tid;
+    long u = 0;
+    if (b < n) {
+      rq = attn_req(a, b);
+      u = attn_units<R, C>(a, rq);
     }
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      if (j < per && base + tid * per + j < n) u[j] = attn_units<R, C>(a, rq[j]);
-      t += u[j];
-    }
-    long inc = t;
-#pragma unroll
+    long inc = u;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const long y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
@@ -190,39 +184,40 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
     if (lane == 31) wsum[ph][warp] = inc;
     __syncthreads();
     long all = 0, ahead = 0;
-#pragma unroll
+#pragma unroll 1
     for (int w = 0; w < W; w++) {
-      if (w < warp) ahead += wsum[ph][w];
-      all += wsum[ph][w];
+      const long y = wsum[ph][w];
+      if (w < warp) ahead += y;
+      all += y;
     }
-    mine_before = ahead + inc - t;
     ph ^= 1;
-    return all;
-  };
-  for (int base = 0; base < n; base += NT * per) total += turn(base);
-  const AttnCut cut(a.ctas, total);
-  const long u0 = cut.begin(blockIdx.x), u1 = cut.begin(blockIdx.x + 1);
-  if (tid == 0) {
-    out->units = u1 - u0;
-    out->end = u1;
-    out->total = total;
-  }
-  if (u1 > u0) {
-    for (int base = 0; base < n; base += NT * per) {
-      const long all = n <= NT * per ? total : turn(base);
-      long at = first + mine_before;
-#pragma unroll
-      for (int j = 0; j < PER; j++) {
-        if (at <= u0 && u0 < at + u[j]) {
-          out->b = base + tid * per + j;
-          out->skip = u0 - at;
-          out->req = rq[j];
-        }
-        at += u[j];
+    base += NT;
+    if (pass == 0) {
+      total += all;
+      if (base < n) continue;
+      const AttnCut cut(a.ctas, total);
+      u0 = cut.begin(blockIdx.x);
+      u1 = cut.begin(blockIdx.x + 1);
+      if (tid == 0) {
+        out->units = u1 - u0;
+        out->end = u1;
+        out->total = total;
       }
-      first += all;
-      if (first > u0) break;
+      if (u1 == u0) break;
+      if (n > NT) {
+        pass = 1;
+        base = 0;
+        continue;
+      }
     }
+    const long at = first + ahead + inc - u;
+    if (at <= u0 && u0 < at + u) {
+      out->b = b;
+      out->skip = u0 - at;
+      out->req = rq;
+    }
+    first += all;
+    if (first > u0) break;
   }
   __syncthreads();
 }
@@ -232,7 +227,8 @@ CTTS_DEV int attn_pieces(const PagedAttnArgs& a, const AttnStart& s, int more) {
   return AttnCut(a.ctas, s.total).owner(s.end + more - 1) - (int)blockIdx.x + 1;
 }
 
-// A place on the line: request, row tile, KV head, key tile.
+// A place on the line: request, row tile, KV head, key tile.  A role walks its
+// CTA's pieces: tiles kt .. nt of one item, then the next item's from 0.
 struct AttnCursor {
   int b, m, h, kt, nt, mt;
   int r0, cnt, nn, len;
@@ -242,16 +238,13 @@ struct AttnCursor {
     mt = (nn * a.group + R - 1) / R;
   }
   template <int R, int C>
-  CTTS_DEV void tiles(const PagedAttnArgs& a) {
-    nt = attn_tiles<R, C>(AttnReq{r0, cnt, nn, len}, m, a.group);
-  }
-  template <int R, int C>
-  static CTTS_DEV AttnCursor at(const PagedAttnArgs& a, const AttnStart& s) {
+  static __device__ __noinline__ AttnCursor at(const PagedAttnArgs& a, const AttnStart& s) {
     AttnCursor c;
     c.b = s.b;
     c.set(a, R, s.req);
     long skip = s.skip;
     AttnRowWalk<R, C> w(s.req, a.group);
+#pragma unroll 1
     for (c.m = 0;; c.m++, w.next()) {
       c.nt = w.tiles();
       const long in = (long)c.nt * a.p.kv.n_kv_heads;
@@ -262,24 +255,26 @@ struct AttnCursor {
     c.kt = (unsigned)skip % (unsigned)c.nt;
     return c;
   }
-  // (never called at the end of the line)
+  // The next item, from its first tile (never called at the end of the line).
   template <int R, int C>
-  CTTS_DEV void next(const PagedAttnArgs& a) {
-    if (++kt < nt) return;
-    kt = 0;
-    if (++h < a.p.kv.n_kv_heads) return;
-    h = 0;
-    if (++m < mt) {
-      tiles<R, C>(a);
-      return;
+  static __device__ __noinline__ AttnCursor next(const PagedAttnArgs& a, AttnCursor c) {
+    c.kt = 0;
+    if (++c.h < a.p.kv.n_kv_heads) return c;
+    c.h = 0;
+    if (++c.m == c.mt) {
+      c.m = 0;
+#pragma unroll 1
+      do {
+        c.b++;
+        c.set(a, R, attn_req(a, c.b));
+      } while (c.mt == 0 && c.b + 1 < a.p.batch);
     }
-    m = 0;
-    do {
-      b++;
-      set(a, R, attn_req(a, b));
-    } while (mt == 0 && b + 1 < a.p.batch);
-    tiles<R, C>(a);
+    c.nt = attn_tiles<R, C>(AttnReq{c.r0, c.cnt, c.nn, c.len}, c.m, a.group);
+    return c;
   }
+  // Packed rows of the item, and the position of the request's first new row.
+  CTTS_DEV int rows(const PagedAttnArgs& a, int R) const { return min(R, nn * a.group - m * R); }
+  CTTS_DEV int pos0() const { return len - cnt; }
 };
 
 // The pool as a 4D tensor map: 128 bytes of a head by `box` slots a copy, the
@@ -297,6 +292,24 @@ CTTS_DEV void copy_box(uint32_t dst, const CUtensorMap* m, int order, int x, int
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
+}
+// Whether the phase with this parity is over.
+CTTS_DEV bool mbar_try(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+// Bounded wait, and a flag for all roles when it gives up: nobody waits after
+// that, the block runs to its end.
+CTTS_DEV void mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  if (mbar_try(bar, parity)) return;
+#pragma unroll 1
+  for (uint32_t it = 0; it < kWaitLimit && !*gave_up; ++it)
+    if (mbar_try(bar, parity)) return;
+  *gave_up = 1;
 }
 CTTS_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -19,8 +19,10 @@
 // and the pass over O in TMEM becomes rare.  S(j+1) of a sub-tile is issued
 // behind P.V(j), so O is at rest while its softmax threads hold S.
 //
+// P arrives in two halves, so P.V begins over the second half's exponentials.
+//
 // float32 queries: queries and weights enter as three bf16 terms (24 bits),
-// key tiles are 64 wide so that three terms of the weights fit over S.  Each
+// key tiles are 64 wide so that three terms of the weights fit beside S.  Each
 // P.V starts at zero and its threads add it to an output row in registers:
 // the tensor core cuts the sums it accumulates instead of rounding them, which
 // over a thousand keys costs 2^-18 of the output (measured against 64 bits).
@@ -39,44 +41,50 @@ namespace ctts {
 namespace {
 
 // Warps: 4 of softmax per sub-tile, then one that issues MMAs and one that
-// issues copies (the block is rounded up to whole warpgroups).  Two softmax
-// warpgroups take registers from the third: 2 x 216 + 72 = 3 x 168.
+// issues copies.
 template <bool QF, int HD>
 struct TcShape {
-  static constexpr int THREADS = QF && HD == 128 ? 256 : 384;
-  static constexpr bool REGS = THREADS == 384;
-  static constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 216, OTHER_REGS = 72;
   static constexpr int KT = QF ? 64 : 128;                // keys per tile
   static constexpr int NSUB = QF && HD == 128 ? 1 : 2;    // three terms of 256 wide queries would not fit
   static constexpr int R = 128 * NSUB;                    // packed rows per item
+  static constexpr int THREADS = R + 64;
   static constexpr int NT = QF ? 3 : 1;                   // terms of queries and weights
   static constexpr int NC = HD / 64;                      // 128-byte column blocks
+  // TMEM columns of sub-tile s: S at s * SREG, P over it (bf16) or behind it
+  // (three terms of KT / 2 columns), O at OREG + s * OSTEP
+  static constexpr uint32_t SREG = QF ? 192 : 128, PCOL = QF ? KT : 0, OREG = QF && NSUB == 2 ? 384 : 256, OSTEP = QF ? 64 : 128;
+  static_assert(OREG + (NSUB - 1) * OSTEP + HD <= 512 && PCOL + NT * (KT / 2) <= SREG && NSUB * SREG <= OREG, "TMEM columns");
   static constexpr uint32_t QTERM = NC * 128 * 128;       // bytes of one term of one sub-tile
   static constexpr uint32_t TILE = NC * KT * 128;         // bytes of a K or V tile
   static constexpr int NS = QF ? (HD == 64 ? 6 : 3) : (HD == 64 ? 4 : 2);
   static constexpr size_t SMEM = (size_t)NSUB * NT * QTERM + (size_t)2 * NS * TILE + 1024;
 };
 
-// Shared-memory descriptor of a 128-byte swizzled operand.  K-major: lbo
-// unused (1).  MN-major: rows of 64 dims per key, `lbo` bytes between blocks
-// of 64 dims, 1024 bytes between groups of 8 keys.
-CTTS_DEV uint64_t tc_desc(uint32_t saddr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)(lbo >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
-}
+// Shared-memory descriptors of 128-byte swizzled operands, as their two words.
+// K-major: the field for the leading distance is unused (1).  MN-major: rows
+// of 64 dims per key, `lbo` bytes between blocks of 64 dims.  Both: 1024 bytes
+// between groups of 8 rows.  An operand d bytes on: the low word + d / 16.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+CTTS_DEV uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 // D f32, A and B bf16, M = 128, N = n; B K-major or MN-major
 CTTS_DEV constexpr uint32_t tc_idesc(int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-CTTS_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {  // A from TMEM
+CTTS_DEV void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi));
+}
+CTTS_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {  // A from TMEM
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi));
+}
+// True in one lane of the warp.
+CTTS_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 CTTS_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 CTTS_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -101,26 +109,80 @@ CTTS_DEV void tmem_st32(uint32_t taddr, const uint32_t* r) {
   tmem_st16(taddr + 16, r + 16);
 }
 
+CTTS_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Pairs of float32 in one instruction.
+CTTS_DEV float2 fma2(float2 x, float a, float b) {  // x * a + b
+  float2 r;
+  asm("{\n\t.reg .b64 x, a, b;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 a, {%4, %4};\n\tmov.b64 b, {%5, %5};\n\t"
+      "fma.rn.f32x2 x, x, a, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(a), "f"(b));
+  return r;
+}
+CTTS_DEV float2 fma2(float2 x, float2 y, float b) {  // x * y + b
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, b;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 b, {%6, %6};\n\t"
+      "fma.rn.f32x2 x, x, y, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(b));
+  return r;
+}
+CTTS_DEV float2 add2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return r;
+}
+// 2^x for a pair of x <= 127 without the special function unit, which makes
+// four results a clock and scheduler and is what the softmax of bf16 calls
+// waits for: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it
+// in the low bits) and |f| <= 1/2, 2^f by its cubic of least relative error
+// (a weighted least-squares fit; off by 7.5e-5, a fiftieth of the rounding to
+// bf16 that follows), n added to the exponent.  Below 2^-126: 2^-126.
+CTTS_DEV float2 exp2_poly(float2 x) {
+  constexpr float kMagic = 12582912.0f;
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 t = add2(x, make_float2(kMagic, kMagic));
+  const float2 n = add2(t, make_float2(-kMagic, -kMagic));
+  const float2 f = add2(x, make_float2(-n.x, -n.y));
+  float2 r = fma2(f, 0.0551716685f, 0.2426111251f);
+  r = fma2(r, f, 0.6932609677f);
+  r = fma2(r, f, 0.9999280572f);
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+
+// Of the 16 pairs of a turn, every kPolyEvery-th by exp2_poly (0: none).
+constexpr int kPolyEvery = 4;
+
 struct TcBars {
   uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], drain;
 };
 
 template <bool QF, int HD>
 __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                                      const __grid_constant__ CUtensorMap tmV, const PagedAttnArgs a,
-                                                                      int box, int order) {
+                                                                                    const __grid_constant__ CUtensorMap tmV,
+                                                                                    const __grid_constant__ PagedAttnArgs a, int box, int order) {
   using S = TcShape<QF, HD>;
   constexpr int KT = S::KT, R = S::R, NS = S::NS, NT = S::NT, NC = S::NC;
   constexpr int W_MMA = 4 * S::NSUB, W_TMA = W_MMA + 1;
+  constexpr int KS = KT / 16, HALF = QF ? 0 : KS / 2;  // bf16 calls: P arrives in two halves
   extern __shared__ uint8_t tc_smem[];
   __shared__ AttnStart start;
   __shared__ __align__(8) TcBars bars;
   __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t dead_keys[8];  // 8-key groups of a tile whose page does not exist
   __shared__ volatile int gave_up;
   const uint32_t sbase = (smem_u32(tc_smem) + 1023u) & ~1023u;
   const uint32_t qs = sbase, ks = qs + S::NSUB * NT * S::QTERM, vs = ks + NS * S::TILE;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
@@ -132,6 +194,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     for (int i = 0; i < 2; i++) {
       mbar_init(&bars.q_full[i], 128);
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], 128);
       mbar_init(&bars.p_full[i], 128);
       mbar_init(&bars.o_full[i], 1);
     }
@@ -145,285 +208,300 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   }
   grid_dep_enter();
   attn_find_start<R, KT, S::THREADS>(a, &start);
+  if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;  // S and P of sub-tile s at column 128 s, O at 256 + 128 s
-  const long units = start.units;
-  if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
-  __syncthreads();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+  const int units = __shfl_sync(0xffffffffu, (int)start.units, 0);  // (of one CTA: 31 bits, the host checks)
 
-  if (warp >= W_MMA) {
-    if (S::REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::OTHER_REGS));
-    if (units > 0 && warp == W_TMA) {
-      // ---- producer: lane i copies page box i of each tile
-      AttnCursor cu = AttnCursor::at<R, KT>(a, start);
-      const int nbox = KT / box;
-      long u = 0;
-      for (; u < units; u++) {
-        const int st = (int)(u % NS);
-        const uint32_t par = (uint32_t)((u / NS) & 1);
-        const int kk = cu.kt * KT + lane * box;
-        int page = -1;
-        if (lane < nbox && kk < cu.len) page = a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)];
-        if ((unsigned)page >= (unsigned)a.p.kv.n_pages) page = a.p.kv.n_pages;  // outside the map: zeros
-        const int slot = kk & (a.p.kv.page_size - 1);
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++) {
-          uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-          if (u >= NS && !mbar_wait(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1)) gave_up = 1;
-          if (__any_sync(0xffffffffu, gave_up)) goto produced;
-          if (lane == 0) mbar_expect_tx(full, S::TILE);
-          __syncwarp();
-          if (lane < nbox) {
-            const uint32_t dst = (kv ? vs : ks) + st * S::TILE + (uint32_t)(lane * box) * 128u;
-#pragma unroll
-            for (int c = 0; c < NC; c++) copy_box(dst + c * KT * 128, kv ? &tmV : &tmK, order, c * 64, slot, cu.h, page, full);
-          }
+  if (units > 0 && warp == W_TMA) {
+    // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
+    // lanes at the boxes' starts copy them
+    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    int kt = cu.kt;
+    auto page_of = [&]() {
+      const int kk = kt * KT + 8 * lane;
+      return lane < KT / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
+    };
+    int page = page_of(), st = 0, u = 0;
+    uint32_t par = 0;
+#pragma unroll 1
+    for (; u < units && !gave_up; u++) {
+      const int kk = kt * KT + 8 * lane, h = cu.h, slot = kk & (a.p.kv.page_size - 1);
+      const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
+      const uint32_t dead = __ballot_sync(0xffffffffu, lane < KT / 8 && kk < cu.len && none);
+      const int from = none ? a.p.kv.n_pages : page;  // outside the map: zeros
+      if (u + 1 < units) {  // the next tile's pages, over the waits
+        if (++kt == cu.nt) {
+          cu = AttnCursor::next<R, KT>(a, cu);
+          kt = 0;
         }
-        if (u + 1 < units) cu.next<R, KT>(a);
+        page = page_of();
       }
-    produced:
-      __syncwarp();
-      if (gave_up)  // copies in flight land before the block may leave
-        for (long w = u > NS ? u - NS : 0; w <= u && w < units; w++) {
-          mbar_wait(&bars.k_full[w % NS], (uint32_t)((w / NS) & 1));
-          mbar_wait(&bars.v_full[w % NS], (uint32_t)((w / NS) & 1));
+      const bool copies = lane < KT / 8 && (8 * lane & (box - 1)) == 0;
+#pragma unroll 1
+      for (int kv = 0; kv < 2; kv++) {
+        uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
+        if (u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &gave_up);
+        if (lane == 0) {
+          if (kv == 0) dead_keys[u & 7] = dead;  // read behind the scores' barrier; the copies are at most 6 tiles ahead
+          mbar_expect_tx(full, S::TILE);
         }
-    } else if (units > 0 && warp == W_MMA) {
-      // ---- MMA issue (one thread)
-      if (lane == 0) {
-        AttnCursor cu = AttnCursor::at<R, KT>(a, start);
-        uint32_t q_par = 0, p_par = 0;  // one bit per sub-tile
-        auto wait = [&](uint64_t* bar, uint32_t par) {
-          if (gave_up || !mbar_wait(bar, par)) gave_up = 1;
-          fence_after();
-          return !gave_up;
-        };
-        auto scores = [&](int s, int st) {
-          // (opaque: the descriptors are made as they are used, not kept in
-          // registers over the loop)
-          uint32_t kb = ks + st * S::TILE, qb = qs + s * NT * S::QTERM, acc = 0;
-          asm volatile("" : "+r"(kb), "+r"(qb));
-          // small terms first: the tensor core cuts what it adds to the
-          // accumulator's precision
-#pragma unroll
-          for (int t = NT - 1; t >= 0; t--)
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-              for (int k = 0; k < 4; k++) {
-                umma_bf16(tmem + 128 * s, tc_desc(qb + t * S::QTERM + c * 16384 + k * 32, 16),
-                          tc_desc(kb + c * KT * 128 + k * 32, 16), tc_idesc(KT, false), acc);
-                acc = 1;
-              }
-          umma_commit(&bars.s_full[s]);
-        };
-        auto values = [&](int s, int st, uint32_t acc) {
-          uint32_t vb = vs + st * S::TILE;
-          asm volatile("" : "+r"(vb));
-#pragma unroll
-          for (int t = NT - 1; t >= 0; t--)
-#pragma unroll
-            for (int k = 0; k < KT / 16; k++) {
-              mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + t * (KT / 2) + k * 8, tc_desc(vb + k * 2048, KT * 128), tc_idesc(HD, true), acc);
-              acc = 1;
-            }
-        };
-        bool fresh = true, ok = true;
-        int nsub = 1;
-        for (long u = 0; u < units && ok; u++) {
-          const int st = (int)(u % NS);
-          if (fresh) {  // a piece begins: its first scores
-            nsub = min(R, cu.nn * a.group - cu.m * R) > 128 ? 2 : 1;
-            ok = wait(&bars.k_full[st], (uint32_t)((u / NS) & 1));
-            for (int s = 0; s < nsub && ok; s++) {
-              ok = wait(&bars.q_full[s], (q_par >> s) & 1);
-              q_par ^= 1u << s;
-              if (ok) scores(s, st);
-            }
-            if (!ok) break;
-            umma_commit(&bars.k_empty[st]);
-          }
-          const bool last = cu.kt + 1 == cu.nt || u + 1 == units;
-          ok = wait(&bars.v_full[st], (uint32_t)((u / NS) & 1));
-          const int sn = (int)((u + 1) % NS);
-          if (ok && !last) ok = wait(&bars.k_full[sn], (uint32_t)(((u + 1) / NS) & 1));
-          for (int s = 0; s < nsub && ok; s++) {
-            ok = wait(&bars.p_full[s], (p_par >> s) & 1);
-            p_par ^= 1u << s;
-            if (!ok) break;
-            values(s, st, fresh || QF ? 0u : 1u);
-            if (last)
-              umma_commit(&bars.o_full[s]);
-            else
-              scores(s, sn);
-          }
-          if (!ok) break;
-          umma_commit(&bars.v_empty[st]);
-          if (!last) umma_commit(&bars.k_empty[sn]);
-          fresh = last;
-          if (u + 1 < units) cu.next<R, KT>(a);
-        }
-        if (!ok) {  // MMAs in flight end before TMEM is given back
-          umma_commit(&bars.drain);
-          mbar_wait(&bars.drain, 0);
+        __syncwarp();
+        if (copies) {
+          const uint32_t dst = (kv ? vs : ks) + st * S::TILE + (uint32_t)lane * 1024u;
+#pragma unroll 1
+          for (int c = 0; c < NC; c++) copy_box(dst + c * KT * 128, kv ? &tmV : &tmK, order, c * 64, slot, h, from, full);
         }
       }
-      __syncwarp();
+      if (++st == NS) {
+        st = 0;
+        par ^= 1;
+      }
     }
-  } else {
-    if (S::REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::SOFTMAX_REGS));
-    if (units > 0) {
-      // ---- softmax: one thread per packed row
-      const int s = warp >> 2, row = (warp & 3) * 32 + lane;
-      const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t tS = tmem + 128 * s + lane_base, tO = tmem + 256 + 128 * s + lane_base;
-      const float c2 = a.c2_hi;
-      AttnCursor cu = AttnCursor::at<R, KT>(a, start);
-      uint32_t s_par = 0, o_par = 0;
-      bool fresh = true, ok = true;
-      int kt0 = 0, nrows = 0, pk = 0, pos = 0, pos_lo = 0;
-      bool mine = false, warp_on = false, on = false;
-      float m = -INFINITY, l = 0.0f;
-      float o_row[QF ? HD : 1];  // float32 calls: the output row so far
-      // adds the product of the last tile to it
-      auto gather = [&]() {
+    if (gave_up)  // copies in flight land before the block may leave
+      for (int w = max(0, u - NS); w < u; w++) {
+        mbar_wait(&bars.k_full[w % NS], (uint32_t)(w / NS) & 1);
+        mbar_wait(&bars.v_full[w % NS], (uint32_t)(w / NS) & 1);
+      }
+  } else if (units > 0 && warp == W_MMA) {
+    // ---- MMA issue.  The warp runs through as one (what it computes with is
+    // uniform), one lane issues; between its products it does next to nothing:
+    // what it spends there the tensor core stands still.
+    const bool leader = elect_one();
+    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    auto scores = [&](int s, int st) {
+      const uint32_t kb = desc_lo(ks + st * S::TILE, 16), qb = desc_lo(qs + s * NT * S::QTERM, 16);
+      fence_after();
+      if (leader) {
+        // small terms first: the tensor core cuts what it adds to the
+        // accumulator's precision
 #pragma unroll
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
-          tmem_ld32_nowait(tO + c, o);
-          tmem_wait();
-          pin32(o);
+        for (int t = NT - 1; t >= 0; t--)
 #pragma unroll
-          for (int j = 0; j < 32; j++) o_row[QF ? c + j : 0] += __uint_as_float(o[j]);
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              mma_ss(tmem + S::SREG * s, qb + (t * S::QTERM + c * 16384 + k * 32) / 16, kb + (c * KT * 128 + k * 32) / 16, tc_idesc(KT, false),
+                     t < NT - 1 || c > 0 || k > 0);
+        umma_commit(&bars.s_full[s]);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int s, int st, int k0, int k1, uint32_t acc) {
+      const uint32_t vb = desc_lo(vs + st * S::TILE, KT * 128);
+      fence_after();
+      if (leader) {
+#pragma unroll
+        for (int t = NT - 1; t >= 0; t--)
+#pragma unroll
+          for (int k = k0; k < k1; k++)
+            mma_ts(tmem + S::OREG + S::OSTEP * s, tmem + S::SREG * s + S::PCOL + t * (KT / 2) + k * 8, vb + k * 128, tc_idesc(HD, true),
+                   t < NT - 1 || k > k0 ? 1u : acc);
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    uint32_t q_par = 0, p_par = 0;  // one bit per sub-tile
+    uint32_t par = 0, par_p = 0;    // of the fills of stages st (tile i) and sp (tile i - 1)
+    int st = 0, sp = 0, done = 0;
+#pragma unroll 1
+    while (true) {
+      const int n = __shfl_sync(0xffffffffu, min(cu.nt - cu.kt, units - done), 0);
+      const int nsub = __shfl_sync(0xffffffffu, cu.rows(a, R) > 128 ? 2 : 1, 0);
+      // a turn: P.V of tile i - 1, scores of tile i
+#pragma unroll 1
+      for (int i = 0; i <= n; i++) {
+        if (i > 0) mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+#pragma unroll 1
+        for (int s = 0; s < nsub; s++) {
+          if (i > 0) {
+            if (HALF) {
+              mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
+              values(s, sp, 0, HALF, i > 1);
+            }
+            mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
+            p_par ^= 1u << s;
+            values(s, sp, HALF, KS, HALF ? 1u : 0u);
+            if (i == n) commit(&bars.o_full[s]);
+          }
+          if (i < n) {
+            if (i == 0) {
+              mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
+              q_par ^= 1u << s;
+            }
+            if (s == 0) mbar_wait_or(&bars.k_full[st], par, &gave_up);
+            scores(s, st);
+          }
         }
-      };
-      for (long u = 0; u < units && ok; u++) {
-        if (fresh) {
-          fresh = false;
-          kt0 = cu.kt;
-          nrows = min(R, cu.nn * a.group - cu.m * R);
-          on = s * 128 < nrows;  // the sub-tile has rows
-          mine = s * 128 + row < nrows;
-          warp_on = s * 128 + (warp & 3) * 32 < nrows;
-          pk = cu.m * R + s * 128 + row;
-          pos = cu.len - cu.cnt + pk / a.group;
-          pos_lo = cu.len - cu.cnt + (pk - lane) / a.group;
-          m = -INFINITY;
-          l = 0.0f;
+        if (i > 0) commit(&bars.v_empty[sp]);
+        if (i < n) {
+          commit(&bars.k_empty[st]);
+          sp = st;
+          par_p = par;
+          if (++st == NS) {
+            st = 0;
+            par ^= 1;
+          }
+        }
+      }
+      done += n;
+      if (done == units) break;
+      cu = AttnCursor::next<R, KT>(a, cu);
+    }
+    if (gave_up) {  // MMAs in flight end before TMEM is given back
+      commit(&bars.drain);
+      mbar_wait(&bars.drain, 0);
+    }
+  } else if (units > 0 && warp < W_MMA) {
+    // ---- softmax: one thread per packed row
+    const int s = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + S::SREG * s + lane_base, tP = tS + S::PCOL, tO = tmem + S::OREG + S::OSTEP * s + lane_base;
+    const float c2 = a.c2_hi;
+    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    uint32_t s_par = 0, o_par = 0;
+    float o_row[QF ? HD : 1];  // float32 calls: the output row so far
+    // adds the product of the last tile to it
+    auto gather = [&]() {
 #pragma unroll
-          for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] = 0.0f;
-          if (on) {
-            // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes
-            // of a row (as bf16), four rows at a time, all loads in flight
-            // before the first is used; rows behind the item are zero
-            const int r0 = (warp & 3) * 32, p0 = cu.m * R + s * 128 + r0;
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        tmem_ld32_nowait(tO + c, o);
+        tmem_wait();
+        pin32(o);
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-              constexpr int RP = 8;  // rows a lane reads: 4 i + lane / 8
-              uint4 x[RP], y[QF ? RP : 1];
+        for (int j = 0; j < 32; j++) o_row[QF ? c + j : 0] += __uint_as_float(o[j]);
+      }
+    };
+    int u = 0;
+#pragma unroll 1
+    while (true) {
+      // ---- a piece: tiles cu.kt .. end of an item
+      const int end = min(cu.nt, cu.kt + units - u), nrows = cu.rows(a, R);
+      if (s * 128 < nrows) {  // the sub-tile has rows
+        const int r0 = s * 128 + (warp & 3) * 32;  // the warp's first row in the item
+        const bool mine = s * 128 + row < nrows, warp_on = r0 < nrows;
+        const int pk = cu.m * R + s * 128 + row;
+        const int pos = cu.pos0() + pk / a.group, pos_lo = cu.pos0() + (pk - lane) / a.group;
+        // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes of a
+        // row (as bf16), four rows at a time, all loads in flight before the
+        // first is used; rows behind the item are zero
+#pragma unroll 1
+        for (int c = 0; c < NC; c++) {
+          constexpr int RP = 8;  // rows a lane reads: 4 i + lane / 8
+          uint4 x[RP], y[QF ? RP : 1];
 #pragma unroll
-              for (int i = 0; i < RP; i++) {
-                const int r = 4 * i + (lane >> 3), p = p0 + r;
-                x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (QF) y[QF ? i : 0] = x[i];
-                if (s * 128 + r0 + r < nrows) {
-                  const int tok = p / a.group;
-                  const long at = (long)(cu.r0 + tok) * a.p.q_ld + (cu.h * a.group + p - tok * a.group) * HD + c * 64 + (lane & 7) * 8;
-                  if (QF) {
-                    x[i] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at);
-                    y[QF ? i : 0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at + 4);
-                  } else {
-                    x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
-                  }
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < RP; i++) {
-                const int r = r0 + 4 * i + (lane >> 3);
-                uint32_t t[4][NT];
-                if (QF) {
-                  const uint4 z = y[QF ? i : 0];
-                  split_bf2<NT>(__uint_as_float(x[i].x), __uint_as_float(x[i].y), t[0]);
-                  split_bf2<NT>(__uint_as_float(x[i].z), __uint_as_float(x[i].w), t[1]);
-                  split_bf2<NT>(__uint_as_float(z.x), __uint_as_float(z.y), t[2]);
-                  split_bf2<NT>(__uint_as_float(z.z), __uint_as_float(z.w), t[3]);
-                } else {
-                  t[0][0] = x[i].x; t[1][0] = x[i].y; t[2][0] = x[i].z; t[3][0] = x[i].w;
-                }
-                const uint32_t dst = qs + s * NT * S::QTERM + c * 16384 + r * 128 + (uint32_t)(((lane ^ r) & 7) << 4);
-#pragma unroll
-                for (int k = 0; k < NT; k++)
-                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + k * S::QTERM), "r"(t[0][k]), "r"(t[1][k]), "r"(t[2][k]),
-                               "r"(t[3][k])
-                               : "memory");
+          for (int i = 0; i < RP; i++) {
+            const int r = r0 + 4 * i + (lane >> 3), p = cu.m * R + r;
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (QF) y[QF ? i : 0] = x[i];
+            if (r < nrows) {
+              const int tok = p / a.group;
+              const long at = (long)(cu.r0 + tok) * a.p.q_ld + (cu.h * a.group + p - tok * a.group) * HD + c * 64 + (lane & 7) * 8;
+              if (QF) {
+                x[i] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at);
+                y[QF ? i : 0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at + 4);
+              } else {
+                x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
               }
             }
-            fence_async();
-            mbar_arrive(&bars.q_full[s]);
+          }
+#pragma unroll
+          for (int i = 0; i < RP; i++) {
+            const int r = (warp & 3) * 32 + 4 * i + (lane >> 3);
+            uint32_t t[4][NT];
+            if (QF) {
+              const uint4 z = y[QF ? i : 0];
+              split_bf2<NT>(__uint_as_float(x[i].x), __uint_as_float(x[i].y), t[0]);
+              split_bf2<NT>(__uint_as_float(x[i].z), __uint_as_float(x[i].w), t[1]);
+              split_bf2<NT>(__uint_as_float(z.x), __uint_as_float(z.y), t[2]);
+              split_bf2<NT>(__uint_as_float(z.z), __uint_as_float(z.w), t[3]);
+            } else {
+              t[0][0] = x[i].x; t[1][0] = x[i].y; t[2][0] = x[i].z; t[3][0] = x[i].w;
+            }
+            const uint32_t dst = qs + s * NT * S::QTERM + c * 16384 + r * 128 + (uint32_t)(((lane ^ r) & 7) << 4);
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + k * S::QTERM), "r"(t[0][k]), "r"(t[1][k]), "r"(t[2][k]),
+                           "r"(t[3][k])
+                           : "memory");
           }
         }
-        const bool ends = cu.kt + 1 == cu.nt, last = ends || u + 1 == units;
-        if (on) {
-          const int key0 = cu.kt * KT;
-          // 8-key groups whose page does not exist
-          uint32_t dead = 0;
-          {
-            const int kk = key0 + lane * 8;
-            bool d = false;
-            if (lane < KT / 8 && kk < cu.len)
-              d = (unsigned)a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] >= (unsigned)a.p.kv.n_pages;
-            dead = __ballot_sync(0xffffffffu, d);
-          }
+        fence_async();
+        mbar_arrive(&bars.q_full[s]);
+
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] = 0.0f;
+#pragma unroll 1
+        for (int kt = cu.kt; kt < end; kt++) {
+          const int key0 = kt * KT;
           if (s == 0 && key0 + KT > cu.len) {
             // slots behind the length may hold anything, and 0 * NaN is NaN:
             // their values become zeros (both sub-tiles' products come after
-            // this sub-tile's arrival at p_full)
-            const int st = (int)(u % NS);
-            if (!mbar_wait(&bars.v_full[st], (uint32_t)((u / NS) & 1))) gave_up = 1;
+            // this sub-tile's arrival at p_half or p_full)
+            const int w = u + kt - cu.kt, st = w % NS;
+            mbar_wait_or(&bars.v_full[st], (uint32_t)(w / NS) & 1, &gave_up);
             if (row < KT && key0 + row >= cu.len) {
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < NC * 8; c++)
                 asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs + st * S::TILE + (c >> 3) * KT * 128 + row * 128 + (c & 7) * 16), "r"(0)
                              : "memory");
             }
             fence_async();
           }
-          if (!mbar_wait(&bars.s_full[s], s_par)) gave_up = 1;
+          mbar_wait_or(&bars.s_full[s], s_par, &gave_up);
           s_par ^= 1;
-          if (__any_sync(0xffffffffu, gave_up)) {
-            ok = false;
-            break;
-          }
           if (warp_on) {
             fence_after();
-            uint32_t x[KT];
-#pragma unroll
-            for (int c = 0; c < KT; c += 32) tmem_ld32_nowait(tS + c, x + c);
-            tmem_wait();
-#pragma unroll
-            for (int c = 0; c < KT; c += 32) pin32(x + c);
+            const uint32_t dead = dead_keys[(u + kt - cu.kt) & 7];
             if (key0 + KT - 1 > pos_lo || dead) {
-              const int lim = pos - key0;
+              // hidden keys: -inf over their scores
+#pragma unroll 1
+              for (int c = 0; c < KT; c += 32) {
+                uint32_t x[32];
+                tmem_ld32_nowait(tS + c, x);
+                tmem_wait();
+                pin32(x);
 #pragma unroll
-              for (int c = 0; c < KT; c++)
-                if (c > lim || ((dead >> (c >> 3)) & 1)) x[c] = 0xff800000u;  // -inf
+                for (int g = 0; g < 4; g++) {
+                  const int lim = (dead >> (c / 8 + g)) & 1 ? -1 : pos - key0 - c - 8 * g;  // the last key of the eight that is seen
+#pragma unroll
+                  for (int j = 0; j < 8; j++)
+                    if (j > lim) x[8 * g + j] = 0xff800000u;
+                }
+                tmem_st32(tS + c, x);
+              }
+              tmem_st_wait();
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mn;
+            {
+              uint32_t x[KT];
 #pragma unroll
-            for (int c = 0; c < KT; c += 4)
+              for (int c = 0; c < KT; c += 32) tmem_ld32_nowait(tS + c, x + c);
+              tmem_wait();
 #pragma unroll
-              for (int j = 0; j < 4; j++) mx[j] = fmaxf(mx[j], __uint_as_float(x[c + j]));
-            const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+              for (int c = 0; c < KT; c += 32) pin32(x + c);
+              float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int c = 0; c < KT; c += 8)
+#pragma unroll
+                for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], __uint_as_float(x[c + 2 * j]), __uint_as_float(x[c + 2 * j + 1]));
+              mn = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * c2;
+            }
             if (QF) {
-              if (cu.kt > kt0) gather();
+              if (kt > cu.kt) gather();
               const float mm = fmaxf(m, mn), f = mm == -INFINITY ? 0.0f : exp2_fast(m - mm);
               m = mm;
               l *= f;
 #pragma unroll
               for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] *= f;
-            } else if (cu.kt == kt0) {
+            } else if (kt == cu.kt) {
               m = mn;  // O is overwritten by the first product
             } else {
               const bool grow = mn > m + 8.0f;
@@ -445,87 +523,138 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
               }
             }
             const float mz = m == -INFINITY ? 0.0f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // the weights, 32 keys at a time from scores read again (bf16
+            // calls: over scores already read)
+            if (QF) {
+              float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+              for (int c = 0; c < KT; c += 32) {
+                uint32_t x[32], p[NT][16];
+                tmem_ld32_nowait(tS + c, x);
+                tmem_wait();
+                pin32(x);
 #pragma unroll
-            for (int c = 0; c < KT; c += 32) {
-              uint32_t p[NT][16];
+                for (int j = 0; j < 32; j += 2) {
+                  const float e0 = exp2_fast(attn_arg<true>(a, __uint_as_float(x[j]), mz));
+                  const float e1 = exp2_fast(attn_arg<true>(a, __uint_as_float(x[j + 1]), mz));
+                  sum[0] += e0;
+                  sum[1] += e1;
+                  uint32_t t[NT];
+                  split_bf2<NT>(e0, e1, t);
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float e0 = exp2_fast(attn_arg<QF>(a, __uint_as_float(x[c + j]), mz));
-                const float e1 = exp2_fast(attn_arg<QF>(a, __uint_as_float(x[c + j + 1]), mz));
-                sum[j & 2] += e0;
-                sum[(j & 2) + 1] += e1;
-                uint32_t t[NT];
-                split_bf2<NT>(e0, e1, t);
+                  for (int k = 0; k < NT; k++) p[k][j >> 1] = t[k];
+                }
 #pragma unroll
-                for (int k = 0; k < NT; k++) p[k][j >> 1] = t[k];
+                for (int k = 0; k < NT; k++) tmem_st16(tP + k * (KT / 2) + (c >> 1), p[k]);
               }
+              l += sum[0] + sum[1];
+            } else {
+              float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+              auto weights = [&](const uint32_t* x, int c) {
+                uint32_t p[16];
 #pragma unroll
-              for (int k = 0; k < NT; k++) tmem_st16(tS + k * (KT / 2) + (c >> 1), p[k]);
+                for (int j = 0; j < 16; j++) {
+                  float2 e = fma2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, -mz);
+                  if (kPolyEvery && j % (kPolyEvery + !kPolyEvery) == kPolyEvery - 1)
+                    e = exp2_poly(e);
+                  else
+                    e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                  sum[j & 1] = add2(sum[j & 1], e);
+                  p[j] = pack_bf2(e.x, e.y);
+                }
+                tmem_st16(tP + (c >> 1), p);
+              };
+              uint32_t x[32], y[32];
+              tmem_ld32_nowait(tS, x);
+              tmem_wait();
+              pin32(x);
+#pragma unroll 1
+              for (int c = 0; c < KT; c += 64) {
+                tmem_ld32_nowait(tS + c + 32, y);
+                weights(x, c);
+                tmem_wait();
+                pin32(y);
+                if (c + 64 < KT) tmem_ld32_nowait(tS + c + 64, x);
+                weights(y, c + 32);
+                if (c + 64 < KT) {
+                  tmem_wait();
+                  pin32(x);
+                  tmem_st_wait();
+                  fence_before();
+                  mbar_arrive(&bars.p_half[s]);
+                }
+              }
+              l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tmem_st_wait();
             fence_before();
+          } else if (!QF) {
+            mbar_arrive(&bars.p_half[s]);
           }
           mbar_arrive(&bars.p_full[s]);
+        }
 
-          if (last) {
-            const bool whole = ends && kt0 == 0;
-            const int slot = 2 * blockIdx.x + (kt0 == 0 ? 1 : 0);
-            if (!ends && kt0 == 0 && s == 0 && row == 0) {
-              AttnPart d;
-              d.pieces = attn_pieces(a, start, cu.nt - 1 - cu.kt);
-              d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
-              a.parts[blockIdx.x] = d;
+        // ---- the piece's output, or its partial state
+        const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
+        const int place = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
+        if (!ends && cu.kt == 0 && s == 0 && row == 0) {
+          AttnPart d;
+          d.pieces = attn_pieces(a, start, cu.nt - end);
+          d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
+          a.parts[blockIdx.x] = d;
+        }
+        mbar_wait_or(&bars.o_full[s], o_par, &gave_up);
+        o_par ^= 1;
+        if (warp_on) {
+          fence_after();
+          const bool none = m == -INFINITY;  // the row saw no key
+          const float inv = whole ? 1.0f / l : 1.0f;
+          const int tok = pk / a.group;
+          const long at = (long)(cu.r0 + tok) * a.p.out_ld + (cu.h * a.group + pk - tok * a.group) * HD;
+          const long pr = (long)place * a.tile_rows + s * 128 + row;
+          if (!whole && mine) a.ml[pr] = make_float2(m, l);
+          if (QF) gather();
+          auto put = [&](int c, const uint32_t* o) {
+            if (!mine) return;
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = none ? 0.0f : __uint_as_float(o[j]) * inv;
+            if (whole && !QF) {
+              uint16_t* w = static_cast<uint16_t*>(a.p.out) + at + c;
+#pragma unroll
+              for (int j = 0; j < 32; j += 8)
+                *reinterpret_cast<uint4*>(w + j) = make_uint4(pack_bf2(v[j], v[j + 1]), pack_bf2(v[j + 2], v[j + 3]),
+                                                              pack_bf2(v[j + 4], v[j + 5]), pack_bf2(v[j + 6], v[j + 7]));
+            } else {
+              float* w = whole ? static_cast<float*>(a.p.out) + at + c : a.acc + pr * HD + c;
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             }
-            if (!mbar_wait(&bars.o_full[s], o_par)) gave_up = 1;
-            o_par ^= 1;
-            if (__any_sync(0xffffffffu, gave_up)) {
-              ok = false;
-              break;
+          };
+          if (QF) {
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] = __float_as_uint(o_row[QF ? c + j : 0]);
+              put(c, o);
             }
-            if (warp_on) {
-              fence_after();
-              const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-              const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD;
-              const long pr = (long)slot * a.tile_rows + s * 128 + row;
-              if (!whole && mine) a.ml[pr] = make_float2(m, l);
-              if (QF) gather();
-#pragma unroll
-              for (int c = 0; c < HD; c += 32) {
-                uint32_t o[32];
-                if (QF) {
-#pragma unroll
-                  for (int j = 0; j < 32; j++) o[j] = __float_as_uint(o_row[QF ? c + j : 0]);
-                } else {
-                  tmem_ld32_nowait(tO + c, o);
-                  tmem_wait();
-                  pin32(o);
-                }
-                if (mine) {
-                  float v[32];
-#pragma unroll
-                  for (int j = 0; j < 32; j++) v[j] = l == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
-                  if (whole && !QF) {
-                    uint16_t* w = static_cast<uint16_t*>(a.p.out) + at + c;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                      *reinterpret_cast<uint4*>(w + j) = make_uint4(pack_bf2(v[j], v[j + 1]), pack_bf2(v[j + 2], v[j + 3]),
-                                                                    pack_bf2(v[j + 4], v[j + 5]), pack_bf2(v[j + 6], v[j + 7]));
-                  } else {
-                    float* w = whole ? static_cast<float*>(a.p.out) + at + c : a.acc + pr * HD + c;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                  }
-                }
-              }
-              fence_before();
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32_nowait(tO + c, o);
+              tmem_wait();
+              pin32(o);
+              put(c, o);
             }
           }
+          fence_before();
         }
-        if (last) fresh = true;
-        if (u + 1 < units) cu.next<R, KT>(a);
       }
+      u += end - cu.kt;
+      if (u == units) break;
+      cu = AttnCursor::next<R, KT>(a, cu);
     }
   }
   fence_before();
@@ -540,15 +669,6 @@ cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
   static SmemOptIn opt;
   CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_tc_kernel<QF, HD>), S::SMEM));
   const int box = std::min(a.p.kv.page_size, S::KT);
-  if (S::REGS) {
-    // the register split below adds up only for a block launched with these
-    static PerDeviceInt regs;
-    const int n = regs.get([] {
-      cudaFuncAttributes at;
-      return cudaFuncGetAttributes(&at, paged_attn_tc_kernel<QF, HD>) == cudaSuccess ? at.numRegs : 0;
-    });
-    if (n != S::LAUNCH_REGS) return cudaErrorLaunchOutOfResources;
-  }
   CUtensorMap mk, mv;
   int order = 0;
   if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
