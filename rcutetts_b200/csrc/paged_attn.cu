@@ -96,11 +96,11 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     gave_up = 0;
   }
   grid_dep_enter();
-  attn_find_start<R, C, kNT + 32>(a, &start);
+  attn_find_start<R, C, kNT + 32>(a.line, &start);
   const int units = (int)start.units;  // (of one CTA: 31 bits, the host checks)
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   if (units == 0) return;
-  AttnCursor cu = AttnCursor::at<R, C>(a, start);
+  AttnCursor cu = AttnCursor::at<R, C>(a.line, start);
 
   if (warp == 4) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
       const int mine = none ? a.p.kv.n_pages : page;
       if (u + 1 < units) {  // the next tile's pages, over the wait
         if (++kt == cu.nt) {
-          cu = AttnCursor::next<R, C>(a, cu);
+          cu = AttnCursor::next<R, C>(a.line, cu);
           kt = 0;
         }
         page = page_of();
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     // ---- a piece: tiles cu.kt .. end of an item
     const int end = min(cu.nt, cu.kt + units - u);
     const int row_base = cu.m * R;  // first packed row of the item
-    const int nrows = cu.rows(a, R);
+    const int nrows = cu.rows(a.line, R);
     const int pos0 = cu.pos0();
     {
       if (CHUNK) sync_rows();  // the queries of the item before are read (short runs: their merge has synchronised)
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
       float* const part = a.acc + (long)slot * a.tile_rows * HD;
       if (!ends && cu.kt == 0 && tid == 0) {
         AttnPart d;
-        d.pieces = attn_pieces(a, start, cu.nt - end);
+        d.pieces = attn_pieces(a.line, start, cu.nt - end);
         d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
         a.parts[blockIdx.x] = d;
       }
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     }
     u += end - cu.kt;
     if (u == units) break;
-    cu = AttnCursor::next<R, C>(a, cu);
+    cu = AttnCursor::next<R, C>(a.line, cu);
   }
 }
 
@@ -597,7 +597,7 @@ cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
   const int box = std::min(a.p.kv.page_size, (int)S::C);
   int order = 0;
   if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
-  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK, RH>, dim3(a.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);
+  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK, RH>, dim3(a.line.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);
 }
 
 // The call's mma.sync shape: f(QF, KF, HD, CHUNK, RH as integral constants).
@@ -681,7 +681,16 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   a.p = p;
   a.group = p.n_heads / p.kv.n_kv_heads;
   while ((1 << a.shift) < p.kv.page_size) a.shift++;
-  a.ctas = pl.ctas;
+  AttnLine& ln = a.line;
+  ln.cu_rows = p.cu_rows;
+  ln.seq_lens = p.seq_lens;
+  ln.batch = p.batch;
+  ln.rows = p.rows;
+  ln.max_new = p.max_new;
+  ln.max_len = p.max_pages * p.kv.page_size;
+  ln.group = a.group;
+  ln.n_kv = p.kv.n_kv_heads;
+  ln.ctas = pl.ctas;
   a.tile_rows = pl.tile_rows;
   a.rows_used = rows_used_of(p);
   const double c2 = (double)p.scale * 1.4426950408889634;
@@ -699,7 +708,7 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
       return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value, decltype(rh)::value>(a, s);
     }));
   const int rows = (int)std::min((long)a.tile_rows, (long)p.max_new * a.group);
-  const dim3 grid(a.ctas, rows > 16 ? 16 : std::min(rows, 4)), block(kJoinThreads);
+  const dim3 grid(a.line.ctas, rows > 16 ? 16 : std::min(rows, 4)), block(kJoinThreads);
   const bool bf = p.q_dtype == CTTS_BF16;
   if (p.kv.head_dim == 64)
     return bf ? launch_k(paged_attn_join_kernel<true, 64>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 64>, grid, block, 0, s, a);

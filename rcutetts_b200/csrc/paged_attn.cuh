@@ -21,10 +21,20 @@ struct AttnPart {
   int pad[3] = {0, 0, 0};
 };
 
+// What the line follows from.  Functions that are called, not inlined, take
+// it by value: a reference to a kernel's parameters would be read as memory.
+struct AttnLine {
+  const int *cu_rows = nullptr, *seq_lens = nullptr;
+  int batch = 0, rows = 0, max_new = 0, max_len = 0;
+  int group = 1, n_kv = 1;  // query heads per KV head, KV heads
+  int ctas = 0;
+};
+
 struct PagedAttnArgs {
   ctts_paged_attn p;
+  AttnLine line;
   int group = 1, shift = 0;      // query heads per KV head, log2 of the page size
-  int ctas = 0, tile_rows = 0;   // CTAs, packed rows per item
+  int tile_rows = 0;             // packed rows per item
   int rows_used = 0;             // packed rows an item can have
   float c2_hi = 0, c2_lo = 0;    // scale * log2(e): scores in powers of two
   AttnPart* parts = nullptr;     // [ctas]
@@ -71,12 +81,12 @@ CTTS_DEV float attn_arg(const PagedAttnArgs& a, float s, float m) {
 struct AttnReq {
   int r0, cnt, nn, len;  // first row, rows, rows computed (cnt cut to max_new), tokens
 };
-CTTS_DEV AttnReq attn_req(const PagedAttnArgs& a, int b) {
+CTTS_DEV AttnReq attn_req(const AttnLine& ln, int b) {
   AttnReq r;
-  r.r0 = min(max(a.p.cu_rows[b], 0), a.p.rows);
-  r.cnt = min(max(a.p.cu_rows[b + 1], r.r0), a.p.rows) - r.r0;
-  r.nn = min(r.cnt, a.p.max_new);
-  r.len = (int)min((long)max(a.p.seq_lens[b], 0), (long)a.p.max_pages << a.shift);
+  r.r0 = min(max(ln.cu_rows[b], 0), ln.rows);
+  r.cnt = min(max(ln.cu_rows[b + 1], r.r0), ln.rows) - r.r0;
+  r.nn = min(r.cnt, ln.max_new);
+  r.len = min(max(ln.seq_lens[b], 0), ln.max_len);
   return r;
 }
 // Row tiles of a request (packed rows fit 31 bits: the host checks).
@@ -119,13 +129,13 @@ struct AttnRowWalk {
   }
 };
 template <int R, int C>
-CTTS_DEV long attn_units(const PagedAttnArgs& a, const AttnReq& r) {
-  const int mt = attn_row_tiles<R>(r, a.group);
-  AttnRowWalk<R, C> w(r, a.group);
+CTTS_DEV long attn_units(const AttnLine& ln, const AttnReq& r) {
+  const int mt = attn_row_tiles<R>(r, ln.group);
+  AttnRowWalk<R, C> w(r, ln.group);
   long n = 0;
 #pragma unroll 1
   for (int m = 0; m < mt; m++, w.next()) n += w.tiles();
-  return n * a.p.kv.n_kv_heads;
+  return n * ln.n_kv;
 }
 // The line is cut into `ctas` pieces of `base` tiles, the first `rest` of them
 // one longer; no more pieces than tiles, so that the pieces of a divided item
@@ -160,10 +170,10 @@ struct AttnStart {
 // kept small throughout these kernels: what does not fit the instruction cache
 // beside the main loop costs more than a rolled loop.)
 template <int R, int C, int NT>
-CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
+CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
   constexpr int W = NT / 32;
   __shared__ long wsum[2][W];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.p.batch;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = ln.batch;
   long total = 0, first = 0, u0 = 0, u1 = 0;
   AttnReq rq = {0, 0, 0, 0};
   int ph = 0, pass = 0, base = 0;
@@ -172,8 +182,8 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
     const int b = base + tid;
     long u = 0;
     if (b < n) {
-      rq = attn_req(a, b);
-      u = attn_units<R, C>(a, rq);
+      rq = attn_req(ln, b);
+      u = attn_units<R, C>(ln, rq);
     }
     long inc = u;
 #pragma unroll 1
@@ -195,7 +205,7 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
     if (pass == 0) {
       total += all;
       if (base < n) continue;
-      const AttnCut cut(a.ctas, total);
+      const AttnCut cut(ln.ctas, total);
       u0 = cut.begin(blockIdx.x);
       u1 = cut.begin(blockIdx.x + 1);
       if (tid == 0) {
@@ -223,8 +233,8 @@ CTTS_DEV void attn_find_start(const PagedAttnArgs& a, AttnStart* out) {
 }
 
 // CTAs from this one to the one that holds tile `more` behind this CTA's end.
-CTTS_DEV int attn_pieces(const PagedAttnArgs& a, const AttnStart& s, int more) {
-  return AttnCut(a.ctas, s.total).owner(s.end + more - 1) - (int)blockIdx.x + 1;
+CTTS_DEV int attn_pieces(const AttnLine& ln, const AttnStart& s, int more) {
+  return AttnCut(ln.ctas, s.total).owner(s.end + more - 1) - (int)blockIdx.x + 1;
 }
 
 // A place on the line: request, row tile, KV head, key tile.  A role walks its
@@ -233,21 +243,20 @@ struct AttnCursor {
   int b, m, h, kt, nt, mt;
   int r0, cnt, nn, len;
 
-  CTTS_DEV void set(const PagedAttnArgs& a, int R, const AttnReq& r) {
+  CTTS_DEV void set(const AttnLine& ln, int R, const AttnReq& r) {
     r0 = r.r0; cnt = r.cnt; nn = r.nn; len = r.len;
-    mt = (nn * a.group + R - 1) / R;
+    mt = (nn * ln.group + R - 1) / R;
   }
   template <int R, int C>
-  static __device__ __noinline__ AttnCursor at(const PagedAttnArgs& a, const AttnStart& s) {
+  static __device__ __noinline__ AttnCursor at(AttnLine ln, AttnReq req, int b, long skip) {
     AttnCursor c;
-    c.b = s.b;
-    c.set(a, R, s.req);
-    long skip = s.skip;
-    AttnRowWalk<R, C> w(s.req, a.group);
+    c.b = b;
+    c.set(ln, R, req);
+    AttnRowWalk<R, C> w(req, ln.group);
 #pragma unroll 1
     for (c.m = 0;; c.m++, w.next()) {
       c.nt = w.tiles();
-      const long in = (long)c.nt * a.p.kv.n_kv_heads;
+      const long in = (long)c.nt * ln.n_kv;
       if (skip < in || c.m + 1 >= c.mt) break;
       skip -= in;
     }
@@ -255,25 +264,33 @@ struct AttnCursor {
     c.kt = (unsigned)skip % (unsigned)c.nt;
     return c;
   }
+  template <int R, int C>
+  static CTTS_DEV AttnCursor at(const AttnLine& ln, const AttnStart& s) {
+    return at<R, C>(ln, s.req, s.b, s.skip);
+  }
   // The next item, from its first tile (never called at the end of the line).
   template <int R, int C>
-  static __device__ __noinline__ AttnCursor next(const PagedAttnArgs& a, AttnCursor c) {
+  static CTTS_DEV AttnCursor next(const AttnLine& ln, AttnCursor c) {
     c.kt = 0;
-    if (++c.h < a.p.kv.n_kv_heads) return c;
+    if (++c.h < ln.n_kv) return c;
+    return next_rows<R, C>(ln, c);
+  }
+  template <int R, int C>
+  static __device__ __noinline__ AttnCursor next_rows(AttnLine ln, AttnCursor c) {
     c.h = 0;
     if (++c.m == c.mt) {
       c.m = 0;
 #pragma unroll 1
       do {
         c.b++;
-        c.set(a, R, attn_req(a, c.b));
-      } while (c.mt == 0 && c.b + 1 < a.p.batch);
+        c.set(ln, R, attn_req(ln, c.b));
+      } while (c.mt == 0 && c.b + 1 < ln.batch);
     }
-    c.nt = attn_tiles<R, C>(AttnReq{c.r0, c.cnt, c.nn, c.len}, c.m, a.group);
+    c.nt = attn_tiles<R, C>(AttnReq{c.r0, c.cnt, c.nn, c.len}, c.m, ln.group);
     return c;
   }
   // Packed rows of the item, and the position of the request's first new row.
-  CTTS_DEV int rows(const PagedAttnArgs& a, int R) const { return min(R, nn * a.group - m * R); }
+  CTTS_DEV int rows(const AttnLine& ln, int R) const { return min(R, nn * ln.group - m * R); }
   CTTS_DEV int pos0() const { return len - cnt; }
 };
 

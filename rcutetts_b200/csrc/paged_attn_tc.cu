@@ -57,7 +57,7 @@ struct TcShape {
   static constexpr uint32_t QTERM = NC * 128 * 128;       // bytes of one term of one sub-tile
   static constexpr uint32_t TILE = NC * KT * 128;         // bytes of a K or V tile
   static constexpr int NS = QF ? (HD == 64 ? 6 : 3) : (HD == 64 ? 4 : 2);
-  static constexpr size_t SMEM = (size_t)NSUB * NT * QTERM + (size_t)2 * NS * TILE + 1024;
+  static constexpr size_t SMEM = (size_t)NSUB * NT * QTERM + (size_t)2 * NS * TILE + NSUB * 4 * 4096 + 1024;  // and 4 KB a softmax warp
 };
 
 // Shared-memory descriptors of 128-byte swizzled operands, as their two words.
@@ -161,6 +161,29 @@ CTTS_DEV float2 exp2_poly(float2 x) {
 // Of the 16 pairs of a turn, every kPolyEvery-th by exp2_poly (0: none).
 constexpr int kPolyEvery = 4;
 
+// Byte offsets of packed rows p, p + 4, p + 8, ... (row of q times its stride
+// plus head times width), one division for all of them.
+struct RowWalk {
+  long off, step, wrap;
+  int g, over, group;
+  CTTS_DEV RowWalk(int p, int grp, long ld_bytes, int head_bytes) : group(grp) {
+    const int row = p / grp, per = 4 / grp;
+    g = p - row * grp;
+    over = 4 - per * grp;
+    off = row * ld_bytes + g * head_bytes;
+    step = per * ld_bytes + over * head_bytes;
+    wrap = ld_bytes - grp * head_bytes;
+  }
+  CTTS_DEV void next4() {
+    off += step;
+    g += over;
+    if (g >= group) {
+      g -= group;
+      off += wrap;
+    }
+  }
+};
+
 struct TcBars {
   uint64_t k_full[6], k_empty[6], v_full[6], v_empty[6];
   uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], drain;
@@ -207,7 +230,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   grid_dep_enter();
-  attn_find_start<R, KT, S::THREADS>(a, &start);
+  attn_find_start<R, KT, S::THREADS>(a.line, &start);
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   fence_before();
   __syncthreads();
@@ -218,7 +241,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   if (units > 0 && warp == W_TMA) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them
-    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
     int kt = cu.kt;
     auto page_of = [&]() {
       const int kk = kt * KT + 8 * lane;
@@ -234,7 +257,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
       const int from = none ? a.p.kv.n_pages : page;  // outside the map: zeros
       if (u + 1 < units) {  // the next tile's pages, over the waits
         if (++kt == cu.nt) {
-          cu = AttnCursor::next<R, KT>(a, cu);
+          cu = AttnCursor::next<R, KT>(a.line, cu);
           kt = 0;
         }
         page = page_of();
@@ -270,7 +293,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     // uniform), one lane issues; between its products it does next to nothing:
     // what it spends there the tensor core stands still.
     const bool leader = elect_one();
-    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
     auto scores = [&](int s, int st) {
       const uint32_t kb = desc_lo(ks + st * S::TILE, 16), qb = desc_lo(qs + s * NT * S::QTERM, 16);
       fence_after();
@@ -312,7 +335,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
 #pragma unroll 1
     while (true) {
       const int n = __shfl_sync(0xffffffffu, min(cu.nt - cu.kt, units - done), 0);
-      const int nsub = __shfl_sync(0xffffffffu, cu.rows(a, R) > 128 ? 2 : 1, 0);
+      const int nsub = __shfl_sync(0xffffffffu, cu.rows(a.line, R) > 128 ? 2 : 1, 0);
       // a turn: P.V of tile i - 1, scores of tile i
 #pragma unroll 1
       for (int i = 0; i <= n; i++) {
@@ -351,7 +374,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
       }
       done += n;
       if (done == units) break;
-      cu = AttnCursor::next<R, KT>(a, cu);
+      cu = AttnCursor::next<R, KT>(a.line, cu);
     }
     if (gave_up) {  // MMAs in flight end before TMEM is given back
       commit(&bars.drain);
@@ -363,7 +386,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + S::SREG * s + lane_base, tP = tS + S::PCOL, tO = tmem + S::OREG + S::OSTEP * s + lane_base;
     const float c2 = a.c2_hi;
-    AttnCursor cu = AttnCursor::at<R, KT>(a, start);
+    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
     uint32_t s_par = 0, o_par = 0;
     float o_row[QF ? HD : 1];  // float32 calls: the output row so far
     // adds the product of the last tile to it
@@ -378,16 +401,16 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         for (int j = 0; j < 32; j++) o_row[QF ? c + j : 0] += __uint_as_float(o[j]);
       }
     };
-    int u = 0;
+    // A turn: the queries of the next piece go to shared memory (and its first
+    // scores may begin), then the piece before is written out, then the next
+    // one's tiles run.
+    AttnCursor nx = cu;
+    int u = 0, next_u = 0, end = 0;
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
     while (true) {
-      // ---- a piece: tiles cu.kt .. end of an item
-      const int end = min(cu.nt, cu.kt + units - u), nrows = cu.rows(a, R);
-      if (s * 128 < nrows) {  // the sub-tile has rows
-        const int r0 = s * 128 + (warp & 3) * 32;  // the warp's first row in the item
-        const bool mine = s * 128 + row < nrows, warp_on = r0 < nrows;
-        const int pk = cu.m * R + s * 128 + row;
-        const int pos = cu.pos0() + pk / a.group, pos_lo = cu.pos0() + (pk - lane) / a.group;
+      if (next_u < units && s * 128 < nx.rows(a.line, R)) {
+        const int r0 = s * 128 + (warp & 3) * 32, nrows = nx.rows(a.line, R);  // the warp's first row in the item
         // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes of a
         // row (as bf16), four rows at a time, all loads in flight before the
         // first is used; rows behind the item are zero
@@ -395,21 +418,24 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         for (int c = 0; c < NC; c++) {
           constexpr int RP = 8;  // rows a lane reads: 4 i + lane / 8
           uint4 x[RP], y[QF ? RP : 1];
+          constexpr int ES = QF ? 4 : 2;
+          RowWalk w(nx.m * R + r0 + (lane >> 3), a.group, a.p.q_ld * ES, HD * ES);
+          const uint8_t* q = static_cast<const uint8_t*>(a.p.q) + ((long)nx.r0 * a.p.q_ld + nx.h * a.group * HD + c * 64 + (lane & 7) * 8) * ES;
+          const int left = nrows - r0 - (lane >> 3);  // rows behind the item (4 i >= left) read its first row and count as zero
 #pragma unroll
           for (int i = 0; i < RP; i++) {
-            const int r = r0 + 4 * i + (lane >> 3), p = cu.m * R + r;
-            x[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (QF) y[QF ? i : 0] = x[i];
-            if (r < nrows) {
-              const int tok = p / a.group;
-              const long at = (long)(cu.r0 + tok) * a.p.q_ld + (cu.h * a.group + p - tok * a.group) * HD + c * 64 + (lane & 7) * 8;
-              if (QF) {
-                x[i] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at);
-                y[QF ? i : 0] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.p.q) + at + 4);
-              } else {
-                x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
+            const uint4* at = reinterpret_cast<const uint4*>(q + (4 * i < left ? w.off : 0));
+            x[i] = at[0];
+            if (QF) y[QF ? i : 0] = at[1];
+            w.next4();
+          }
+          if (r0 + 32 > nrows) {
+#pragma unroll
+            for (int i = 0; i < RP; i++)
+              if (4 * i >= left) {
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (QF) y[QF ? i : 0] = x[i];
               }
-            }
           }
 #pragma unroll
           for (int i = 0; i < RP; i++) {
@@ -434,8 +460,115 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         }
         fence_async();
         mbar_arrive(&bars.q_full[s]);
-
-        float m = -INFINITY, l = 0.0f;
+      }
+      if (u < next_u && s * 128 < cu.rows(a.line, R)) {
+        const int nrows = cu.rows(a.line, R);
+        const bool mine = s * 128 + row < nrows, warp_on = s * 128 + (warp & 3) * 32 < nrows;
+        // ---- the piece's output, or its partial state
+        const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
+        const int place = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
+        if (!ends && cu.kt == 0 && s == 0 && row == 0) {
+          AttnPart d;
+          d.pieces = attn_pieces(a.line, start, cu.nt - end);
+          d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
+          a.parts[blockIdx.x] = d;
+        }
+        mbar_wait_or(&bars.o_full[s], o_par, &gave_up);
+        o_par ^= 1;
+        if (warp_on) {
+          fence_after();
+          const bool none = m == -INFINITY;  // the row saw no key
+          const float inv = whole && !none ? 1.0f / l : 1.0f;
+          if (!whole && mine) a.ml[(long)place * a.tile_rows + s * 128 + row] = make_float2(m, l);
+          if (QF) gather();
+          // 32 columns of the warp's 32 rows by way of shared memory: a lane
+          // holds a row, eight lanes write 128 bytes of one (four lanes 64
+          // bytes in bf16)
+          const uint32_t stage = vs + NS * S::TILE + warp * 4096;
+          const bool half = whole && !QF;
+          const int r0 = s * 128 + (warp & 3) * 32, left = nrows - r0 - (lane >> 3), es = half ? 2 : 4;
+          RowWalk w0(cu.m * R + r0 + (lane >> 3), a.group, a.p.out_ld * es, HD * es);
+          uint8_t* dst = static_cast<uint8_t*>(a.p.out) + ((long)cu.r0 * a.p.out_ld + cu.h * a.group * HD) * es;
+          if (!whole) {  // rows of the partial state follow one another
+            w0.off = (long)(r0 + (lane >> 3)) * HD * 4;
+            w0.step = 4 * HD * 4;
+            w0.g = w0.over = 0;
+            dst = reinterpret_cast<uint8_t*>(a.acc + (long)place * a.tile_rows * HD);
+          }
+          dst += (lane & 7) * 16;
+          const bool writes = !half || (lane & 7) < 4;
+          auto put = [&](int c, uint32_t* o) {
+            if (none) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) v[e] = __uint_as_float(o[4 * j + e]) * inv;
+              if (half)
+                asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(stage + lane * 128 + (((j >> 1) ^ lane) & 7) * 16 + (j & 1) * 8),
+                             "r"(pack_bf2(v[0], v[1])), "r"(pack_bf2(v[2], v[3]))
+                             : "memory");
+              else
+                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((j ^ lane) & 7) * 16), "f"(v[0]), "f"(v[1]),
+                             "f"(v[2]), "f"(v[3])
+                             : "memory");
+            }
+            __syncwarp();
+            RowWalk w = w0;
+            uint8_t* d = dst + c * es;
+            uint4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int r = 4 * i + (lane >> 3);
+              asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
+                           : "r"(stage + r * 128 + ((lane ^ r) & 7) * 16)
+                           : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              if (writes && 4 * i < left) *reinterpret_cast<uint4*>(d + w.off) = v[i];
+              w.next4();
+            }
+            __syncwarp();
+          };
+          if (QF) {
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] = __float_as_uint(o_row[QF ? c + j : 0]);
+              put(c, o);
+            }
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32_nowait(tO + c, o);
+              tmem_wait();
+              pin32(o);
+              put(c, o);
+            }
+          }
+          fence_before();
+        }
+      }
+      if (next_u == units) break;
+      // ---- a piece: tiles cu.kt .. end of an item
+      cu = nx;
+      u = next_u;
+      end = min(cu.nt, cu.kt + units - u);
+      next_u = u + end - cu.kt;
+      const int nrows = cu.rows(a.line, R);
+      if (s * 128 < nrows) {  // the sub-tile has rows
+        const bool warp_on = s * 128 + (warp & 3) * 32 < nrows;
+        const int pk = cu.m * R + s * 128 + row;
+        const int pos = cu.pos0() + pk / a.group, pos_lo = cu.pos0() + (pk - lane) / a.group;
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
         for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] = 0.0f;
 #pragma unroll 1
@@ -593,68 +726,8 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           }
           mbar_arrive(&bars.p_full[s]);
         }
-
-        // ---- the piece's output, or its partial state
-        const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
-        const int place = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
-        if (!ends && cu.kt == 0 && s == 0 && row == 0) {
-          AttnPart d;
-          d.pieces = attn_pieces(a, start, cu.nt - end);
-          d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
-          a.parts[blockIdx.x] = d;
-        }
-        mbar_wait_or(&bars.o_full[s], o_par, &gave_up);
-        o_par ^= 1;
-        if (warp_on) {
-          fence_after();
-          const bool none = m == -INFINITY;  // the row saw no key
-          const float inv = whole ? 1.0f / l : 1.0f;
-          const int tok = pk / a.group;
-          const long at = (long)(cu.r0 + tok) * a.p.out_ld + (cu.h * a.group + pk - tok * a.group) * HD;
-          const long pr = (long)place * a.tile_rows + s * 128 + row;
-          if (!whole && mine) a.ml[pr] = make_float2(m, l);
-          if (QF) gather();
-          auto put = [&](int c, const uint32_t* o) {
-            if (!mine) return;
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = none ? 0.0f : __uint_as_float(o[j]) * inv;
-            if (whole && !QF) {
-              uint16_t* w = static_cast<uint16_t*>(a.p.out) + at + c;
-#pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                *reinterpret_cast<uint4*>(w + j) = make_uint4(pack_bf2(v[j], v[j + 1]), pack_bf2(v[j + 2], v[j + 3]),
-                                                              pack_bf2(v[j + 4], v[j + 5]), pack_bf2(v[j + 6], v[j + 7]));
-            } else {
-              float* w = whole ? static_cast<float*>(a.p.out) + at + c : a.acc + pr * HD + c;
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(w + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            }
-          };
-          if (QF) {
-#pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t o[32];
-#pragma unroll
-              for (int j = 0; j < 32; j++) o[j] = __float_as_uint(o_row[QF ? c + j : 0]);
-              put(c, o);
-            }
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t o[32];
-              tmem_ld32_nowait(tO + c, o);
-              tmem_wait();
-              pin32(o);
-              put(c, o);
-            }
-          }
-          fence_before();
-        }
       }
-      u += end - cu.kt;
-      if (u == units) break;
-      cu = AttnCursor::next<R, KT>(a, cu);
+      if (next_u < units) nx = AttnCursor::next<R, KT>(a.line, cu);
     }
   }
   fence_before();
@@ -672,7 +745,7 @@ cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
   CUtensorMap mk, mv;
   int order = 0;
   if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
-  return launch_k(paged_attn_tc_kernel<QF, HD>, dim3(a.ctas), dim3(S::THREADS), S::SMEM, s, mk, mv, a, box, order);
+  return launch_k(paged_attn_tc_kernel<QF, HD>, dim3(a.line.ctas), dim3(S::THREADS), S::SMEM, s, mk, mv, a, box, order);
 }
 
 }  // namespace
