@@ -412,7 +412,8 @@ CTTS_API int ctts_op_paged_plan(const ctts_paged_plan* p, void* stream);
  * keys and values to slots[row] of the pools, each rounded once to its type.
  * A row whose slot lies outside the pools (-1: padding) writes nothing, its
  * query included.  The slots of one call are distinct.  x_ld and q_ld are row
- * strides in elements (multiples of 16 bytes; x and q 16-byte aligned). */
+ * strides in elements (multiples of 16 bytes); x, q, q_norm and k_norm are
+ * 16-byte aligned. */
 typedef struct {
   ctts_paged_kv kv;
   const void* x;

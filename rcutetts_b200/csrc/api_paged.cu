@@ -96,7 +96,8 @@ extern "C" int ctts_op_paged_append(const ctts_paged_append* p, void* stream) {
   rc = check_pool_data(p->kv);
   if (rc != CTTS_OK) return rc;
   CTTS_REQ(p->x && p->q && p->positions && p->slots, CTTS_ERR_ARG, "null argument");
-  CTTS_REQ(aligned16(p->x) && aligned16(p->q), CTTS_ERR_ARG, "x and q must be 16-byte aligned");
+  CTTS_REQ(aligned16(p->x) && aligned16(p->q) && aligned16(p->q_norm) && aligned16(p->k_norm), CTTS_ERR_ARG,
+           "x, q, q_norm and k_norm must be 16-byte aligned");
   CTTS_CK(launch_paged_append(*p, as_stream(stream, 0)));
   return CTTS_OK;
 }

@@ -173,9 +173,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const ctts_pag
 // or into the cache.  A lane holds V elements of both halves of a head (the
 // RoPE pairs (d, d + hd/2)), L = hd/(2V) lanes hold a head, so the norm is a
 // sum over L lanes and the rotation stays in the lane; loads and stores are
-// 16 bytes.  The sine and cosine of a row's hd/2 angles are computed once per
-// row, for all its heads, after the row's first loads are in flight.
-constexpr int kAppThreads = 256;
+// 16 bytes.  A warp takes a row: it passes over 32/L heads at a time with the
+// same dims in a lane, so a lane computes its V angles once for all of them
+// (after the first heads' loads are in flight), and nothing is shared or
+// waited for between warps.  Few rows (a decode step): several warps a row.
+// 16381 rows, 16 + 2 x 8 heads of 128, bf16: @@ us, @@ TB/s (one row a block
+// and its angles through shared memory: 89 us).
+constexpr int kAppWarps = 4;   // a block
+constexpr int kAppAhead = 4;   // loads in flight: passes of a warp
 
 // Turns per position of each frequency: theta^(-2i/hd) / (2 pi).  In double
 // and reduced to a fraction of a turn before rounding: in float32 an angle of
@@ -184,26 +189,11 @@ struct AppFreq {
   double turns[64];
 };
 
-template <typename T, int V>
-struct Vec;
-template <>
-struct Vec<float, 4> {
-  float v[4];
-  CTTS_DEV void load(const void* p, long i) {
-    const float4 f = ld_stream_f4(static_cast<const float*>(p) + i);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-  }
-};
-template <>
-struct Vec<uint16_t, 8> {
-  float v[8];
-  CTTS_DEV void load(const void* p, long i) {
-    const uint4 u = ld_stream_u4(static_cast<const uint16_t*>(p) + i);
-    v[0] = bf_lo(u.x); v[1] = bf_hi(u.x); v[2] = bf_lo(u.y); v[3] = bf_hi(u.y);
-    v[4] = bf_lo(u.z); v[5] = bf_hi(u.z); v[6] = bf_lo(u.w); v[7] = bf_hi(u.w);
-  }
-};
-CTTS_DEV uint32_t pack2(float lo, float hi) { return (uint32_t)f2bf(lo) | ((uint32_t)f2bf(hi) << 16); }
+CTTS_DEV uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 template <int V>
 CTTS_DEV void store(void* p, int bf16, long i, const float* v) {
   if (bf16) {
@@ -218,83 +208,96 @@ CTTS_DEV void store(void* p, int bf16, long i, const float* v) {
     for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(q + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   }
 }
+// 16 bytes: four float32 or eight bf16
+template <int V>
+CTTS_DEV void widen(const uint4& u, float* v) {
+  if (V == 4) {
+    v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+  } else {
+    v[0] = bf_lo(u.x); v[1] = bf_hi(u.x); v[2] = bf_lo(u.y); v[3] = bf_hi(u.y);
+    v[4 % V] = bf_lo(u.z); v[5 % V] = bf_hi(u.z); v[6 % V] = bf_lo(u.w); v[7 % V] = bf_hi(u.w);
+  }
+}
 
-// grid (rows), kAppThreads threads; XT float or uint16_t (bf16 bits)
-template <typename XT, int V, int HD>
-__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const ctts_paged_append a, const AppFreq fr, int shift) {
-  constexpr int HALF = HD / 2, L = HALF / V, UNITS = kAppThreads / L;
-  __shared__ __align__(16) float cs[HALF], sn[HALF];
+// `parts` warps a row; V = 4 (float32 x) or 8 (bf16)
+template <int V, int HD>
+__global__ void __launch_bounds__(kAppWarps * 32, V == 8 ? 5 : 6) paged_append_kernel(const ctts_paged_append a, const __grid_constant__ AppFreq fr, int shift,
+                                                                      int parts) {
+  constexpr int HALF = HD / 2, L = HALF / V, AT_ONCE = 32 / L, ES = 16 / V;
   grid_dep_enter();
-  const int row = blockIdx.x, tid = threadIdx.x;
-  const int sub = tid % L, d = sub * V;
+  const int lane = threadIdx.x & 31, w = blockIdx.x * kAppWarps + (threadIdx.x >> 5);
+  const int row = w / parts, part = w - row * parts;
+  if (row >= a.rows) return;
   const int nq = a.n_heads, nkv = a.kv.n_kv_heads, heads = nq + 2 * nkv;
-  const int slot = a.slots[row];
-  if (slot < 0 || slot >= a.kv.n_pages * a.kv.page_size) return;
-  const XT* x = static_cast<const XT*>(a.x) + (long)row * a.x_ld;
-  Vec<XT, V> lo, hi;
-  int h = tid / L;
-  if (h < heads) {
-    lo.load(x, h * HD + d);
-    hi.load(x, h * HD + HALF + d);
-  }
-  if (tid < HALF) {
-    const double t = (double)a.positions[row] * fr.turns[tid];
-    float s, c;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-    cs[tid] = c;
-    sn[tid] = s;
-  }
-  __syncthreads();
-  const long kv_at = (long)(slot >> shift) * a.kv.page_stride + (long)(slot & (a.kv.page_size - 1)) * a.kv.token_stride;
+  const int d = (lane % L) * V;
+  const uint8_t* x = static_cast<const uint8_t*>(a.x) + ((long)row * a.x_ld + d) * ES;
+  const int slot = a.slots[row], pos = a.positions[row];
   const bool normed = a.q_norm != nullptr;
-  // (every lane of a warp takes the same number of turns: the sums below are warp-wide)
-  for (int h0 = 0; h0 < heads; h0 += UNITS, h += UNITS) {
-    const bool on = h < heads;
-    Vec<XT, V> nlo, nhi;  // the next head, in flight over this one
-    if (h + UNITS < heads) {
-      nlo.load(x, (h + UNITS) * HD + d);
-      nhi.load(x, (h + UNITS) * HD + HALF + d);
-    }
-    const bool is_q = h < nq, is_v = h >= nq + nkv;
-    float ss = 0.0f;
-    if (on && !is_v && normed) {
+  const int step = parts * AT_ONCE;
+  float cs[V], sn[V];
+  bool ready = false;
+  // (every lane of a warp makes the same passes: the sums are warp-wide)
+  for (int h0 = part * AT_ONCE; h0 < heads; h0 += kAppAhead * step) {
+    uint4 lo[kAppAhead], hi[kAppAhead];
 #pragma unroll
-      for (int j = 0; j < V; j++) ss = fmaf(lo.v[j], lo.v[j], fmaf(hi.v[j], hi.v[j], ss));
+    for (int i = 0; i < kAppAhead; i++) {
+      const int h = h0 + i * step + lane / L;
+      if (h < heads) {
+        lo[i] = ld_stream_u4(x + (long)h * HD * ES);
+        hi[i] = ld_stream_u4(x + (long)h * HD * ES + HALF * ES);
+      }
     }
-    if (normed) {
+    if (!ready) {
+      ready = true;
+      if (slot < 0 || slot >= a.kv.n_pages * a.kv.page_size) return;
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      for (int j = 0; j < V; j++) {
+        const double t = (double)pos * fr.turns[d + j];
+        sincospif(2.0f * (float)(t - rint(t)), &sn[j], &cs[j]);
+      }
     }
-    if (on) {
-      if (!is_v) {
-        if (normed) {
+    const long kv_at = (long)(slot >> shift) * a.kv.page_stride + (long)(slot & (a.kv.page_size - 1)) * a.kv.token_stride + d;
+#pragma unroll
+    for (int i = 0; i < kAppAhead; i++) {
+      const int h = h0 + i * step + lane / L;
+      if (h0 + i * step >= heads) break;
+      const bool on = h < heads, is_q = h < nq, is_v = h >= nq + nkv;
+      float u[V], v[V];
+      widen<V>(lo[i], u);
+      widen<V>(hi[i], v);
+      if (normed) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; j++) ss = fmaf(u[j], u[j], fmaf(v[j], v[j], ss));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!is_v) {
           const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
-          const float* g = is_q ? a.q_norm : a.k_norm;
+          const float* g = (is_q ? a.q_norm : a.k_norm) + d;  // (512 bytes that stay in L1)
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            lo.v[j] = lo.v[j] * inv * g[d + j];
-            hi.v[j] = hi.v[j] * inv * g[HALF + d + j];
+          for (int j = 0; j < V; j += 4) {
+            const float4 p = *reinterpret_cast<const float4*>(g + j), q = *reinterpret_cast<const float4*>(g + HALF + j);
+            u[j] *= inv * p.x; u[j + 1] *= inv * p.y; u[j + 2] *= inv * p.z; u[j + 3] *= inv * p.w;
+            v[j] *= inv * q.x; v[j + 1] *= inv * q.y; v[j + 2] *= inv * q.z; v[j + 3] *= inv * q.w;
           }
         }
+      }
+      if (!is_v) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          const float x1 = lo.v[j], x2 = hi.v[j], c = cs[d + j], s = sn[d + j];
-          lo.v[j] = x1 * c - x2 * s;
-          hi.v[j] = x1 * s + x2 * c;
+          const float x1 = u[j], x2 = v[j];
+          u[j] = x1 * cs[j] - x2 * sn[j];
+          v[j] = x1 * sn[j] + x2 * cs[j];
         }
       }
-      if (is_q) {
-        const long at = (long)row * a.q_ld + h * HD + d;
-        store<V>(a.q, a.q_dtype == CTTS_BF16, at, lo.v);
-        store<V>(a.q, a.q_dtype == CTTS_BF16, at + HALF, hi.v);
-      } else {
-        const long at = kv_at + (long)(is_v ? h - nq - nkv : h - nq) * a.kv.head_stride + d;
-        store<V>(is_v ? a.kv.v : a.kv.k, a.kv.dtype == CTTS_BF16, at, lo.v);
-        store<V>(is_v ? a.kv.v : a.kv.k, a.kv.dtype == CTTS_BF16, at + HALF, hi.v);
+      if (on) {
+        void* to = is_q ? a.q : (is_v ? a.kv.v : a.kv.k);
+        const int bf16 = (is_q ? a.q_dtype : a.kv.dtype) == CTTS_BF16;
+        const long at = is_q ? (long)row * a.q_ld + h * HD + d : kv_at + (long)(is_v ? h - nq - nkv : h - nq) * a.kv.head_stride;
+        store<V>(to, bf16, at, u);
+        store<V>(to, bf16, at + HALF, v);
       }
     }
-    lo = nlo;
-    hi = nhi;
   }
 }
 
@@ -324,13 +327,17 @@ cudaError_t launch_paged_append(const ctts_paged_append& a, cudaStream_t s) {
   const double step = pow(a.theta, -2.0 / hd);
   double f = 1.0 / (2.0 * 3.14159265358979323846);
   for (int i = 0; i < 64; i++, f *= step) fr.turns[i] = i < hd / 2 ? f : 0.0;
-  const dim3 grid(a.rows), block(kAppThreads);
   const bool bf = a.x_dtype == CTTS_BF16;
+  // warps a row: enough for about 48 warps an SM, up to a pass each
+  const int passes = (a.n_heads + 2 * a.kv.n_kv_heads) * hd / (bf ? 512 : 256);
+  int parts = 1;
+  while (parts * 2 <= passes && (long)a.rows * parts < 48L * device_sms()) parts *= 2;
+  const dim3 grid((unsigned)(((long)a.rows * parts + kAppWarps - 1) / kAppWarps)), block(kAppWarps * 32);
   if (hd == 64)
-    return bf ? launch_k(paged_append_kernel<uint16_t, 8, 64>, grid, block, 0, s, a, fr, shift)
-              : launch_k(paged_append_kernel<float, 4, 64>, grid, block, 0, s, a, fr, shift);
-  return bf ? launch_k(paged_append_kernel<uint16_t, 8, 128>, grid, block, 0, s, a, fr, shift)
-            : launch_k(paged_append_kernel<float, 4, 128>, grid, block, 0, s, a, fr, shift);
+    return bf ? launch_k(paged_append_kernel<8, 64>, grid, block, 0, s, a, fr, shift, parts)
+              : launch_k(paged_append_kernel<4, 64>, grid, block, 0, s, a, fr, shift, parts);
+  return bf ? launch_k(paged_append_kernel<8, 128>, grid, block, 0, s, a, fr, shift, parts)
+            : launch_k(paged_append_kernel<4, 128>, grid, block, 0, s, a, fr, shift, parts);
 }
 
 }  // namespace ctts

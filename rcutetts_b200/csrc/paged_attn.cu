@@ -97,16 +97,16 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
   }
   grid_dep_enter();
   attn_find_start<R, C, kNT + 32>(a.line, &start);
-  const int units = (int)start.units;  // (of one CTA: 31 bits, the host checks)
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
-  if (units == 0) return;
-  AttnCursor cu = AttnCursor::at<R, C>(a.line, start);
+  int left;
+  AttnCursor cu = AttnCursor::at<R, C>(a.line, start, &left);
+  if (left == 0) return;
 
   if (warp == 4) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them.  Pages that do not exist are
     // outside the map and arrive as zeros.
-    int kt = cu.kt;
+    int kt = cu.kt, end = cu.kt + cu.tiles(left);  // of the piece
     auto page_of = [&]() {
       const int kk = kt * C + 8 * lane;
       return lane < C / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
@@ -114,18 +114,21 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     int page = page_of(), st = 0;
     uint32_t par = 0;
 #pragma unroll 1
-    for (int u = 0; u < units && !gave_up; u++) {
+    for (int u = 0, more = 1; more && !gave_up; u++) {
       const int kk = kt * C + 8 * lane, h = cu.h;
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < C / 8 && kk < cu.len && none);
       const int mine = none ? a.p.kv.n_pages : page;
-      if (u + 1 < units) {  // the next tile's pages, over the wait
-        if (++kt == cu.nt) {
+      if (++kt == end) {
+        left = AttnCursor::behind(left, end - cu.kt);
+        more = left > 0;
+        if (more) {
           cu = AttnCursor::next<R, C>(a.line, cu);
           kt = 0;
+          end = cu.tiles(left);
         }
-        page = page_of();
       }
+      if (more) page = page_of();  // of the next tile, over the wait
       if (u >= NS) mbar_wait_or(&empty[st], par ^ 1, &gave_up);
       if (lane == 0) {
         dead_keys[st] = dead;
@@ -163,12 +166,12 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
   const float c2 = a.c2_hi;
   uint32_t qr[S::QREG ? KS : 1][S::NQ][2 * RH];  // QREG: fragments of the item's queries
   float o[NO][4], m2[2], l2[2];
-  int buf = 0, u = 0;
+  int buf = 0;
   uint32_t par = 0;
 #pragma unroll 1
   while (true) {
     // ---- a piece: tiles cu.kt .. end of an item
-    const int end = min(cu.nt, cu.kt + units - u);
+    const int end = cu.kt + cu.tiles(left);
     const int row_base = cu.m * R;  // first packed row of the item
     const int nrows = cu.rows(a.line, R);
     const int pos0 = cu.pos0();
@@ -497,8 +500,8 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
         }
       }
     }
-    u += end - cu.kt;
-    if (u == units) break;
+    left = AttnCursor::behind(left, end - cu.kt);
+    if (left == 0) break;
     cu = AttnCursor::next<R, C>(a.line, cu);
   }
 }

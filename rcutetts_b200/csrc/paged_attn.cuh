@@ -102,6 +102,12 @@ CTTS_DEV int attn_tiles(const AttnReq& r, int m, int group) {
   const int ahead = packed >= r.nn * group ? r.nn : (packed - 1) / group + 1;
   return max(1, (min(r.len, r.len - r.cnt + ahead) + C - 1) / C);
 }
+// To begin and to end an item (queries in, output out) costs about as much as
+// this many key tiles: so much of the line an item takes ahead of its tiles.
+// (Without it the CTAs that draw many short items end last: decodes with
+// chunks 39 us instead of @@, prompts 47 instead of @@.)
+constexpr int kItemCost = 2;
+
 // The row tiles of a request in order: the rows ahead of each one's end by
 // running quotient and remainder, without a division a tile.
 template <int R, int C>
@@ -134,7 +140,7 @@ CTTS_DEV long attn_units(const AttnLine& ln, const AttnReq& r) {
   AttnRowWalk<R, C> w(r, ln.group);
   long n = 0;
 #pragma unroll 1
-  for (int m = 0; m < mt; m++, w.next()) n += w.tiles();
+  for (int m = 0; m < mt; m++, w.next()) n += w.tiles() + kItemCost;
   return n * ln.n_kv;
 }
 // The line is cut into `ctas` pieces of `base` tiles, the first `rest` of them
@@ -186,7 +192,7 @@ CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
       u = attn_units<R, C>(ln, rq);
     }
     long inc = u;
-#pragma unroll 1
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
@@ -194,7 +200,7 @@ CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
     if (lane == 31) wsum[ph][warp] = inc;
     __syncthreads();
     long all = 0, ahead = 0;
-#pragma unroll 1
+#pragma unroll
     for (int w = 0; w < W; w++) {
       const long y = wsum[ph][w];
       if (w < warp) ahead += y;
@@ -238,7 +244,7 @@ CTTS_DEV int attn_pieces(const AttnLine& ln, const AttnStart& s, int more) {
 }
 
 // A place on the line: request, row tile, KV head, key tile.  A role walks its
-// CTA's pieces: tiles kt .. nt of one item, then the next item's from 0.
+// CTA's pieces: tiles kt .. of one item, then the next item's from 0.
 struct AttnCursor {
   int b, m, h, kt, nt, mt;
   int r0, cnt, nn, len;
@@ -256,18 +262,34 @@ struct AttnCursor {
 #pragma unroll 1
     for (c.m = 0;; c.m++, w.next()) {
       c.nt = w.tiles();
-      const long in = (long)c.nt * ln.n_kv;
+      const long in = (long)(c.nt + kItemCost) * ln.n_kv;
       if (skip < in || c.m + 1 >= c.mt) break;
       skip -= in;
     }
-    c.h = (unsigned)skip / (unsigned)c.nt;  // (skip is inside one row tile's heads: 31 bits)
-    c.kt = (unsigned)skip % (unsigned)c.nt;
+    const unsigned item = c.nt + kItemCost;  // (skip is inside one row tile's heads: 31 bits)
+    c.h = (unsigned)skip / item;
+    c.kt = (int)((unsigned)skip % item) - kItemCost;
     return c;
   }
+  // The CTA's first piece; left: what it has of the line (0: nothing to do).
   template <int R, int C>
-  static CTTS_DEV AttnCursor at(const AttnLine& ln, const AttnStart& s) {
-    return at<R, C>(ln, s.req, s.b, s.skip);
+  static CTTS_DEV AttnCursor at(const AttnLine& ln, const AttnStart& s, int* left) {
+    *left = (int)s.units;  // (of one CTA: 31 bits, the host checks)
+    AttnCursor c{};
+    if (*left > 0) {
+      c = at<R, C>(ln, s.req, s.b, s.skip);
+      if (c.kt < 0) {
+        *left = max(0, *left + c.kt);
+        c.kt = 0;
+      }
+    }
+    return c;
   }
+  // Tiles of the piece.
+  CTTS_DEV int tiles(int left) const { return min(nt - kt, left); }
+  // What is left of the line behind a piece of n tiles and the cost of the
+  // item that follows (0: it was the last).
+  static CTTS_DEV int behind(int left, int n) { return max(0, left - n - kItemCost); }
   // The next item, from its first tile (never called at the end of the line).
   template <int R, int C>
   static CTTS_DEV AttnCursor next(const AttnLine& ln, AttnCursor c) {

@@ -236,13 +236,13 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   __syncthreads();
   fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  const int units = __shfl_sync(0xffffffffu, (int)start.units, 0);  // (of one CTA: 31 bits, the host checks)
+  int left;
+  AttnCursor cu = AttnCursor::at<R, KT>(a.line, start, &left);
 
-  if (units > 0 && warp == W_TMA) {
+  if (left > 0 && warp == W_TMA) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them
-    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
-    int kt = cu.kt;
+    int kt = cu.kt, end = cu.kt + cu.tiles(left);  // of the piece
     auto page_of = [&]() {
       const int kk = kt * KT + 8 * lane;
       return lane < KT / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
@@ -250,18 +250,21 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     int page = page_of(), st = 0, u = 0;
     uint32_t par = 0;
 #pragma unroll 1
-    for (; u < units && !gave_up; u++) {
+    for (bool more = true; more && !gave_up; u++) {
       const int kk = kt * KT + 8 * lane, h = cu.h, slot = kk & (a.p.kv.page_size - 1);
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < KT / 8 && kk < cu.len && none);
       const int from = none ? a.p.kv.n_pages : page;  // outside the map: zeros
-      if (u + 1 < units) {  // the next tile's pages, over the waits
-        if (++kt == cu.nt) {
+      if (++kt == end) {
+        left = AttnCursor::behind(left, end - cu.kt);
+        more = left > 0;
+        if (more) {
           cu = AttnCursor::next<R, KT>(a.line, cu);
           kt = 0;
+          end = cu.tiles(left);
         }
-        page = page_of();
       }
+      if (more) page = page_of();  // of the next tile, over the waits
       const bool copies = lane < KT / 8 && (8 * lane & (box - 1)) == 0;
 #pragma unroll 1
       for (int kv = 0; kv < 2; kv++) {
@@ -288,12 +291,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         mbar_wait(&bars.k_full[w % NS], (uint32_t)(w / NS) & 1);
         mbar_wait(&bars.v_full[w % NS], (uint32_t)(w / NS) & 1);
       }
-  } else if (units > 0 && warp == W_MMA) {
+  } else if (left > 0 && warp == W_MMA) {
     // ---- MMA issue.  The warp runs through as one (what it computes with is
     // uniform), one lane issues; between its products it does next to nothing:
     // what it spends there the tensor core stands still.
     const bool leader = elect_one();
-    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
     auto scores = [&](int s, int st) {
       const uint32_t kb = desc_lo(ks + st * S::TILE, 16), qb = desc_lo(qs + s * NT * S::QTERM, 16);
       fence_after();
@@ -331,10 +333,10 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     };
     uint32_t q_par = 0, p_par = 0;  // one bit per sub-tile
     uint32_t par = 0, par_p = 0;    // of the fills of stages st (tile i) and sp (tile i - 1)
-    int st = 0, sp = 0, done = 0;
+    int st = 0, sp = 0;
 #pragma unroll 1
     while (true) {
-      const int n = __shfl_sync(0xffffffffu, min(cu.nt - cu.kt, units - done), 0);
+      const int n = __shfl_sync(0xffffffffu, cu.tiles(left), 0);
       const int nsub = __shfl_sync(0xffffffffu, cu.rows(a.line, R) > 128 ? 2 : 1, 0);
       // a turn: P.V of tile i - 1, scores of tile i
 #pragma unroll 1
@@ -372,21 +374,20 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           }
         }
       }
-      done += n;
-      if (done == units) break;
+      left = __shfl_sync(0xffffffffu, AttnCursor::behind(left, n), 0);
+      if (left == 0) break;
       cu = AttnCursor::next<R, KT>(a.line, cu);
     }
     if (gave_up) {  // MMAs in flight end before TMEM is given back
       commit(&bars.drain);
       mbar_wait(&bars.drain, 0);
     }
-  } else if (units > 0 && warp < W_MMA) {
+  } else if (left > 0 && warp < W_MMA) {
     // ---- softmax: one thread per packed row
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + S::SREG * s + lane_base, tP = tS + S::PCOL, tO = tmem + S::OREG + S::OSTEP * s + lane_base;
     const float c2 = a.c2_hi;
-    AttnCursor cu = AttnCursor::at<R, KT>(a.line, start);
     uint32_t s_par = 0, o_par = 0;
     float o_row[QF ? HD : 1];  // float32 calls: the output row so far
     // adds the product of the last tile to it
@@ -405,11 +406,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     // scores may begin), then the piece before is written out, then the next
     // one's tiles run.
     AttnCursor nx = cu;
-    int u = 0, next_u = 0, end = 0;
+    int u = 0, end = -1;  // tiles of the pieces before; of the current piece (-1: none yet)
     float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
     while (true) {
-      if (next_u < units && s * 128 < nx.rows(a.line, R)) {
+      if (left > 0 && s * 128 < nx.rows(a.line, R)) {
         const int r0 = s * 128 + (warp & 3) * 32, nrows = nx.rows(a.line, R);  // the warp's first row in the item
         // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes of a
         // row (as bf16), four rows at a time, all loads in flight before the
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         fence_async();
         mbar_arrive(&bars.q_full[s]);
       }
-      if (u < next_u && s * 128 < cu.rows(a.line, R)) {
+      if (end >= 0 && s * 128 < cu.rows(a.line, R)) {
         const int nrows = cu.rows(a.line, R);
         const bool mine = s * 128 + row < nrows, warp_on = s * 128 + (warp & 3) * 32 < nrows;
         // ---- the piece's output, or its partial state
@@ -556,12 +557,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           fence_before();
         }
       }
-      if (next_u == units) break;
+      if (left == 0) break;
       // ---- a piece: tiles cu.kt .. end of an item
+      if (end >= 0) u += end - cu.kt;
       cu = nx;
-      u = next_u;
-      end = min(cu.nt, cu.kt + units - u);
-      next_u = u + end - cu.kt;
+      end = cu.kt + cu.tiles(left);
       const int nrows = cu.rows(a.line, R);
       if (s * 128 < nrows) {  // the sub-tile has rows
         const bool warp_on = s * 128 + (warp & 3) * 32 < nrows;
@@ -727,7 +727,8 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
           mbar_arrive(&bars.p_full[s]);
         }
       }
-      if (next_u < units) nx = AttnCursor::next<R, KT>(a.line, cu);
+      left = AttnCursor::behind(left, end - cu.kt);
+      if (left > 0) nx = AttnCursor::next<R, KT>(a.line, cu);
     }
   }
   fence_before();
