@@ -616,7 +616,6 @@ auto with_shape(const ctts_paged_attn& p, F f) {
   using R1 = std::integral_constant<int, 1>;
   using R2 = std::integral_constant<int, 2>;
   auto g = [&](auto hd) {
-    if (kf && rows > 16) return f(T{}, T{}, hd, T{}, R2{});
     if (kf) return rows > 8 ? f(T{}, T{}, hd, N{}, R2{}) : f(T{}, T{}, hd, N{}, R1{});
     if (qf) return rows > 8 ? f(T{}, N{}, hd, N{}, R2{}) : f(T{}, N{}, hd, N{}, R1{});
     return rows > 8 ? f(N{}, N{}, hd, N{}, R2{}) : f(N{}, N{}, hd, N{}, R1{});
@@ -624,9 +623,9 @@ auto with_shape(const ctts_paged_attn& p, F f) {
   return p.kv.head_dim == 128 ? g(std::integral_constant<int, 128>{}) : g(std::integral_constant<int, 64>{});
 }
 
-// Chunks over a bf16 cache run on tcgen05 (paged_attn_tc.cu).
+// More than 16 packed rows in an item: on tcgen05 (paged_attn_tc.cu).
 bool use_tc(const ctts_paged_attn& p) {
-  return p.kv.dtype == CTTS_BF16 && (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) > 16;
+  return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) > 16;
 }
 
 int rows_used_of(const ctts_paged_attn& p) {

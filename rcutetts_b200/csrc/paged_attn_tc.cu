@@ -40,23 +40,33 @@ namespace ctts {
 
 namespace {
 
-// Warps: 4 of softmax per sub-tile, then one that issues MMAs and one that
-// issues copies.
-template <bool QF, int HD>
+// Warps: 4 of softmax per sub-tile, one that issues MMAs, and one that issues
+// the copies of a bf16 cache or some that bring in a float32 one.
+template <bool QF, bool KF, int HD>
 struct TcShape {
-  static constexpr int KT = QF ? 64 : 128;                // keys per tile
-  static constexpr int NSUB = QF && HD == 128 ? 1 : 2;    // three terms of 256 wide queries would not fit
-  static constexpr int R = 128 * NSUB;                    // packed rows per item
-  static constexpr int THREADS = R + 64;
-  static constexpr int NT = QF ? 3 : 1;                   // terms of queries and weights
-  static constexpr int NC = HD / 64;                      // 128-byte column blocks
-  // TMEM columns of sub-tile s: S at s * SREG, P over it (bf16) or behind it
-  // (three terms of KT / 2 columns), O at OREG + s * OSTEP
-  static constexpr uint32_t SREG = QF ? 192 : 128, PCOL = QF ? KT : 0, OREG = QF && NSUB == 2 ? 384 : 256, OSTEP = QF ? 64 : 128;
-  static_assert(OREG + (NSUB - 1) * OSTEP + HD <= 512 && PCOL + NT * (KT / 2) <= SREG && NSUB * SREG <= OREG, "TMEM columns");
-  static constexpr uint32_t QTERM = NC * 128 * 128;       // bytes of one term of one sub-tile
-  static constexpr uint32_t TILE = NC * KT * 128;         // bytes of a K or V tile
-  static constexpr int NS = QF ? (HD == 64 ? 6 : 3) : (HD == 64 ? 4 : 2);
+  static constexpr int KT = QF ? 64 : 128;                     // keys per tile
+  static constexpr int NSUB = KF || (QF && HD == 128) ? 1 : 2; // sub-tiles: as many as shared memory and registers hold
+  static constexpr int R = 128 * NSUB;                         // packed rows per item
+  // warps that bring in a float32 cache: two leave the softmax of 128 dims the
+  // registers of an output row
+  static constexpr int CW = HD == 64 ? 4 : 2;
+  static constexpr int THREADS = R + 32 + (KF ? 32 * CW : 32);
+  static constexpr int NT = QF ? 3 : 1;                        // bf16 terms of queries and weights
+  static constexpr int NK = KF ? 3 : 1;                        // of keys and values
+  static constexpr int NC = HD / 64;                           // 128-byte column blocks
+  static constexpr uint32_t QTERM = NC * 128 * 128;            // bytes of one term of one sub-tile
+  static constexpr uint32_t KTERM = NC * KT * 128;             // of one term of a K or V tile
+  static constexpr uint32_t TILE = NK * KTERM;
+  static constexpr int NS = KF ? (HD == 64 ? 3 : 1) : (QF ? (HD == 64 ? 6 : 3) : (HD == 64 ? 4 : 2));
+  // One sub-tile: the scores of tile i + 1 are computed while tile i is in its
+  // softmax, into the other of two S.  Two: they take turns instead.
+  static constexpr bool PIPE = NSUB == 1;
+  // TMEM columns of sub-tile s: S at s * SREG (PIPE: two of KT columns), P over
+  // it (bf16) or behind it (three terms of KT / 2), O at OREG + s * OSTEP
+  static constexpr uint32_t SREG = QF ? 192 : 128, PCOL = PIPE ? 2 * KT : (QF ? KT : 0);
+  static constexpr uint32_t OREG = QF && NSUB == 2 ? 384 : 256, OSTEP = QF ? 64 : 128;
+  static_assert(OREG + (NSUB - 1) * OSTEP + HD <= 512 && (PIPE ? PCOL + NT * (KT / 2) <= OREG : PCOL + NT * (KT / 2) <= SREG && NSUB * SREG <= OREG),
+                "TMEM columns");
   static constexpr size_t SMEM = (size_t)NSUB * NT * QTERM + (size_t)2 * NS * TILE + NSUB * 4 * 4096 + 1024;  // and 4 KB a softmax warp
 };
 
@@ -189,11 +199,11 @@ struct TcBars {
   uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], drain;
 };
 
-template <bool QF, int HD>
-__global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK,
+template <bool QF, bool KF, int HD>
+__global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                                     const __grid_constant__ CUtensorMap tmV,
                                                                                     const __grid_constant__ PagedAttnArgs a, int box, int order) {
-  using S = TcShape<QF, HD>;
+  using S = TcShape<QF, KF, HD>;
   constexpr int KT = S::KT, R = S::R, NS = S::NS, NT = S::NT, NC = S::NC;
   constexpr int W_MMA = 4 * S::NSUB, W_TMA = W_MMA + 1;
   constexpr int KS = KT / 16, HALF = QF ? 0 : KS / 2;  // bf16 calls: P arrives in two halves
@@ -209,9 +219,9 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
 
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
-      mbar_init(&bars.k_full[i], 1);
+      mbar_init(&bars.k_full[i], KF ? 32 * S::CW : 1);
       mbar_init(&bars.k_empty[i], 1);
-      mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.v_full[i], KF ? 32 * S::CW : 1);
       mbar_init(&bars.v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   int left;
   AttnCursor cu = AttnCursor::at<R, KT>(a.line, start, &left);
 
-  if (left > 0 && warp == W_TMA) {
+  if (!KF && left > 0 && warp == W_TMA) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
     // lanes at the boxes' starts copy them
     int kt = cu.kt, end = cu.kt + cu.tiles(left);  // of the piece
@@ -291,26 +301,119 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
         mbar_wait(&bars.k_full[w % NS], (uint32_t)(w / NS) & 1);
         mbar_wait(&bars.v_full[w % NS], (uint32_t)(w / NS) & 1);
       }
+  } else if (KF && left > 0 && warp > W_MMA) {
+    // ---- producers of a float32 cache: keys and values come in by plain
+    // loads (16 threads a row of 64 dims), 64 dims of 64 keys ahead of the
+    // ones that are being split into their bf16 terms
+    const int ct = tid - 32 * (W_MMA + 1), f4 = ct & 15, kr = ct >> 4;
+    constexpr int JOBS = 2 * NC;  // a tile: K's blocks of 64 dims, then V's
+    constexpr int RT = 2 * S::CW, NI = KT / RT;  // rows a turn, turns
+    int kt = cu.kt, end = cu.kt + cu.tiles(left), st = 0, u = 0;
+    uint32_t par = 0, dead = 0, dead_next = 0;
+    int page = -1;
+    bool more = true;
+    float4 buf[2][NI];
+    auto look = [&]() {  // lane i: the page of keys 8i..8i+7 of tile kt
+      const int kk = kt * KT + 8 * lane;
+      page = lane < 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
+      const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
+      dead_next = __ballot_sync(0xffffffffu, lane < 8 && kk < cu.len && none);
+      if (none) page = -1;
+    };
+    auto fetch = [&](int job, float4* r) {
+      const float* pool = static_cast<const float*>(job < NC ? a.p.kv.k : a.p.kv.v) + (long)cu.h * a.p.kv.head_stride + (job % NC) * 64 + f4 * 4;
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int key = kt * KT + RT * i + kr, pg = __shfl_sync(0xffffffffu, page, RT * i >> 3);
+        r[i] = make_float4(0.f, 0.f, 0.f, 0.f);  // slots behind the length and missing pages
+        if (key < cu.len && pg >= 0)
+          r[i] = *reinterpret_cast<const float4*>(pool + (long)pg * a.p.kv.page_stride + (long)(key & (a.p.kv.page_size - 1)) * a.p.kv.token_stride);
+      }
+    };
+    look();
+    fetch(0, buf[0]);
+#pragma unroll 1
+    while (more) {
+      dead = dead_next;
+#pragma unroll
+      for (int job = 0; job < JOBS; job++) {
+        if (job + 1 < JOBS) {
+          fetch(job + 1, buf[(job + 1) & 1]);
+        } else {
+          if (++kt == end) {
+            left = AttnCursor::behind(left, end - cu.kt);
+            more = left > 0;
+            if (more) {
+              cu = AttnCursor::next<R, KT>(a.line, cu);
+              kt = 0;
+              end = cu.tiles(left);
+            }
+          }
+          if (more) {
+            look();
+            fetch(0, buf[0]);
+          }
+        }
+        const int kv = job / NC, c = job % NC;
+        uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
+        if (c == 0 && u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &gave_up);
+        const uint32_t dst = (kv ? vs : ks) + st * S::TILE + c * KT * 128;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          const float4 x = buf[job & 1][i];
+          const int key = RT * i + kr;
+          uint32_t t[2][3];
+          split_bf2<3>(x.x, x.y, t[0]);
+          split_bf2<3>(x.z, x.w, t[1]);
+#pragma unroll
+          for (int k = 0; k < 3; k++)
+            asm volatile("st.shared.v2.b32 [%0], {%1,%2};" ::"r"(dst + k * S::KTERM + key * 128 + (((f4 >> 1) ^ key) & 7) * 16 + (f4 & 1) * 8),
+                         "r"(t[0][k]), "r"(t[1][k])
+                         : "memory");
+        }
+        if (c == NC - 1) {
+          if (job == NC - 1 && ct == 0) dead_keys[u & 7] = dead;
+          fence_async();
+          mbar_arrive(full);
+        }
+      }
+      u++;
+      if (++st == NS) {
+        st = 0;
+        par ^= 1;
+      }
+    }
   } else if (left > 0 && warp == W_MMA) {
     // ---- MMA issue.  The warp runs through as one (what it computes with is
     // uniform), one lane issues; between its products it does next to nothing:
     // what it spends there the tensor core stands still.
     const bool leader = elect_one();
-    auto scores = [&](int s, int st) {
+    // Products of terms i of one operand and j of the other whose orders add
+    // up to more than two are left out: they lie below 2^-24 of the whole.
+    // Small ones first: the tensor core cuts what it adds to the accumulator's
+    // precision.
+    constexpr int ORDER = (NT - 1) > (S::NK - 1) ? NT - 1 : S::NK - 1;
+    auto scores = [&](int s, int st, uint32_t col, uint64_t* bar) {
       const uint32_t kb = desc_lo(ks + st * S::TILE, 16), qb = desc_lo(qs + s * NT * S::QTERM, 16);
       fence_after();
       if (leader) {
-        // small terms first: the tensor core cuts what it adds to the
-        // accumulator's precision
+        uint32_t acc = 0;
 #pragma unroll
-        for (int t = NT - 1; t >= 0; t--)
+        for (int o = ORDER; o >= 0; o--)
 #pragma unroll
-          for (int c = 0; c < NC; c++)
+          for (int t = 0; t < NT; t++) {
+            const int j = o - t;
+            if (j < 0 || j >= S::NK) continue;
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-              mma_ss(tmem + S::SREG * s, qb + (t * S::QTERM + c * 16384 + k * 32) / 16, kb + (c * KT * 128 + k * 32) / 16, tc_idesc(KT, false),
-                     t < NT - 1 || c > 0 || k > 0);
-        umma_commit(&bars.s_full[s]);
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                mma_ss(tmem + col, qb + (t * S::QTERM + c * 16384 + k * 32) / 16, kb + (j * S::KTERM + c * KT * 128 + k * 32) / 16,
+                       tc_idesc(KT, false), acc);
+                acc = 1;
+              }
+          }
+        umma_commit(bar);
       }
       __syncwarp();
     };
@@ -319,11 +422,18 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
       fence_after();
       if (leader) {
 #pragma unroll
-        for (int t = NT - 1; t >= 0; t--)
+        for (int o = ORDER; o >= 0; o--)
 #pragma unroll
-          for (int k = k0; k < k1; k++)
-            mma_ts(tmem + S::OREG + S::OSTEP * s, tmem + S::SREG * s + S::PCOL + t * (KT / 2) + k * 8, vb + k * 128, tc_idesc(HD, true),
-                   t < NT - 1 || k > k0 ? 1u : acc);
+          for (int t = 0; t < NT; t++) {
+            const int j = o - t;
+            if (j < 0 || j >= S::NK) continue;
+#pragma unroll
+            for (int k = k0; k < k1; k++) {
+              mma_ts(tmem + S::OREG + S::OSTEP * s, tmem + S::SREG * s + S::PCOL + t * (KT / 2) + k * 8, vb + j * (S::KTERM / 16) + k * 128,
+                     tc_idesc(HD, true), acc);
+              acc = 1;
+            }
+          }
       }
       __syncwarp();
     };
@@ -338,39 +448,69 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     while (true) {
       const int n = __shfl_sync(0xffffffffu, cu.tiles(left), 0);
       const int nsub = __shfl_sync(0xffffffffu, cu.rows(a.line, R) > 128 ? 2 : 1, 0);
-      // a turn: P.V of tile i - 1, scores of tile i
+      if (S::PIPE) {
+        // a turn: scores of tile i, then P.V of tile i - 1
+        mbar_wait_or(&bars.q_full[0], q_par, &gave_up);
+        q_par ^= 1;
 #pragma unroll 1
-      for (int i = 0; i <= n; i++) {
-        if (i > 0) mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
-#pragma unroll 1
-        for (int s = 0; s < nsub; s++) {
+        for (int i = 0; i <= n; i++) {
+          if (i < n) {
+            mbar_wait_or(&bars.k_full[st], par, &gave_up);
+            scores(0, st, (i & 1) * KT, &bars.s_full[i & 1]);
+            commit(&bars.k_empty[st]);
+          }
           if (i > 0) {
-            if (HALF) {
-              mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
-              values(s, sp, 0, HALF, i > 1);
-            }
-            mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
-            p_par ^= 1u << s;
-            values(s, sp, HALF, KS, HALF ? 1u : 0u);
-            if (i == n) commit(&bars.o_full[s]);
+            mbar_wait_or(&bars.p_full[0], p_par, &gave_up);
+            p_par ^= 1;
+            mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+            values(0, sp, 0, KS, 0);
+            commit(&bars.o_full[0]);
+            commit(&bars.v_empty[sp]);
           }
           if (i < n) {
-            if (i == 0) {
-              mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
-              q_par ^= 1u << s;
+            sp = st;
+            par_p = par;
+            if (++st == NS) {
+              st = 0;
+              par ^= 1;
             }
-            if (s == 0) mbar_wait_or(&bars.k_full[st], par, &gave_up);
-            scores(s, st);
           }
         }
-        if (i > 0) commit(&bars.v_empty[sp]);
-        if (i < n) {
-          commit(&bars.k_empty[st]);
-          sp = st;
-          par_p = par;
-          if (++st == NS) {
-            st = 0;
-            par ^= 1;
+      } else {
+        // a turn: P.V of tile i - 1, scores of tile i
+#pragma unroll 1
+        for (int i = 0; i <= n; i++) {
+          if (i > 0) mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+#pragma unroll 1
+          for (int s = 0; s < nsub; s++) {
+            if (i > 0) {
+              if (HALF) {
+                mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
+                values(s, sp, 0, HALF, i > 1);
+              }
+              mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
+              p_par ^= 1u << s;
+              values(s, sp, HALF, KS, HALF ? 1u : 0u);
+              if (i == n) commit(&bars.o_full[s]);
+            }
+            if (i < n) {
+              if (i == 0) {
+                mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
+                q_par ^= 1u << s;
+              }
+              if (s == 0) mbar_wait_or(&bars.k_full[st], par, &gave_up);
+              scores(s, st, S::SREG * s, &bars.s_full[s]);
+            }
+          }
+          if (i > 0) commit(&bars.v_empty[sp]);
+          if (i < n) {
+            commit(&bars.k_empty[st]);
+            sp = st;
+            par_p = par;
+            if (++st == NS) {
+              st = 0;
+              par ^= 1;
+            }
           }
         }
       }
@@ -386,7 +526,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
     // ---- softmax: one thread per packed row
     const int s = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + S::SREG * s + lane_base, tP = tS + S::PCOL, tO = tmem + S::OREG + S::OSTEP * s + lane_base;
+    const uint32_t tS0 = tmem + S::SREG * s + lane_base, tP = tS0 + S::PCOL, tO = tmem + S::OREG + S::OSTEP * s + lane_base;
     const float c2 = a.c2_hi;
     uint32_t s_par = 0, o_par = 0;
     float o_row[QF ? HD : 1];  // float32 calls: the output row so far
@@ -574,7 +714,7 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
 #pragma unroll 1
         for (int kt = cu.kt; kt < end; kt++) {
           const int key0 = kt * KT;
-          if (s == 0 && key0 + KT > cu.len) {
+          if (!KF && s == 0 && key0 + KT > cu.len) {
             // slots behind the length may hold anything, and 0 * NaN is NaN:
             // their values become zeros (both sub-tiles' products come after
             // this sub-tile's arrival at p_half or p_full)
@@ -588,8 +728,10 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
             }
             fence_async();
           }
-          mbar_wait_or(&bars.s_full[s], s_par, &gave_up);
-          s_par ^= 1;
+          const int sb = S::PIPE ? (kt - cu.kt) & 1 : s;
+          const uint32_t tS = tS0 + (S::PIPE ? sb * KT : 0);
+          mbar_wait_or(&bars.s_full[sb], (s_par >> sb) & 1, &gave_up);
+          s_par ^= 1u << sb;
           if (warp_on) {
             fence_after();
             const uint32_t dead = dead_keys[(u + kt - cu.kt) & 7];
@@ -628,7 +770,14 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
               mn = max3(mx[0], mx[1], fmaxf(mx[2], mx[3])) * c2;
             }
             if (QF) {
-              if (kt > cu.kt) gather();
+              if (kt > cu.kt) {
+                if (S::PIPE) {  // (two sub-tiles: the scores were issued behind it)
+                  mbar_wait_or(&bars.o_full[0], o_par, &gave_up);
+                  o_par ^= 1;
+                  fence_after();
+                }
+                gather();
+              }
               const float mm = fmaxf(m, mn), f = mm == -INFINITY ? 0.0f : exp2_fast(m - mm);
               m = mm;
               l *= f;
@@ -723,6 +872,11 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
             fence_before();
           } else if (!QF) {
             mbar_arrive(&bars.p_half[s]);
+          } else if (S::PIPE && kt > cu.kt) {
+            // a warp without rows keeps step: its arrival for this tile must
+            // not count for the one before
+            mbar_wait_or(&bars.o_full[0], o_par, &gave_up);
+            o_par ^= 1;
           }
           mbar_arrive(&bars.p_full[s]);
         }
@@ -737,16 +891,29 @@ __global__ void __launch_bounds__(TcShape<QF, HD>::THREADS, 1) paged_attn_tc_ker
   if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-template <bool QF, int HD>
+template <bool QF, bool KF, int HD>
 cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
-  using S = TcShape<QF, HD>;
+  using S = TcShape<QF, KF, HD>;
   static SmemOptIn opt;
-  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_tc_kernel<QF, HD>), S::SMEM));
-  const int box = std::min(a.p.kv.page_size, S::KT);
-  CUtensorMap mk, mv;
+  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_tc_kernel<QF, KF, HD>), S::SMEM));
+  const int box = std::min(a.p.kv.page_size, (int)S::KT);
+  CUtensorMap mk{}, mv{};
   int order = 0;
-  if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
-  return launch_k(paged_attn_tc_kernel<QF, HD>, dim3(a.line.ctas), dim3(S::THREADS), S::SMEM, s, mk, mv, a, box, order);
+  if (!KF && (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)))
+    return cudaErrorInvalidValue;
+  return launch_k(paged_attn_tc_kernel<QF, KF, HD>, dim3(a.line.ctas), dim3(S::THREADS), S::SMEM, s, mk, mv, a, box, order);
+}
+
+// f(QF, KF, HD as integral constants) of the call
+template <class F>
+auto with_tc_shape(const ctts_paged_attn& p, F f) {
+  using T = std::true_type;
+  using N = std::false_type;
+  auto g = [&](auto hd) {
+    if (p.q_dtype == CTTS_BF16) return f(N{}, N{}, hd);
+    return p.kv.dtype == CTTS_F32 ? f(T{}, T{}, hd) : f(T{}, N{}, hd);
+  };
+  return p.kv.head_dim == 128 ? g(std::integral_constant<int, 128>{}) : g(std::integral_constant<int, 64>{});
 }
 
 }  // namespace
@@ -754,14 +921,12 @@ cudaError_t launch_tc(const PagedAttnArgs& a, cudaStream_t s) {
 PagedAttnTc paged_attn_tc_plan(const ctts_paged_attn& p) {
   PagedAttnTc t;
   t.ctas = device_sms();
-  t.tile_rows = p.q_dtype == CTTS_F32 && p.kv.head_dim == 128 ? 128 : 256;
+  t.tile_rows = with_tc_shape(p, [](auto q, auto k, auto hd) { return TcShape<decltype(q)::value, decltype(k)::value, decltype(hd)::value>::R; });
   return t;
 }
 
 cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, cudaStream_t s) {
-  const bool qf = a.p.q_dtype == CTTS_F32;
-  if (a.p.kv.head_dim == 64) return qf ? launch_tc<true, 64>(a, s) : launch_tc<false, 64>(a, s);
-  return qf ? launch_tc<true, 128>(a, s) : launch_tc<false, 128>(a, s);
+  return with_tc_shape(a.p, [&](auto q, auto k, auto hd) { return launch_tc<decltype(q)::value, decltype(k)::value, decltype(hd)::value>(a, s); });
 }
 
 }  // namespace ctts
