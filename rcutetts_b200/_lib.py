@@ -124,7 +124,7 @@ SIGNATURES = {
     "ctts_op_swiglu": (C.c_int, [vp, C.c_int, C.c_int, vp, vp]),
     "ctts_op_causal_conv1d": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, C.c_int,
                                         C.c_int, C.c_int, C.c_int, vp, vp]),
-    # argument structs packed by the caller (rcutetts_b200.paged)
+    # argument structs as packed bytes; torch callers: rcutetts_b200.paged
     "ctts_op_paged_plan": (C.c_int, [C.c_char_p, vp]),
     "ctts_op_paged_append": (C.c_int, [C.c_char_p, vp]),
     "ctts_op_paged_attention": (C.c_int, [C.c_char_p, vp]),

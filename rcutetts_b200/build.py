@@ -1,4 +1,5 @@
-"""Build libcutetts_b200.so (sm_100a) in-tree with nvcc.
+"""Build libcutetts_b200.so (sm_100a) in-tree with nvcc, and the torch binding
+of the paged operators beside it.
 
 Each source compiles to an object under rcutetts_b200/_build/ (in parallel,
 skipped when up to date), then one shared library is linked next to this
@@ -20,6 +21,9 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libcutetts_b200.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
+# the torch binding of the paged operators (rcutetts_b200/paged.py)
+EXT_SRC = os.path.join(HERE, "csrc_py", "paged_ext.cpp")
+EXT = os.path.join(HERE, "_paged_ext.so")
 NVFLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
            "-Xcompiler", "-fvisibility=hidden", "-I", os.path.join(ROOT, "include")]
 
@@ -74,7 +78,30 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    build_ext()
     return LIB
+
+
+def build_ext() -> str:
+    """_paged_ext.so against the installed torch, linked to the library beside it."""
+    newest = max(os.path.getmtime(p) for p in (EXT_SRC, os.path.join(ROOT, "include", "cutetts_b200.h")))
+    if os.path.exists(EXT) and os.path.getmtime(EXT) >= newest:
+        return EXT
+    import sysconfig
+
+    import torch
+
+    troot = os.path.dirname(torch.__file__)
+    inc = [os.path.join(troot, "include"), os.path.join(troot, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{p}" for p in inc] + [
+           EXT_SRC, "-o", EXT, f"-L{HERE}", "-l:libcutetts_b200.so", f"-L{os.path.join(troot, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {EXT_SRC}:\n{r.stderr[-4000:]}")
+    return EXT
 
 
 if __name__ == "__main__":

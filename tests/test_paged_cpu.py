@@ -1,12 +1,22 @@
 """Refusals of the paged KV-cache operators that need no GPU: every argument
 the host can see is checked before anything is launched."""
 import ctypes as C
+import os
+import struct
 
 import pytest
 import torch
 
-from rcutetts_b200 import _lib, paged
+from rcutetts_b200 import _lib, build
 
+if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(build.EXT)):
+    build.build()
+from rcutetts_b200 import paged  # noqa: E402
+
+# the argument structs of the C ABI (native order and alignment)
+POOL = "PPqqqiiiii4x"
+STRUCT = {"plan": struct.Struct("@PPPPPPPPPPqiiiii4x"), "append": struct.Struct("@" + POOL + "PPPPPPqqdfiiii4x"),
+          "attention": struct.Struct("@" + POOL + "PPPPPPNqqqiiiiiif4x")}
 PTR = 1 << 20  # a 16-byte aligned address that is never looked at
 
 
@@ -26,7 +36,7 @@ ATTN = dict(KV, q=PTR, out=PTR, tables=PTR, cu=PTR, lens=PTR, ws=PTR, wsb=1 << 4
 
 def pack(kind, **over):
     d = dict({"plan": PLAN, "append": APPEND, "attention": ATTN}[kind], **over)
-    return {"plan": paged._PLAN, "append": paged._APPEND, "attention": paged._ATTN}[kind].pack(*d.values())
+    return STRUCT[kind].pack(*d.values())
 
 
 @pytest.mark.parametrize("kind", ["plan", "append", "attention"])
