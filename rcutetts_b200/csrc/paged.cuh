@@ -16,8 +16,8 @@ cudaError_t launch_paged_append(const ctts_paged_append& p, cudaStream_t s);
 // Attention: how a call is laid out over the GPU; it follows from the host's
 // arguments and the device alone.
 struct PagedAttnPlan {
-  int tile_rows = 0;  // packed rows (token-major, query heads of a KV head inside) per work item
   int ctas = 0;       // persistent CTAs
+  int tile_rows = 0;  // packed rows (token-major, query heads of a KV head inside) per work item
   size_t ws_bytes = 0;
 };
 PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p);

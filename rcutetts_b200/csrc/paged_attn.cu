@@ -42,39 +42,44 @@ CTTS_DEV void ldsm4_t(uint32_t addr, uint32_t* r) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// One kernel shape.  CHUNK = false: 16 packed rows per item (single tokens and
-// short runs), the four warps share the rows and split each key tile's keys,
-// each with their own softmax states; RH = 1 when no item has more than 8
-// rows (the upper half of the MMA's rows stays zero and unread).  CHUNK =
-// true: 64 packed rows, 16 per warp, every warp takes all keys.
-template <bool QF, bool KF, int HD, bool CHUNK, int RH>
+// Short items: up to 16 packed rows (single tokens and short runs).  The four
+// warps share the rows and split each key tile's keys, each with their own
+// softmax states, which merge in warp order at the end of a piece.  RH = 1: no
+// item has more than 8 rows (the upper half of the MMA's 16 rows stays zero
+// and unread).  Bound by the cache's bytes: what there is to compute per key
+// (mma.sync m16n8k16, two products of 16 rows) is far below what the tensor
+// core's legacy path gives, so the tiles go by in a ring that one producer
+// warp fills by TMA, and two blocks an SM overlap their latencies.
+// 30 requests of 2000 to 32000 tokens, 8 KV heads of 128, bf16: 181 us, 6.5
+// TB/s (plain cp.async loads by the computing warps: 272 us).
+template <bool QF, bool KF, int HD, int RH>
 struct Shape {
-  static constexpr int R = CHUNK ? 64 : 8 * RH;
-  static constexpr int RQ = CHUNK ? 64 : 16;  // query rows held
+  static constexpr int R = 8 * RH;
+  static constexpr int RQ = 16;  // query rows held
   // bf16 terms of a float32 operand (queries and softmax weights; keys and
   // values of a float32 cache): 24 bits, so a float32 call keeps float32
   static constexpr int NQ = QF ? 3 : 1;
   static constexpr int NP = QF ? 3 : 1;
   static constexpr int ES = KF ? 4 : 2;
-  static constexpr int C = !KF && HD == 64 ? 128 : 64;  // keys per tile: 16 KB of K, and as much of V
-  static constexpr int NB = HD * ES / 128;           // 128-byte blocks of a row
-  static constexpr uint32_t TILE = NB * C * 128;  // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
+  static constexpr int C = !KF && HD == 64 ? 128 : 64;  // keys per tile: 16 KB of K (float32 of 128 dims: 32), and as much of V
+  static constexpr int NB = HD * ES / 128;              // 128-byte blocks of a row
+  static constexpr uint32_t TILE = NB * C * 128;        // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
   static constexpr uint32_t STAGE = 2 * TILE;
   static constexpr int NS = STAGE <= 32768 ? 3 : 2;
   static constexpr int QBYTES = NQ * RQ * HD * 2;
-  static constexpr int KT = CHUNK ? C / 8 : C / 32;  // 8-key column tiles per warp and key tile
-  // short runs keep their query fragments in registers where they are few
-  static constexpr bool QREG = !CHUNK && NQ * (HD / 16) * 2 * RH <= 24;
+  static constexpr int KT = C / 32;  // 8-key column tiles per warp and key tile
+  // query fragments stay in registers where they are few
+  static constexpr bool QREG = NQ * (HD / 16) * 2 * RH <= 16;
   static constexpr int CTAS = STAGE <= 32768 ? 2 : 1;  // an SM holds at least this many blocks
-  static size_t smem(int rows_used) {
-    return 1024 + (size_t)NS * STAGE + QBYTES + (CHUNK ? 0 : (size_t)4 * rows_used * (HD + 2) * 4);
-  }
+  static size_t smem(int rows_used) { return 1024 + (size_t)NS * STAGE + QBYTES + (size_t)4 * rows_used * (HD + 2) * 4; }
 };
 
-template <bool QF, bool KF, int HD, bool CHUNK, int RH>
-__global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                                                              const __grid_constant__ PagedAttnArgs a, int box, int order) {
-  using S = Shape<QF, KF, HD, CHUNK, RH>;
+template <bool QF, bool KF, int HD, int RH>
+__global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                                                       const __grid_constant__ CUtensorMap tmV,
+                                                                                       const __grid_constant__ PagedAttnArgs a, int box,
+                                                                                       int order) {
+  using S = Shape<QF, KF, HD, RH>;
   constexpr int R = S::R, C = S::C, KT = S::KT, NO = HD / 8, KS = HD / 16, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnStart start;
@@ -175,329 +180,298 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
     const int row_base = cu.m * R;  // first packed row of the item
     const int nrows = cu.rows(a.line, R);
     const int pos0 = cu.pos0();
-    {
-      if (CHUNK) sync_rows();  // the queries of the item before are read (short runs: their merge has synchronised)
-      // queries of the tile as bf16 terms; rows behind nrows are zero
-      constexpr int CH = HD / 8;
-      for (int i = tid; i < S::RQ * CH; i += kNT) {
-        const int r = i / CH, ch = i % CH;
-        float v[8];
+    // its queries as bf16 terms; rows behind nrows are zero (what read the
+    // item's before has synchronised since)
+    constexpr int CH = HD / 8;
+    for (int i = tid; i < S::RQ * CH; i += kNT) {
+      const int r = i / CH, ch = i % CH;
+      float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = 0.0f;
-        if (r < nrows) {
-          const int pr = row_base + r;
-          const long at = (long)(cu.r0 + pr / a.group) * a.p.q_ld + (long)(cu.h * a.group + pr % a.group) * HD + ch * 8;
-          if (QF) {
-            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at);
-            const float4 y = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + 4);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-          } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
-            v[0] = bf_lo(x.x); v[1] = bf_hi(x.x); v[2] = bf_lo(x.y); v[3] = bf_hi(x.y);
-            v[4] = bf_lo(x.z); v[5] = bf_hi(x.z); v[6] = bf_lo(x.w); v[7] = bf_hi(x.w);
-          }
+      for (int j = 0; j < 8; j++) v[j] = 0.0f;
+      if (r < nrows) {
+        const int pr = row_base + r;
+        const long at = (long)(cu.r0 + pr / a.group) * a.p.q_ld + (long)(cu.h * a.group + pr % a.group) * HD + ch * 8;
+        if (QF) {
+          const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at);
+          const float4 y = *reinterpret_cast<const float4*>(static_cast<const float*>(a.p.q) + at + 4);
+          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p.q) + at);
+          v[0] = bf_lo(x.x); v[1] = bf_hi(x.x); v[2] = bf_lo(x.y); v[3] = bf_hi(x.y);
+          v[4] = bf_lo(x.z); v[5] = bf_hi(x.z); v[6] = bf_lo(x.w); v[7] = bf_hi(x.w);
         }
-        uint32_t t[4][3];
-#pragma unroll
-        for (int j = 0; j < 4; j++) split_bf2<S::NQ>(v[2 * j], v[2 * j + 1], t[j]);
-#pragma unroll
-        for (int k = 0; k < S::NQ; k++)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_addr(k, r, ch)), "r"(t[0][k]), "r"(t[1][k]),
-                       "r"(t[2][k]), "r"(t[3][k])
-                       : "memory");
       }
+      uint32_t t[4][3];
 #pragma unroll
-      for (int t = 0; t < NO; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-      m2[0] = m2[1] = -INFINITY;
-      l2[0] = l2[1] = 0.0f;
-      sync_rows();
-      if (S::QREG) {
+      for (int j = 0; j < 4; j++) split_bf2<S::NQ>(v[2 * j], v[2 * j + 1], t[j]);
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-          for (int k = 0; k < S::NQ; k++) {
-            uint32_t t[4];
-            ldsm4(q_addr(k, lane & 15, 2 * ks + (lane >> 4)), t);
-#pragma unroll
-            for (int i = 0; i < 2 * RH; i++) qr[S::QREG ? ks : 0][k][i] = t[RH == 2 ? i : 2 * i];  // rows 8..15 (t[1], t[3]) are zero when RH = 1
-          }
-      }
+      for (int k = 0; k < S::NQ; k++)
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_addr(k, r, ch)), "r"(t[0][k]), "r"(t[1][k]),
+                     "r"(t[2][k]), "r"(t[3][k])
+                     : "memory");
     }
-    const int wrow = CHUNK ? warp * 16 : 0;      // the warp's rows and keys
-    const int wkey = CHUNK ? 0 : warp * (C / 4);
+#pragma unroll
+    for (int t = 0; t < NO; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+    m2[0] = m2[1] = -INFINITY;
+    l2[0] = l2[1] = 0.0f;
+    sync_rows();
+    if (S::QREG) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int k = 0; k < S::NQ; k++) {
+          uint32_t t[4];
+          ldsm4(q_addr(k, lane & 15, 2 * ks + (lane >> 4)), t);
+#pragma unroll
+          for (int i = 0; i < 2 * RH; i++) qr[S::QREG ? ks : 0][k][i] = t[RH == 2 ? i : 2 * i];  // rows 8..15 (t[1], t[3]) are zero when RH = 1
+        }
+    }
+    const int wkey = warp * (C / 4);  // the warp's keys
     // positions of the thread's two rows; rows behind the tile see nothing (their queries are zero, their states unused)
     int pr[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      const int r = wrow + gq + 8 * e;
+      const int r = gq + 8 * e;
       pr[e] = r < nrows ? pos0 + (row_base + r) / a.group : -1;
     }
-    const int plast = wrow < nrows ? pos0 + (row_base + min(nrows, wrow + 16) - 1) / a.group : -1;
-    const int pfirst = pos0 + (row_base + wrow) / a.group;
+    const int plast = pos0 + (row_base + nrows - 1) / a.group, pfirst = pos0 + row_base / a.group;
 #pragma unroll 1
     for (int kt = cu.kt; kt < end; kt++) {
-    const int key0 = kt * C + wkey;
-    mbar_wait_or(&full[buf], par, &gave_up);
-    if (key0 <= plast) {
-      const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + S::TILE;
-      const uint8_t* const kt_p = smem + buf * S::STAGE;
-      const bool tail = key0 + 8 * KT > cu.len;  // slots behind the length: their values may be anything, and 0 * NaN is NaN
-      if (!KF && tail) {
-        for (int i = lane; i < 8 * KT * (HD / 8); i += 32) {
-          const int key = wkey + i / (HD / 8);
-          if (kt * C + key >= cu.len)
-            *reinterpret_cast<uint4*>(smem + buf * S::STAGE + S::TILE + sw(key, i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        __syncwarp();
-        fence_async();  // before the next copy into the stage
-      }
-      // The tensor core cuts what it adds to the accumulator's precision, so
-      // the small products of a float32 call (all but the leading terms') are
-      // summed apart and added once.
-      float s[KT][4], lo[QF ? KT : 1][4];
-#pragma unroll
-      for (int j = 0; j < KT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < (QF ? KT : 1); j++) lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        uint32_t qa[S::NQ][4];
-#pragma unroll
-        for (int k = 0; k < S::NQ; k++) {
-          if (S::QREG) {
-            const uint32_t* q = qr[S::QREG ? ks : 0][k];
-            qa[k][0] = q[0];
-            qa[k][1] = RH == 2 ? q[1] : 0u;
-            qa[k][2] = q[RH];
-            qa[k][3] = RH == 2 ? q[3 % (2 * RH)] : 0u;
-          } else {
-            ldsm4(q_addr(k, wrow + (lane & 15), 2 * ks + (lane >> 4)), qa[k]);
+      const int key0 = kt * C + wkey;
+      mbar_wait_or(&full[buf], par, &gave_up);
+      if (key0 <= plast) {
+        const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + S::TILE;
+        const uint8_t* const kt_p = smem + buf * S::STAGE;
+        const bool tail = key0 + 8 * KT > cu.len;  // slots behind the length: their values may be anything, and 0 * NaN is NaN
+        if (!KF && tail) {
+          for (int i = lane; i < 8 * KT * (HD / 8); i += 32) {
+            const int key = wkey + i / (HD / 8);
+            if (kt * C + key >= cu.len)
+              *reinterpret_cast<uint4*>(smem + buf * S::STAGE + S::TILE + sw(key, i % (HD / 8))) = make_uint4(0u, 0u, 0u, 0u);
           }
+          __syncwarp();
+          fence_async();  // before the next copy into the stage
         }
-        if (KF) {
+        // The tensor core cuts what it adds to the accumulator's precision, so
+        // the small products of a float32 call (all but the leading terms') are
+        // summed apart and added once.
+        float s[KT][4], lo[QF ? KT : 1][4];
 #pragma unroll
-          for (int j = 0; j < KT; j++) {
-            const int key = wkey + 8 * j + gq, ch = 4 * ks + (tq >> 1);
-            const float2 x = *reinterpret_cast<const float2*>(kt_p + sw(key, ch) + (tq & 1) * 8);
-            const float2 y = *reinterpret_cast<const float2*>(kt_p + sw(key, ch + 2) + (tq & 1) * 8);
-            uint32_t b0[3], b1[3];
-            split_bf2<3>(x.x, x.y, b0);
-            split_bf2<3>(y.x, y.y, b1);
-            // products of terms whose orders add up to less than 2^-24 of the whole are left out
+        for (int j = 0; j < KT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
-            for (int sum = 2; sum >= 0; sum--)
+        for (int j = 0; j < (QF ? KT : 1); j++) lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.0f;
 #pragma unroll
-              for (int k = 0; k <= sum; k++) mma_16816(sum ? lo[QF ? j : 0] : s[j], qa[QF ? k : 0], b0[sum - k], b1[sum - k]);
-          }
-        } else {
+        for (int ks = 0; ks < KS; ks++) {
+          uint32_t qa[S::NQ][4];
 #pragma unroll
-          for (int j = 0; j < KT; j += 2) {
-            // matrices: (keys 0-7, dims lo), (keys 0-7, dims hi), (keys 8-15, lo), (keys 8-15, hi)
-            uint32_t kb[4];
-            ldsm4(kt_s + sw(wkey + 8 * j + 8 * (mi >> 1) + (lane & 7), 2 * ks + (mi & 1)), kb);
-#pragma unroll
-            for (int k = S::NQ - 1; k >= 0; k--) {
-              mma_16816(k ? lo[QF ? j : 0] : s[j], qa[k], kb[0], kb[1]);
-              mma_16816(k ? lo[QF ? j + 1 : 0] : s[j + 1], qa[k], kb[2], kb[3]);
-            }
-          }
-        }
-      }
-      if (QF) {
-#pragma unroll
-        for (int j = 0; j < KT; j++)
-#pragma unroll
-          for (int e = 0; e < 2 * RH; e++) s[j][e] += lo[QF ? j : 0][e];
-      }
-      // causal mask and missing pages; a tile that every row sees whole needs none
-      const uint32_t gone = (dead_keys[buf] >> (wkey >> 3)) & ((1u << KT) - 1);
-      if (key0 + 8 * KT - 1 > pfirst || gone) {
-#pragma unroll
-        for (int j = 0; j < KT; j++)
-#pragma unroll
-          for (int e = 0; e < 2 * RH; e++)
-            if (key0 + 8 * j + 2 * tq + (e & 1) > pr[e >> 1] || ((gone >> j) & 1)) s[j][e] = -INFINITY;
-      }
-      float f[2] = {0.0f, 0.0f}, mm[2];
-#pragma unroll
-      for (int e = 0; e < RH; e++) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < KT; j++) mx = fmaxf(mx, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m2[e], mx * c2);
-        mm[e] = mn == -INFINITY ? 0.0f : mn;
-        f[e] = exp2_fast(m2[e] - mm[e]);
-        m2[e] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KT; j++) {
-          s[j][2 * e] = exp2_fast(attn_arg<QF>(a, s[j][2 * e], mm[e]));
-          s[j][2 * e + 1] = exp2_fast(attn_arg<QF>(a, s[j][2 * e + 1], mm[e]));
-          sum += s[j][2 * e] + s[j][2 * e + 1];
-        }
-        l2[e] = l2[e] * f[e] + sum;  // this thread's share of the row sum
-      }
-#pragma unroll
-      for (int t = 0; t < NO; t++) {
-        o[t][0] *= f[0];
-        o[t][1] *= f[0];
-        if (RH == 2) {
-          o[t][2] *= f[1];
-          o[t][3] *= f[1];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < KT; j += 2) {
-        uint32_t pa[S::NP][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t t[S::NP] = {};
-          if (RH == 2 || (i & 1) == 0) split_bf2<S::NP>(s[j + (i >> 1)][2 * (i & 1)], s[j + (i >> 1)][2 * (i & 1) + 1], t);
-#pragma unroll
-          for (int k = 0; k < S::NP; k++) pa[k][i] = t[k];
-        }
-        // float32 calls: 16 keys at a time in an accumulator of their own,
-        // small products first, added to the output in float32
-        if (KF) {
-#pragma unroll
-          for (int t = 0; t < NO; t++) {
-            const int key = wkey + 8 * j + 2 * tq;
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const int kk = key + (i & 1) + 8 * (i >> 1);
-              v[i] = *reinterpret_cast<const float*>(kt_p + S::TILE + sw(kk, 2 * t + (gq >> 2)) + (gq & 3) * 4);
-              if (tail && kt * C + kk >= cu.len) v[i] = 0.0f;
-            }
-            uint32_t b0[3], b1[3];
-            split_bf2<3>(v[0], v[1], b0);
-            split_bf2<3>(v[2], v[3], b1);
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int sum = 2; sum >= 0; sum--)
-#pragma unroll
-              for (int k = 0; k <= sum; k++) mma_16816(x, pa[QF ? k : 0], b0[sum - k], b1[sum - k]);
-#pragma unroll
-            for (int e = 0; e < 2 * RH; e++) o[t][e] += x[e];
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < NO; t += 2) {
-            // matrices: (keys 0-7, dims 8t..), (keys 8-15, 8t..), (keys 0-7, 8t+8..), (keys 8-15, 8t+8..)
-            uint32_t vb[4];
-            ldsm4_t(vt_s + sw(wkey + 8 * j + 8 * (mi & 1) + (lane & 7), t + (mi >> 1)), vb);
-            if (QF) {
-              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int k = S::NP - 1; k >= 0; k--) {
-                mma_16816(x, pa[k], vb[0], vb[1]);
-                mma_16816(y, pa[k], vb[2], vb[3]);
-              }
-#pragma unroll
-              for (int e = 0; e < 2 * RH; e++) {
-                o[t][e] += x[e];
-                o[t + 1][e] += y[e];
-              }
+          for (int k = 0; k < S::NQ; k++) {
+            if (S::QREG) {
+              const uint32_t* q = qr[S::QREG ? ks : 0][k];
+              qa[k][0] = q[0];
+              qa[k][1] = RH == 2 ? q[1] : 0u;
+              qa[k][2] = q[RH];
+              qa[k][3] = RH == 2 ? q[3 % (2 * RH)] : 0u;
             } else {
-              mma_16816(o[t], pa[0], vb[0], vb[1]);
-              mma_16816(o[t + 1], pa[0], vb[2], vb[3]);
+              ldsm4(q_addr(k, lane & 15, 2 * ks + (lane >> 4)), qa[k]);
             }
           }
-        }
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[buf]);  // the stage is consumed
-    if (++buf == NS) {
-      buf = 0;
-      par ^= 1;
-    }
-    }
-
-    {  // the piece is done: to the output when it is the whole item, else to the workspace
-      const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
-      // a piece from the item's start goes to the CTA's second place, one that enters the CTA to its first
-      const int slot = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
-      float2* const pml = a.ml + (long)slot * a.tile_rows;
-      float* const part = a.acc + (long)slot * a.tile_rows * HD;
-      if (!ends && cu.kt == 0 && tid == 0) {
-        AttnPart d;
-        d.pieces = attn_pieces(a.line, start, cu.nt - end);
-        d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
-        a.parts[blockIdx.x] = d;
-      }
+          if (KF) {
 #pragma unroll
-      for (int e = 0; e < RH; e++) {
-        l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 1);
-        l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 2);
-      }
-      if (CHUNK) {
+            for (int j = 0; j < KT; j++) {
+              const int key = wkey + 8 * j + gq, ch = 4 * ks + (tq >> 1);
+              const float2 x = *reinterpret_cast<const float2*>(kt_p + sw(key, ch) + (tq & 1) * 8);
+              const float2 y = *reinterpret_cast<const float2*>(kt_p + sw(key, ch + 2) + (tq & 1) * 8);
+              uint32_t b0[3], b1[3];
+              split_bf2<3>(x.x, x.y, b0);
+              split_bf2<3>(y.x, y.y, b1);
+              // products of terms whose orders add up to less than 2^-24 of the whole are left out
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int r = wrow + gq + 8 * e;
-          if (r >= nrows) continue;
-          if (whole) {
-            const int pk = row_base + r;
-            const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD + 2 * tq;
-            const float inv = l2[e] == 0.0f ? 0.0f : 1.0f / l2[e];
+              for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
-            for (int t = 0; t < NO; t++) {
-              const float x = o[t][2 * e] * inv, y = o[t][2 * e + 1] * inv;
-              if (QF)
-                *reinterpret_cast<float2*>(static_cast<float*>(a.p.out) + at + 8 * t) = make_float2(x, y);
-              else
-                *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at + 8 * t) = pack_bf2(x, y);
+                for (int k = 0; k <= sum; k++) mma_16816(sum ? lo[QF ? j : 0] : s[j], qa[QF ? k : 0], b0[sum - k], b1[sum - k]);
             }
           } else {
-            if (tq == 0) pml[r] = make_float2(m2[e], l2[e]);
 #pragma unroll
-            for (int t = 0; t < NO; t++)
-              *reinterpret_cast<float2*>(part + (long)r * HD + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+            for (int j = 0; j < KT; j += 2) {
+              // matrices: (keys 0-7, dims lo), (keys 0-7, dims hi), (keys 8-15, lo), (keys 8-15, hi)
+              uint32_t kb[4];
+              ldsm4(kt_s + sw(wkey + 8 * j + 8 * (mi >> 1) + (lane & 7), 2 * ks + (mi & 1)), kb);
+#pragma unroll
+              for (int k = S::NQ - 1; k >= 0; k--) {
+                mma_16816(k ? lo[QF ? j : 0] : s[j], qa[k], kb[0], kb[1]);
+                mma_16816(k ? lo[QF ? j + 1 : 0] : s[j + 1], qa[k], kb[2], kb[3]);
+              }
+            }
           }
         }
-      } else {
-        // the four warps' states, merged in warp order
+        if (QF) {
+#pragma unroll
+          for (int j = 0; j < KT; j++)
+#pragma unroll
+            for (int e = 0; e < 2 * RH; e++) s[j][e] += lo[QF ? j : 0][e];
+        }
+        // causal mask and missing pages; a tile that every row sees whole needs none
+        const uint32_t gone = (dead_keys[buf] >> (wkey >> 3)) & ((1u << KT) - 1);
+        if (key0 + 8 * KT - 1 > pfirst || gone) {
+#pragma unroll
+          for (int j = 0; j < KT; j++)
+#pragma unroll
+            for (int e = 0; e < 2 * RH; e++)
+              if (key0 + 8 * j + 2 * tq + (e & 1) > pr[e >> 1] || ((gone >> j) & 1)) s[j][e] = -INFINITY;
+        }
+        float f[2] = {0.0f, 0.0f}, mm[2];
 #pragma unroll
         for (int e = 0; e < RH; e++) {
-          const int r = gq + 8 * e;
-          if (r >= nrows) continue;
-          float* w = wst + (warp * a.rows_used + r) * (HD + 2);
-          if (tq == 0) *reinterpret_cast<float2*>(w) = make_float2(m2[e], l2[e]);
+          float mx = -INFINITY;
 #pragma unroll
-          for (int t = 0; t < NO; t++)
-            *reinterpret_cast<float2*>(w + 2 + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
-        }
-        sync_rows();
-        for (int i = tid; i < nrows * (HD / 2); i += kNT) {
-          const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
-          const float* w = wst + r * (HD + 2);
-          const int ws = a.rows_used * (HD + 2);
-          float M = -INFINITY, L = 0.0f, x = 0.0f, y = 0.0f;
+          for (int j = 0; j < KT; j++) mx = fmaxf(mx, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float mn = fmaxf(m2[e], mx * c2);
+          mm[e] = mn == -INFINITY ? 0.0f : mn;
+          f[e] = exp2_fast(m2[e] - mm[e]);
+          m2[e] = mn;
+          float sum = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 4; k++) M = fmaxf(M, w[k * ws]);
-          const float mz = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float g = exp2_fast(w[k * ws] - mz);
-            L = fmaf(w[k * ws + 1], g, L);
-            x = fmaf(w[k * ws + 2 + d], g, x);
-            y = fmaf(w[k * ws + 3 + d], g, y);
+          for (int j = 0; j < KT; j++) {
+            s[j][2 * e] = exp2_fast(attn_arg<QF>(a, s[j][2 * e], mm[e]));
+            s[j][2 * e + 1] = exp2_fast(attn_arg<QF>(a, s[j][2 * e + 1], mm[e]));
+            sum += s[j][2 * e] + s[j][2 * e + 1];
           }
-          if (whole) {
-            const int pk = row_base + r;
-            const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD + d;
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            if (QF)
-              *reinterpret_cast<float2*>(static_cast<float*>(a.p.out) + at) = make_float2(x * inv, y * inv);
-            else
-              *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at) = pack_bf2(x * inv, y * inv);
+          l2[e] = l2[e] * f[e] + sum;  // this thread's share of the row sum
+        }
+#pragma unroll
+        for (int t = 0; t < NO; t++) {
+          o[t][0] *= f[0];
+          o[t][1] *= f[0];
+          if (RH == 2) {
+            o[t][2] *= f[1];
+            o[t][3] *= f[1];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < KT; j += 2) {
+          uint32_t pa[S::NP][4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t t[S::NP] = {};
+            if (RH == 2 || (i & 1) == 0) split_bf2<S::NP>(s[j + (i >> 1)][2 * (i & 1)], s[j + (i >> 1)][2 * (i & 1) + 1], t);
+#pragma unroll
+            for (int k = 0; k < S::NP; k++) pa[k][i] = t[k];
+          }
+          // float32 calls: 16 keys at a time in an accumulator of their own,
+          // small products first, added to the output in float32
+          if (KF) {
+#pragma unroll
+            for (int t = 0; t < NO; t++) {
+              const int key = wkey + 8 * j + 2 * tq;
+              float v[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int kk = key + (i & 1) + 8 * (i >> 1);
+                v[i] = *reinterpret_cast<const float*>(kt_p + S::TILE + sw(kk, 2 * t + (gq >> 2)) + (gq & 3) * 4);
+                if (tail && kt * C + kk >= cu.len) v[i] = 0.0f;
+              }
+              uint32_t b0[3], b1[3];
+              split_bf2<3>(v[0], v[1], b0);
+              split_bf2<3>(v[2], v[3], b1);
+              float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int sum = 2; sum >= 0; sum--)
+#pragma unroll
+                for (int k = 0; k <= sum; k++) mma_16816(x, pa[QF ? k : 0], b0[sum - k], b1[sum - k]);
+#pragma unroll
+              for (int e = 0; e < 2 * RH; e++) o[t][e] += x[e];
+            }
           } else {
-            if (d == 0) pml[r] = make_float2(M, L);
-            *reinterpret_cast<float2*>(part + (long)r * HD + d) = make_float2(x, y);
+#pragma unroll
+            for (int t = 0; t < NO; t += 2) {
+              // matrices: (keys 0-7, dims 8t..), (keys 8-15, 8t..), (keys 0-7, 8t+8..), (keys 8-15, 8t+8..)
+              uint32_t vb[4];
+              ldsm4_t(vt_s + sw(wkey + 8 * j + 8 * (mi & 1) + (lane & 7), t + (mi >> 1)), vb);
+              if (QF) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = S::NP - 1; k >= 0; k--) {
+                  mma_16816(x, pa[k], vb[0], vb[1]);
+                  mma_16816(y, pa[k], vb[2], vb[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2 * RH; e++) {
+                  o[t][e] += x[e];
+                  o[t + 1][e] += y[e];
+                }
+              } else {
+                mma_16816(o[t], pa[0], vb[0], vb[1]);
+                mma_16816(o[t + 1], pa[0], vb[2], vb[3]);
+              }
+            }
           }
         }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[buf]);  // the stage is consumed
+      if (++buf == NS) {
+        buf = 0;
+        par ^= 1;
+      }
+    }
+
+    // the piece is done: to the output when it is the whole item, else to the workspace
+    const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
+    // a piece from the item's start goes to the CTA's second place, one that enters the CTA to its first
+    const int slot = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
+    float2* const pml = a.ml + (long)slot * a.tile_rows;
+    float* const part = a.acc + (long)slot * a.tile_rows * HD;
+    if (!ends && cu.kt == 0 && tid == 0) {
+      AttnPart d;
+      d.pieces = attn_pieces(a.line, start, cu.nt - end);
+      d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
+      a.parts[blockIdx.x] = d;
+    }
+#pragma unroll
+    for (int e = 0; e < RH; e++) {
+      l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 1);
+      l2[e] += __shfl_xor_sync(0xffffffffu, l2[e], 2);
+    }
+    // the four warps' states, merged in warp order
+#pragma unroll
+    for (int e = 0; e < RH; e++) {
+      const int r = gq + 8 * e;
+      if (r >= nrows) continue;
+      float* w = wst + (warp * a.rows_used + r) * (HD + 2);
+      if (tq == 0) *reinterpret_cast<float2*>(w) = make_float2(m2[e], l2[e]);
+#pragma unroll
+      for (int t = 0; t < NO; t++)
+        *reinterpret_cast<float2*>(w + 2 + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
+    }
+    sync_rows();
+    for (int i = tid; i < nrows * (HD / 2); i += kNT) {
+      const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
+      const float* w = wst + r * (HD + 2);
+      const int ws = a.rows_used * (HD + 2);
+      float M = -INFINITY, L = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) M = fmaxf(M, w[k * ws]);
+      const float mz = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float g = exp2_fast(w[k * ws] - mz);
+        L = fmaf(w[k * ws + 1], g, L);
+        x = fmaf(w[k * ws + 2 + d], g, x);
+        y = fmaf(w[k * ws + 3 + d], g, y);
+      }
+      if (whole) {
+        const int pk = row_base + r;
+        const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD + d;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        if (QF)
+          *reinterpret_cast<float2*>(static_cast<float*>(a.p.out) + at) = make_float2(x * inv, y * inv);
+        else
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p.out) + at) = pack_bf2(x * inv, y * inv);
+      } else {
+        if (d == 0) pml[r] = make_float2(M, L);
+        *reinterpret_cast<float2*>(part + (long)r * HD + d) = make_float2(x, y);
       }
     }
     left = AttnCursor::behind(left, end - cu.kt);
@@ -514,7 +488,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, CHUNK, RH>::CTAS) 
 // merge in shared memory in group order.
 constexpr int kJoinThreads = 256;
 template <bool BF, int HD>
-__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a) {
   constexpr int COLS = HD / 4, G = kJoinThreads / COLS, FEW = 8;
   __shared__ float4 gv[G][COLS];
   __shared__ float2 gml[G];
@@ -582,55 +556,50 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const Pag
   }
 }
 
-template <bool QF, bool KF, int HD, bool CHUNK, int RH>
+template <bool QF, bool KF, int HD, int RH>
 int attn_ctas(int rows_used) {
-  using S = Shape<QF, KF, HD, CHUNK, RH>;
+  using S = Shape<QF, KF, HD, RH>;
   // shared memory: 228 KB an SM, of which each block takes 1 KB beside its own
   const int occ = std::max(1, std::min(4, (int)(228 * 1024 / (S::smem(rows_used) + 1024 + 512))));
   return device_sms() * occ;
 }
 
-template <bool QF, bool KF, int HD, bool CHUNK, int RH>
+template <bool QF, bool KF, int HD, int RH>
 cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
-  using S = Shape<QF, KF, HD, CHUNK, RH>;
+  using S = Shape<QF, KF, HD, RH>;
   static SmemOptIn opt;
   const size_t smem = S::smem(a.rows_used);
-  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, CHUNK, RH>), smem));
+  CTTS_LK(opt.ensure(reinterpret_cast<const void*>(paged_attn_kernel<QF, KF, HD, RH>), smem));
   CUtensorMap mk, mv;
   const int box = std::min(a.p.kv.page_size, (int)S::C);
   int order = 0;
   if (!paged_pool_map(&mk, a.p.kv.k, a.p.kv, box, &order) || !paged_pool_map(&mv, a.p.kv.v, a.p.kv, box, &order)) return cudaErrorInvalidValue;
-  return launch_k(paged_attn_kernel<QF, KF, HD, CHUNK, RH>, dim3(a.line.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);
+  return launch_k(paged_attn_kernel<QF, KF, HD, RH>, dim3(a.line.ctas), dim3(kNT + 32), smem, s, mk, mv, a, box, order);
 }
 
-// The call's mma.sync shape: f(QF, KF, HD, CHUNK, RH as integral constants).
-// Short runs share the key tile between the warps; beyond 16 packed rows
-// every warp has rows of its own (a float32 cache; over a bf16 one those
-// calls run on tcgen05).
+// f(QF, KF, HD, RH as integral constants) for short items of up to `rows`
+// packed rows.
 template <class F>
-auto with_shape(const ctts_paged_attn& p, F f) {
-  const bool qf = p.q_dtype == CTTS_F32, kf = p.kv.dtype == CTTS_F32;
-  const long rows = (long)p.max_new * (p.n_heads / p.kv.n_kv_heads);
+auto with_shape(const ctts_paged_attn& p, int rows, F f) {
   using T = std::true_type;
   using N = std::false_type;
-  using R1 = std::integral_constant<int, 1>;
-  using R2 = std::integral_constant<int, 2>;
-  auto g = [&](auto hd) {
-    if (kf) return rows > 8 ? f(T{}, T{}, hd, N{}, R2{}) : f(T{}, T{}, hd, N{}, R1{});
-    if (qf) return rows > 8 ? f(T{}, N{}, hd, N{}, R2{}) : f(T{}, N{}, hd, N{}, R1{});
-    return rows > 8 ? f(N{}, N{}, hd, N{}, R2{}) : f(N{}, N{}, hd, N{}, R1{});
+  auto g = [&](auto q, auto k, auto hd) {
+    return rows > 8 ? f(q, k, hd, std::integral_constant<int, 2>{}) : f(q, k, hd, std::integral_constant<int, 1>{});
   };
-  return p.kv.head_dim == 128 ? g(std::integral_constant<int, 128>{}) : g(std::integral_constant<int, 64>{});
+  auto h = [&](auto hd) {
+    if (p.kv.dtype == CTTS_F32) return g(T{}, T{}, hd);
+    return p.q_dtype == CTTS_F32 ? g(T{}, N{}, hd) : g(N{}, N{}, hd);
+  };
+  return p.kv.head_dim == 128 ? h(std::integral_constant<int, 128>{}) : h(std::integral_constant<int, 64>{});
 }
 
-// More than 16 packed rows in an item: on tcgen05 (paged_attn_tc.cu).
-bool use_tc(const ctts_paged_attn& p) {
-  return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) > 16;
-}
-
-int rows_used_of(const ctts_paged_attn& p) {
-  return (int)std::min(16L, std::max(1L, (long)p.max_new * (p.n_heads / p.kv.n_kv_heads)));
-}
+// Items of up to 16 packed rows run on this file's kernel, calls with longer
+// ones on the tcgen05 kernel (paged_attn_tc.cu) -- their short requests too: a
+// tile of 128 rows costs a short item as much as a long one, yet two launches
+// after one another took longer (43 decodes and 5 chunks of 200 to 512: 40 us
+// against 35).
+bool is_short(const ctts_paged_attn& p) { return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) <= 16; }
+int rows_used_of(const ctts_paged_attn& p) { return std::max(1, p.max_new * (p.n_heads / p.kv.n_kv_heads)); }
 
 }  // namespace
 
@@ -659,18 +628,18 @@ bool paged_pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, i
 
 PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
   PagedAttnPlan pl;
-  if (use_tc(p)) {
-    const PagedAttnTc t = paged_attn_tc_plan(p);
-    pl.ctas = t.ctas;
-    pl.tile_rows = t.tile_rows;
-  } else {
-    with_shape(p, [&](auto q, auto k, auto hd, auto ch, auto rh) {
-      constexpr bool QF = decltype(q)::value, KF = decltype(k)::value, CH = decltype(ch)::value;
+  if (is_short(p)) {
+    const int rows = rows_used_of(p);
+    with_shape(p, rows, [&](auto q, auto k, auto hd, auto rh) {
+      constexpr bool QF = decltype(q)::value, KF = decltype(k)::value;
       constexpr int HD = decltype(hd)::value, RH = decltype(rh)::value;
-      pl.ctas = attn_ctas<QF, KF, HD, CH, RH>(rows_used_of(p));
-      pl.tile_rows = Shape<QF, KF, HD, CH, RH>::R;
+      pl.ctas = attn_ctas<QF, KF, HD, RH>(rows);
+      pl.tile_rows = Shape<QF, KF, HD, RH>::R;
       return 0;
     });
+  } else {
+    pl.ctas = device_sms();
+    pl.tile_rows = paged_attn_tc_rows(p);
   }
   pl.ws_bytes = pl.ctas * (sizeof(AttnPart) + (size_t)2 * pl.tile_rows * (p.kv.head_dim + 2) * sizeof(float));
   return pl;
@@ -694,7 +663,6 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   ln.n_kv = p.kv.n_kv_heads;
   ln.ctas = pl.ctas;
   a.tile_rows = pl.tile_rows;
-  a.rows_used = rows_used_of(p);
   const double c2 = (double)p.scale * 1.4426950408889634;
   a.c2_hi = (float)c2;
   // the first part below the factor, so that the second is positive: -inf times either is -inf
@@ -703,14 +671,15 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   a.parts = static_cast<AttnPart*>(p.workspace);
   a.acc = reinterpret_cast<float*>(a.parts + pl.ctas);
   a.ml = reinterpret_cast<float2*>(a.acc + (size_t)2 * pl.ctas * pl.tile_rows * p.kv.head_dim);
-  if (use_tc(p))
-    CTTS_LK(launch_paged_attn_tc(a, s));
-  else
-    CTTS_LK(with_shape(p, [&](auto q, auto k, auto hd, auto ch, auto rh) {
-      return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(ch)::value, decltype(rh)::value>(a, s);
+  if (is_short(p)) {
+    a.rows_used = rows_used_of(p);
+    CTTS_LK(with_shape(p, a.rows_used, [&](auto q, auto k, auto hd, auto rh) {
+      return launch_attn<decltype(q)::value, decltype(k)::value, decltype(hd)::value, decltype(rh)::value>(a, s);
     }));
-  const int rows = (int)std::min((long)a.tile_rows, (long)p.max_new * a.group);
-  const dim3 grid(a.line.ctas, rows > 16 ? 16 : std::min(rows, 4)), block(kJoinThreads);
+  } else {
+    CTTS_LK(launch_paged_attn_tc(a, s));
+  }
+  const dim3 grid(pl.ctas, is_short(p) ? std::min(a.rows_used, 4) : 16), block(kJoinThreads);
   const bool bf = p.q_dtype == CTTS_BF16;
   if (p.kv.head_dim == 64)
     return bf ? launch_k(paged_attn_join_kernel<true, 64>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 64>, grid, block, 0, s, a);

@@ -35,7 +35,7 @@ struct PagedAttnArgs {
   AttnLine line;
   int group = 1, shift = 0;      // query heads per KV head, log2 of the page size
   int tile_rows = 0;             // packed rows per item
-  int rows_used = 0;             // packed rows an item can have
+  int rows_used = 0;             // packed rows a short item can have
   float c2_hi = 0, c2_lo = 0;    // scale * log2(e): scores in powers of two
   AttnPart* parts = nullptr;     // [ctas]
   float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum (in powers of two), sum
@@ -355,11 +355,8 @@ CTTS_DEV void mbar_arrive(uint64_t* bar) {
 }
 CTTS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// tcgen05 form (paged_attn_tc.cu): chunks over a bf16 cache.
-struct PagedAttnTc {
-  int tile_rows = 0, ctas = 0;
-};
-PagedAttnTc paged_attn_tc_plan(const ctts_paged_attn& p);
+// Long items on tcgen05 (paged_attn_tc.cu).
+int paged_attn_tc_rows(const ctts_paged_attn& p);  // packed rows per item
 cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, cudaStream_t s);
 
 }  // namespace ctts

@@ -918,11 +918,8 @@ auto with_tc_shape(const ctts_paged_attn& p, F f) {
 
 }  // namespace
 
-PagedAttnTc paged_attn_tc_plan(const ctts_paged_attn& p) {
-  PagedAttnTc t;
-  t.ctas = device_sms();
-  t.tile_rows = with_tc_shape(p, [](auto q, auto k, auto hd) { return TcShape<decltype(q)::value, decltype(k)::value, decltype(hd)::value>::R; });
-  return t;
+int paged_attn_tc_rows(const ctts_paged_attn& p) {
+  return with_tc_shape(p, [](auto q, auto k, auto hd) { return TcShape<decltype(q)::value, decltype(k)::value, decltype(hd)::value>::R; });
 }
 
 cudaError_t launch_paged_attn_tc(const PagedAttnArgs& a, cudaStream_t s) {
