@@ -354,11 +354,13 @@ CTTS_API int ctts_op_embed_gather(const float* table, int vocab, int H, const in
  * new keys and values into their slots) and attention (the new rows of every
  * request over its pages).  No counterpart in the reference, whose cache is
  * one growing vector per utterance (qwen.rs:139-149); ctts_kv_* is the
- * contiguous form of this framework.  All pointers are device pointers, every
- * call is asynchronous on `stream`, allocates nothing and can be captured in
- * a CUDA graph.  Arguments the host can see are checked (CTTS_ERR_ARG,
- * CTTS_ERR_RANGE); lengths, offsets and page numbers live on the device and
- * are clamped there, so a bad one never reads or writes out of range. */
+ * contiguous form of this framework.  All pointers are device pointers of the
+ * current device, every call is asynchronous on `stream`, allocates nothing
+ * and can be captured in a CUDA graph.  Arguments the host can see are checked
+ * (CTTS_ERR_ARG, CTTS_ERR_RANGE); lengths, offsets and page numbers live on
+ * the device and are clamped there, so a bad one never reads or writes out of
+ * range.  Waits inside a kernel are bounded; one that gives up, which no valid
+ * call reaches, ends the kernel without a code, as in ctts_op_linear_noalloc. */
 
 /* K and V pools of n_pages pages of page_size token slots (a power of two,
  * 8..256).  Element d of KV head h of slot t of page p lies at
@@ -436,14 +438,15 @@ CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
  * key (its position is negative, or only pages with numbers outside
  * 0..n_pages-1, whose keys are hidden) gives zeros; rows behind
  * cu_rows[batch] are left as they were.  Slots at and behind a request's
- * length are never read into a result, whatever they hold.
+ * length never reach a result, whatever they hold.  (Of the keys ahead of a
+ * row that are its request's own later rows only finite ones are without
+ * effect: weight 0 times an infinite or NaN value is NaN.)  out may be q.
  * max_new is an upper bound of the requests' new rows (rows beyond it are
  * left as they were); a length above max_pages*page_size is cut to that.
  * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
  * n_heads / n_kv_heads <= 16.  Scores, softmax and sums are float32.  With
  * bf16 queries the softmax weights enter the product with V in bf16; with
- * float32 queries every product carries at least 16 significant bits of the
- * weights and 24 of the scores' operands.
+ * float32 queries every operand carries 24 bits.
  * The result depends on the split of the work over the GPU, which follows
  * from the lengths: the same call gives the same bits.
  * workspace: ctts_op_paged_attention_workspace bytes, 16-byte aligned, no

@@ -86,6 +86,7 @@ extern "C" int ctts_op_paged_append(const ctts_paged_append* p, void* stream) {
   if (rc != CTTS_OK) return rc;
   CTTS_REQ((p->x_dtype == CTTS_F32 || p->x_dtype == CTTS_BF16) && (p->q_dtype == CTTS_F32 || p->q_dtype == CTTS_BF16), CTTS_ERR_ARG,
            "bad dtype");
+  CTTS_REQ(p->rows <= 1 << 30, CTTS_ERR_RANGE, "too many rows");
   CTTS_REQ(p->rows >= 0 && p->theta > 0.0 && std::isfinite(p->theta) && p->eps >= 0.0f, CTTS_ERR_ARG, "bad size, theta or eps");
   CTTS_REQ(!p->q_norm == !p->k_norm, CTTS_ERR_ARG, "q_norm and k_norm come together");
   const int64_t width = (int64_t)(p->n_heads + 2 * p->kv.n_kv_heads) * p->kv.head_dim;

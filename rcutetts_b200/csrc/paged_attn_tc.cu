@@ -148,16 +148,22 @@ CTTS_DEV float2 add2(float2 x, float2 y) {
       : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return r;
 }
+CTTS_DEV float max_nan(float a, float b) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^x for a pair of x <= 127 without the special function unit, which makes
 // four results a clock and scheduler and is what the softmax of bf16 calls
 // waits for: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it
 // in the low bits) and |f| <= 1/2, 2^f by its cubic of least relative error
 // (a weighted least-squares fit; off by 7.5e-5, a fiftieth of the rounding to
-// bf16 that follows), n added to the exponent.  Below 2^-126: 2^-126.
+// bf16 that follows), n added to the exponent.  Below 2^-126: 2^-126; of NaN:
+// not finite in bf16.
 CTTS_DEV float2 exp2_poly(float2 x) {
   constexpr float kMagic = 12582912.0f;
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
+  x.x = max_nan(x.x, -126.0f);
+  x.y = max_nan(x.y, -126.0f);
   const float2 t = add2(x, make_float2(kMagic, kMagic));
   const float2 n = add2(t, make_float2(-kMagic, -kMagic));
   const float2 f = add2(x, make_float2(-n.x, -n.y));

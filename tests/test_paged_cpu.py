@@ -74,7 +74,7 @@ POOL_BAD = [
     (dict(theta=0.0), _lib.ERR_ARG), (dict(theta=float("nan")), _lib.ERR_ARG), (dict(theta=float("inf")), _lib.ERR_ARG), (dict(eps=-1.0), _lib.ERR_ARG),
     (dict(eps=float("nan")), _lib.ERR_ARG), (dict(rows=-1), _lib.ERR_ARG), (dict(heads=10), _lib.ERR_ARG), (dict(heads=0), _lib.ERR_ARG),
     (dict(xt=2), _lib.ERR_ARG), (dict(qt=-1), _lib.ERR_ARG), (dict(x=PTR + 4), _lib.ERR_ARG), (dict(q=PTR + 8), _lib.ERR_ARG),
-    (dict(qn=PTR + 4), _lib.ERR_ARG), (dict(kn=PTR + 8), _lib.ERR_ARG),
+    (dict(qn=PTR + 4), _lib.ERR_ARG), (dict(kn=PTR + 8), _lib.ERR_ARG), (dict(rows=0x7fffffff), _lib.ERR_RANGE),
 ])
 def test_append_refuses(over, code):
     assert call("ctts_op_paged_append", pack("append", **over))[0] == code

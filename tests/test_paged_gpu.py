@@ -639,3 +639,69 @@ def test_append_other_orders_in_memory():
     for kk, vv in ((side[:, 0], side[:, 1]), outer):
         paged.paged_append(x, kk, vv, pos, slots, 4)
         assert torch.equal(kk, k) and torch.equal(vv, v)
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("ctx, new", [([300, 0, 9000], 1), ([300, 0, 2000], 90)])
+def test_output_over_the_queries(q_t, kv_t, ctx, new):
+    c = Case(ctx, [new] * 3, 4, 2, 64, 16, q_t, kv_t, seed=12)
+    want = c.run()
+    c.q = c.q.clone()
+    assert torch.equal(c.run(out=c.q), want)
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+def test_bad_values_stay_with_their_request(q_t, kv_t, hd, new):
+    """A NaN key, an infinite value or a NaN query reaches the rows that see it and no other request's."""
+    c = Case([200, 90, 300], [new] * 3, 4, 2, hd, 16, q_t, kv_t, seed=14)
+    want = c.run()
+    for j in (0, 3, 6, 7, 130):  # key positions that different parts of a tile hold
+        page, slot = int(c.tables[2, j // 16]), j % 16
+        keep = c.k[page, slot, 1].clone()
+        c.k[page, slot, 1] = float("nan")
+        out = c.run()
+        c.k[page, slot, 1] = keep
+        b2, rest = out[int(c.cu[2]):], out[: int(c.cu[2])]
+        assert not torch.isfinite(b2[:, 2:]).any() and torch.equal(b2[:, :2], want[int(c.cu[2]):, :2])
+        assert torch.equal(rest, want[: int(c.cu[2])])
+    page = int(c.tables[0, 3])
+    keep = c.v[page, 5, 0, 7].clone()
+    c.v[page, 5, 0, 7] = float("inf")
+    out = c.run()
+    c.v[page, 5, 0, 7] = keep
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[: new, :2, 7] = True
+    assert not torch.isfinite(out[bad]).any() and torch.equal(out[~bad], want[~bad])
+    c.q[new // 2, 1, 0] = float("nan")
+    out = c.run()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[new // 2, 1] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], want[~bad])
+
+
+def test_another_stream_owns_what_it_uses():
+    """Calls given a stream: outputs and workspaces come from that stream's memory, so work on the current one cannot reuse them."""
+    c = Case([900, 4000, 40], [1, 1, 1], 4, 2, 64, 16, BF16, BF16)
+    x = torch.randn(3, 8 * 64, device="cuda").to(BF16)
+    want = c.run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    need = paged.paged_attention_workspace(c.q, c.k, c.v, 1)
+    for how in (side, side.cuda_stream):
+        torch.cuda._sleep(2_000_000)  # the current stream is busy
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000)
+        outs = []
+        for _ in range(4):
+            outs.append(c.run(stream=how))
+            torch.empty(need, dtype=torch.uint8, device="cuda").fill_(255)
+            step = paged.paged_plan(ints([0, 5]), ints([1, 2]), torch.zeros(2, 4, dtype=torch.int32, device="cuda"), ints([1, 2, 3]), ints([3]), 16, 3)
+            torch.full((64,), -9, dtype=torch.int32, device="cuda")
+        side.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+        torch.cuda.synchronize()
+        assert step.state.tolist() == [2, 3, 2, 1]
+    with pytest.raises((TypeError, AttributeError)):
+        c.run(stream="no stream")
