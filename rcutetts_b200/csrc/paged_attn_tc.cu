@@ -133,14 +133,6 @@ CTTS_DEV float2 fma2(float2 x, float a, float b) {  // x * a + b
       : "f"(x.x), "f"(x.y), "f"(a), "f"(b));
   return r;
 }
-CTTS_DEV float2 fma2(float2 x, float2 y, float b) {  // x * y + b
-  float2 r;
-  asm("{\n\t.reg .b64 x, y, b;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 b, {%6, %6};\n\t"
-      "fma.rn.f32x2 x, x, y, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(b));
-  return r;
-}
 CTTS_DEV float2 add2(float2 x, float2 y) {
   float2 r;
   asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
@@ -148,34 +140,6 @@ CTTS_DEV float2 add2(float2 x, float2 y) {
       : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return r;
 }
-CTTS_DEV float max_nan(float a, float b) {  // NaN if one is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// 2^x for a pair of x <= 127 without the special function unit, which makes
-// four results a clock and scheduler and is what the softmax of bf16 calls
-// waits for: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it
-// in the low bits) and |f| <= 1/2, 2^f by its cubic of least relative error
-// (a weighted least-squares fit; off by 7.5e-5, a fiftieth of the rounding to
-// bf16 that follows), n added to the exponent.  Below 2^-126: 2^-126; of NaN:
-// not finite in bf16.
-CTTS_DEV float2 exp2_poly(float2 x) {
-  constexpr float kMagic = 12582912.0f;
-  x.x = max_nan(x.x, -126.0f);
-  x.y = max_nan(x.y, -126.0f);
-  const float2 t = add2(x, make_float2(kMagic, kMagic));
-  const float2 n = add2(t, make_float2(-kMagic, -kMagic));
-  const float2 f = add2(x, make_float2(-n.x, -n.y));
-  float2 r = fma2(f, 0.0551716685f, 0.2426111251f);
-  r = fma2(r, f, 0.6932609677f);
-  r = fma2(r, f, 0.9999280572f);
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
-}
-
-// Of the 16 pairs of a turn, every kPolyEvery-th by exp2_poly (0: none).
-constexpr int kPolyEvery = 4;
 
 // Byte offsets of packed rows p, p + 4, p + 8, ... (row of q times its stride
 // plus head times width), one division for all of them.
@@ -761,8 +725,8 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
               tmem_st_wait();
             }
             float mn;
+            uint32_t x[KT];
             {
-              uint32_t x[KT];
 #pragma unroll
               for (int c = 0; c < KT; c += 32) tmem_ld32_nowait(tS + c, x + c);
               tmem_wait();
@@ -811,8 +775,8 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
               }
             }
             const float mz = m == -INFINITY ? 0.0f : m;
-            // the weights, 32 keys at a time from scores read again (bf16
-            // calls: over scores already read)
+            // the weights, 32 keys at a time (bf16 calls from the scores in
+            // registers; float32 ones read theirs again)
             if (QF) {
               float sum[2] = {0.f, 0.f};
 #pragma unroll 1
@@ -843,30 +807,16 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                   float2 e = fma2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, -mz);
-                  if (kPolyEvery && j % (kPolyEvery + !kPolyEvery) == kPolyEvery - 1)
-                    e = exp2_poly(e);
-                  else
-                    e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                  e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                   sum[j & 1] = add2(sum[j & 1], e);
                   p[j] = pack_bf2(e.x, e.y);
                 }
                 tmem_st16(tP + (c >> 1), p);
               };
-              uint32_t x[32], y[32];
-              tmem_ld32_nowait(tS, x);
-              tmem_wait();
-              pin32(x);
-#pragma unroll 1
-              for (int c = 0; c < KT; c += 64) {
-                tmem_ld32_nowait(tS + c + 32, y);
-                weights(x, c);
-                tmem_wait();
-                pin32(y);
-                if (c + 64 < KT) tmem_ld32_nowait(tS + c + 64, x);
-                weights(y, c + 32);
-                if (c + 64 < KT) {
-                  tmem_wait();
-                  pin32(x);
+#pragma unroll
+              for (int c = 0; c < KT; c += 32) {
+                weights(x + c, c);
+                if (c + 32 == HALF * 16) {
                   tmem_st_wait();
                   fence_before();
                   mbar_arrive(&bars.p_half[s]);
