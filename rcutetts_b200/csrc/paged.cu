@@ -178,10 +178,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const ctts_pag
 // same dims in a lane, so a lane computes its V angles once for all of them
 // (after the first heads' loads are in flight), and nothing is shared or
 // waited for between warps.  Few rows (a decode step): several warps a row.
-// 16381 rows, 16 + 2 x 8 heads of 128, bf16: @@ us, @@ TB/s (one row a block
-// and its angles through shared memory: 89 us).
+// 16381 rows, 16 + 2 x 8 heads of 128, bf16: 55 us, 4.9 TB/s (one row a block
+// and its angles through shared memory: 89 us; four passes in flight at fewer
+// warps: 58 us, eight: 64 us).  4001 rows, 12 + 2 x 4 heads of 64, float32:
+// 9.5 us, 4.3 TB/s.
 constexpr int kAppWarps = 4;   // a block
-constexpr int kAppAhead = 4;   // loads in flight: passes of a warp
+constexpr int kAppAhead = 2;   // loads in flight: passes of a warp
 
 // Turns per position of each frequency: theta^(-2i/hd) / (2 pi).  In double
 // and reduced to a fraction of a turn before rounding: in float32 an angle of
@@ -222,7 +224,7 @@ CTTS_DEV void widen(const uint4& u, float* v) {
 
 // `parts` warps a row; V = 4 (float32 x) or 8 (bf16)
 template <int V, int HD>
-__global__ void __launch_bounds__(kAppWarps * 32, V == 8 ? 5 : 6) paged_append_kernel(const ctts_paged_append a, const __grid_constant__ AppFreq fr, int shift,
+__global__ void __launch_bounds__(kAppWarps * 32, V == 8 ? 7 : 8) paged_append_kernel(const ctts_paged_append a, const __grid_constant__ AppFreq fr, int shift,
                                                                       int parts) {
   constexpr int HALF = HD / 2, L = HALF / V, AT_ONCE = 32 / L, ES = 16 / V;
   grid_dep_enter();

@@ -104,8 +104,8 @@ CTTS_DEV int attn_tiles(const AttnReq& r, int m, int group) {
 }
 // To begin and to end an item (queries in, output out) costs about as much as
 // this many key tiles: so much of the line an item takes ahead of its tiles.
-// (Without it the CTAs that draw many short items end last: decodes with
-// chunks 39 us instead of @@, prompts 47 instead of @@.)
+// (Without it the CTAs that draw many short items end last: 43 decodes with 5
+// chunks of 200 to 512 took 39 us instead of 34.)
 constexpr int kItemCost = 2;
 
 // The row tiles of a request in order: the rows ahead of each one's end by
