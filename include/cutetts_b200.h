@@ -413,7 +413,8 @@ CTTS_API int ctts_op_paged_plan(const ctts_paged_plan* p, void* stream);
  * far positions keep theirs).  Queries go to q [rows, n_heads, head_dim],
  * keys and values to slots[row] of the pools, each rounded once to its type.
  * A row whose slot lies outside the pools (-1: padding) writes nothing, its
- * query included.  The slots of one call are distinct.  x_ld and q_ld are row
+ * query included.  The slots of one call are distinct; x, q and the pools do
+ * not overlap.  x_ld and q_ld are row
  * strides in elements (multiples of 16 bytes); x, q, q_norm and k_norm are
  * 16-byte aligned. */
 typedef struct {
@@ -460,7 +461,7 @@ typedef struct {
   size_t workspace_bytes;
   int64_t q_ld, out_ld, table_ld;
   int batch, rows, n_heads, max_pages, max_new, q_dtype;
-  float scale; /* > 0 */
+  float scale; /* 1e-20 .. 1e20 */
 } ctts_paged_attn;
 CTTS_API int ctts_op_paged_attention(const ctts_paged_attn* p, void* stream);
 /* Workspace bytes a call with these sizes needs on the current device (the

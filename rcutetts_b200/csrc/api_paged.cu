@@ -116,7 +116,8 @@ extern "C" int ctts_op_paged_attention_workspace(const ctts_paged_attn* p, size_
 extern "C" int ctts_op_paged_attention(const ctts_paged_attn* p, void* stream) {
   int rc = check_attn(p);
   if (rc != CTTS_OK) return rc;
-  CTTS_REQ(p->scale > 0.0f && std::isfinite(p->scale), CTTS_ERR_ARG, "scale must be positive");
+  // (its factor to powers of two has to stay clear of zero and infinity, which make NaN of hidden scores)
+  CTTS_REQ(p->scale >= 1e-20f && p->scale <= 1e20f, CTTS_ERR_ARG, "scale must lie between 1e-20 and 1e20");
   const int64_t width = (int64_t)p->n_heads * p->kv.head_dim;
   CTTS_REQ(stride_ok(p->q_ld, width, p->q_dtype) && stride_ok(p->out_ld, width, p->q_dtype) && p->table_ld >= p->max_pages, CTTS_ERR_ARG,
            "q_ld, out_ld and table_ld must hold a row (q_ld and out_ld in multiples of 16 bytes)");

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
   };
   // 16-byte chunk of a key's row in a tile
   auto sw = [](int key, int chunk) { return (uint32_t)(chunk >> 3) * (C * 128) + (uint32_t)key * 128 + (uint32_t)((chunk ^ key) & 7) * 16u; };
-  const float c2 = a.c2_hi;
+  const float c2 = a.c2;
   uint32_t qr[S::QREG ? KS : 1][S::NQ][2 * RH];  // QREG: fragments of the item's queries
   float o[NO][4], m2[2], l2[2];
   int buf = 0;
@@ -327,15 +327,15 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
           for (int j = 0; j < KT; j++) mx = fmaxf(mx, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m2[e], mx * c2);
+          const float mn = fmaxf(m2[e], mx);
           mm[e] = mn == -INFINITY ? 0.0f : mn;
-          f[e] = exp2_fast(m2[e] - mm[e]);
+          f[e] = exp2_fast(attn_arg(m2[e], mm[e], c2));
           m2[e] = mn;
           float sum = 0.0f;
 #pragma unroll
           for (int j = 0; j < KT; j++) {
-            s[j][2 * e] = exp2_fast(attn_arg<QF>(a, s[j][2 * e], mm[e]));
-            s[j][2 * e + 1] = exp2_fast(attn_arg<QF>(a, s[j][2 * e + 1], mm[e]));
+            s[j][2 * e] = exp2_fast(attn_arg(s[j][2 * e], mm[e], c2));
+            s[j][2 * e + 1] = exp2_fast(attn_arg(s[j][2 * e + 1], mm[e], c2));
             sum += s[j][2 * e] + s[j][2 * e + 1];
           }
           l2[e] = l2[e] * f[e] + sum;  // this thread's share of the row sum
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
       const float mz = M == -INFINITY ? 0.0f : M;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const float g = exp2_fast(w[k * ws] - mz);
+        const float g = exp2_fast(attn_arg(w[k * ws], mz, c2));
         L = fmaf(w[k * ws + 1], g, L);
         x = fmaf(w[k * ws + 2 + d], g, x);
         y = fmaf(w[k * ws + 3 + d], g, y);
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
         const float2 ml = a.ml[at];
         const float4 w = *reinterpret_cast<const float4*>(a.acc + at * HD + 4 * col);
         const float mn = fmaxf(m, ml.x), mz = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2_fast(m - mz), g = exp2_fast(ml.x - mz);
+        const float f = exp2_fast(attn_arg(m, mz, a.c2)), g = exp2_fast(attn_arg(ml.x, mz, a.c2));
         m = mn;
         l = fmaf(ml.y, g, l * f);
         v.x = fmaf(w.x, g, v.x * f);
@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
         v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < G; k++) {
-          const float g = exp2_fast(gml[k].x - M);
+          const float g = exp2_fast(attn_arg(gml[k].x, M, a.c2));
           const float4 w = gv[k][col];
           l = fmaf(gml[k].y, g, l);
           v.x = fmaf(w.x, g, v.x);
@@ -663,11 +663,7 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   ln.n_kv = p.kv.n_kv_heads;
   ln.ctas = pl.ctas;
   a.tile_rows = pl.tile_rows;
-  const double c2 = (double)p.scale * 1.4426950408889634;
-  a.c2_hi = (float)c2;
-  // the first part below the factor, so that the second is positive: -inf times either is -inf
-  if ((double)a.c2_hi >= c2) a.c2_hi = std::nextafter(a.c2_hi, 0.0f);
-  a.c2_lo = (float)(c2 - (double)a.c2_hi);
+  a.c2 = (float)((double)p.scale * 1.4426950408889634);
   a.parts = static_cast<AttnPart*>(p.workspace);
   a.acc = reinterpret_cast<float*>(a.parts + pl.ctas);
   a.ml = reinterpret_cast<float2*>(a.acc + (size_t)2 * pl.ctas * pl.tile_rows * p.kv.head_dim);

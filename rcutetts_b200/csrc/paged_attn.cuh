@@ -36,9 +36,9 @@ struct PagedAttnArgs {
   int group = 1, shift = 0;      // query heads per KV head, log2 of the page size
   int tile_rows = 0;             // packed rows per item
   int rows_used = 0;             // packed rows a short item can have
-  float c2_hi = 0, c2_lo = 0;    // scale * log2(e): scores in powers of two
+  float c2 = 0;                  // scale * log2(e): scores to powers of two
   AttnPart* parts = nullptr;     // [ctas]
-  float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum (in powers of two), sum
+  float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum of q . k, sum
   float* acc = nullptr;          // [2 * ctas][tile_rows][hd]: unnormalised output
 };
 
@@ -69,13 +69,10 @@ CTTS_DEV float exp2_fast(float x) {
   return r;
 }
 
-// score s and maximum m (in powers of two) to the exponential's argument; a
-// float32 call takes the factor in two parts, or its rounding would cost
-// 2^-24 of the argument
-template <bool QF>
-CTTS_DEV float attn_arg(const PagedAttnArgs& a, float s, float m) {
-  return QF ? fmaf(s, a.c2_hi, fmaf(s, a.c2_lo, -m)) : fmaf(s, a.c2_hi, -m);
-}
+// Score s = q . k under a maximum m to the exponential's argument.  The
+// difference first: the roundings then cost a few 2^-24 of the argument, not
+// of the score, and the maximum's own weight is 1 however large the scores are.
+CTTS_DEV float attn_arg(float s, float m, float c2) { return (s - m) * c2; }
 
 // A request's lengths, cut to what the buffers hold.
 struct AttnReq {

@@ -93,6 +93,11 @@ def test_attention_refuses(over, code):
     assert call("ctts_op_paged_attention", pack("attention", **over))[0] == code
 
 
+@pytest.mark.parametrize("scale", [1e-21, 1e-45, 2e20, 3e38])
+def test_attention_refuses_a_scale_whose_factor_vanishes_or_overflows(scale):
+    assert call("ctts_op_paged_attention", pack("attention", scale=scale))[0] == _lib.ERR_ARG
+
+
 def test_nothing_to_do_is_no_error():
     assert call("ctts_op_paged_append", pack("append", rows=0))[0] == 0
     assert call("ctts_op_paged_attention", pack("attention", rows=0))[0] == 0

@@ -681,6 +681,72 @@ def test_bad_values_stay_with_their_request(q_t, kv_t, hd, new):
     assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], want[~bad])
 
 
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_bad_queries_of_short_requests(q_t, kv_t, hd, new):
+    """Many short requests, whose items no cut divides: a row whose query is NaN gives NaN, every other what it gave."""
+    c = Case([21] * 400, [new] * 400, 4, 2, hd, 16, q_t, kv_t, seed=15)
+    want = c.run()
+    rows = torch.arange(0, 400, 3, device="cuda") * new + new // 2
+    c.q[rows, 3, 5] = float("nan")
+    out = c.run()
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[rows, 3] = True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [1e-20, 1e20])
+def test_scales_at_their_bounds(q_t, kv_t, new, scale):
+    """The smallest scale: the mean of the values seen; the largest: the value of the best key."""
+    c = Case([37, 300, 2000], [new] * 3, 4, 2, 64, 16, q_t, kv_t, seed=16)
+    c.scale = scale
+    if scale > 1:  # scores 1 at one key, 0 at the others: weights of exactly 1 and 0
+        c.q.zero_()
+        c.q[..., 0] = 1.0
+        c.k[..., 0] = 0.0
+        for b in range(3):
+            c.k[int(c.tables[b, 0]), 11, :, 0] = 1.0
+    out = c.run().double()
+    for b, n in enumerate([37, 300, 2000]):
+        v = c.v[c.tables[b].long()].flatten(0, 1).double()[: n + new]  # [tokens, 2, 64]
+        for i in range(new):
+            want = v[11] if scale > 1 else v[: n + i + 1].mean(0)
+            # weights rounded to bf16 are exact here; the sum's float32 adds and one rounding to the output's type
+            tol = want.abs() * torch.finfo(q_t).eps / 2 + v[: n + i + 1].abs().mean(0) * (n + i + 1) * 2.0**-23
+            assert ((out[b * new + i].view(2, 2, 64) - want[:, None]).abs() <= tol[:, None]).all()
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_huge_scores(q_t, kv_t, hd, new, sign):
+    """Scores of 10^11 and more: the best key takes all, or those within rounding of it share."""
+    c = Case([37, 300, 2000] + [21] * 200, [new] * 203, 4, 2, hd, 16, q_t, kv_t, seed=17, spread=1e6)
+    c.q, c.k = c.q.abs(), sign * c.k.abs()
+    out = c.run().double().view(-1, 2, 2, hd)
+    single = 0
+    for b in (0, 1, 2, 50, 202):
+        L = c.ctx[b] + new
+        k, v = (x[c.tables[b].long()].flatten(0, 1)[:L].double() for x in (c.k, c.v))
+        for i in range(new):
+            s = torch.einsum("hgd,khd->hgk", c.q[b * new + i].view(2, 2, hd).double(), k[: L - new + i + 1])
+            # sums of hd terms of one sign, each rounded or cut to 2^-23; the operands' 2^-24 (3 terms)
+            close = s >= s.amax(-1, keepdim=True) - s.abs().amax(-1, keepdim=True) * (2 * hd + 4) * 2.0**-23
+            got = out[b * new + i]
+            for h in range(2):
+                for g in range(2):
+                    of = v[: L - new + i + 1][close[h, g], h]
+                    lo, hi = of.amin(0), of.amax(0)
+                    tol = torch.maximum(lo.abs(), hi.abs()) * (2.0**-8 if q_t is BF16 else 2.0**-20)
+                    assert ((got[h, g] >= lo - tol) & (got[h, g] <= hi + tol)).all()
+                    single += of.shape[0] == 1
+    assert single > 0.7 * 5 * new * 4
+
+
 def test_another_stream_owns_what_it_uses():
     """Calls given a stream: outputs and workspaces come from that stream's memory, so work on the current one cannot reuse them."""
     c = Case([900, 4000, 40], [1, 1, 1], 4, 2, 64, 16, BF16, BF16)
