@@ -2,7 +2,8 @@
 
 The compute lives in libcutetts_b200.so (hand-written CUDA behind the C ABI
 of include/cutetts_b200.h); this package is the host-side mirror of the
-reference crate's model API (see rcutetts_b200.model).
+reference crate's model API (see rcutetts_b200.model) and of the paged KV-cache
+operators (rcutetts_b200.paged).
 """
 from .config import DiTConfig, FrameConfig, LMConfig, VAEConfig  # noqa: F401
 
@@ -12,7 +13,9 @@ _MODEL_NAMES = {
     "load_decoder_weights", "decode",
 }
 
-__all__ = ["LMConfig", "DiTConfig", "VAEConfig", "FrameConfig"] + sorted(_MODEL_NAMES)
+_PAGED_NAMES = {"PagedStep", "paged_plan", "paged_append", "paged_attention", "paged_attention_workspace"}
+
+__all__ = ["LMConfig", "DiTConfig", "VAEConfig", "FrameConfig"] + sorted(_MODEL_NAMES | _PAGED_NAMES)
 
 
 def __getattr__(name):
@@ -22,4 +25,8 @@ def __getattr__(name):
         from . import model
 
         return getattr(model, name)
+    if name in _PAGED_NAMES:
+        from . import paged
+
+        return getattr(paged, name)
     raise AttributeError(name)

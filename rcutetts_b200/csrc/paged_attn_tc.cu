@@ -1,31 +1,47 @@
-// paged_attn_tc.cu -- attention of chunks of new rows over a bf16 paged cache
-// on the 5th-generation tensor cores (tcgen05).
+// paged_attn_tc.cu -- attention of chunks of new rows over a paged cache on
+// the 5th-generation tensor cores (tcgen05).
 //
-// An item is up to two sub-tiles of 128 packed rows (one row per TMEM lane)
+// An item is one or two sub-tiles of 128 packed rows (one row per TMEM lane)
 // of one request and KV head.  Per key tile and sub-tile:
 //   S = Q . K^T   both operands in shared memory (K-major, 128-byte swizzle),
 //   softmax       one thread per row: S read from TMEM, the weights written
-//                 back over it in bf16,
+//                 back in bf16 (bf16 calls: over S),
 //   O += P . V    P read from TMEM, V from shared memory as it lies in the
 //                 pages ([key][dim]: the MN-major form of the B operand).
-// Warps 0-3 and 4-7 run the softmax of the two sub-tiles, so one computes
-// exponentials while the tensor core multiplies for the other; warp 8 issues
-// the MMAs, warp 9 the TMA copies: one box per page and 64 dims (a 4D map over
-// the pool), K and V in rings of their own.  Missing pages are boxes
-// outside the map, which arrive as zeros.
+// Four warps run the softmax of a sub-tile, one warp issues the MMAs.  A bf16
+// cache comes in by one warp's TMA copies: a box per page and 64 dims (a 4D
+// map over the pool), K and V in rings of their own; missing pages are boxes
+// outside the map, which arrive as zeros.  A float32 cache comes in by two or
+// four warps' plain loads, which split it into its bf16 terms on the way.
 //
-// The output is rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time: weights up to 256 lose nothing in floating point,
-// and the pass over O in TMEM becomes rare.  S(j+1) of a sub-tile is issued
-// behind P.V(j), so O is at rest while its softmax threads hold S.
+// Two sub-tiles take turns: one computes exponentials while the tensor core
+// multiplies for the other, and P arrives in two halves, so that P.V begins
+// over the second half's exponentials.  One sub-tile (where shared memory or
+// registers hold no second) has two S instead: the scores of tile i + 1 are
+// computed over the softmax of tile i.
 //
-// P arrives in two halves, so P.V begins over the second half's exponentials.
+// bf16: the output is rescaled only when a row's maximum has grown by more
+// than 2^8 since the last time: weights up to 256 lose nothing in floating
+// point, and the pass over O in TMEM becomes rare.  The scores stay in
+// registers between the maximum and the exponentials.
 //
 // float32 queries: queries and weights enter as three bf16 terms (24 bits),
-// key tiles are 64 wide so that three terms of the weights fit beside S.  Each
-// P.V starts at zero and its threads add it to an output row in registers:
-// the tensor core cuts the sums it accumulates instead of rounding them, which
-// over a thousand keys costs 2^-18 of the output (measured against 64 bits).
+// and so do keys and values of a float32 cache; of the products those below
+// 2^-24 of the whole are left out, which leaves three or six.  Key tiles are
+// 64 wide so that three terms of the weights fit beside S.  Each P.V starts
+// at zero and its threads add it to an output row in registers: the tensor
+// core cuts the sums it accumulates instead of rounding them, which over a
+// thousand keys costs 2^-18 of the output (measured against 64 bits).
+//
+// What bounds it.  bf16, 128 dims: a 256 x 128 tile costs 2048 clocks of
+// tensor time and 2900 in the steady state, the rest is the chain scores ->
+// softmax -> weights of two sub-tiles that cannot cover one another whole
+// (tensor pipe 62 %, special functions 60 % busy); 4 chunks of 1500 to 2048
+// rows over 4000 to 6100 tokens, 16 heads over 8 KV heads: 335 to 350 us, 910
+// to 960 TFLOP/s.  float32: three or six products a tile and as many splits;
+// 8 prompts of 190 to 900 rows, 12 heads of 64 over 4, bf16 cache: 38 to 47 us;
+// 2 chunks of 700 to 1500 over float32: 61 to 64 us.  Short calls: some 5 us from the
+// launch to the first scores and as much for each further item, and the join.
 //
 // Every wait is bounded; one that gives up raises a flag that ends all roles.
 #include <algorithm>

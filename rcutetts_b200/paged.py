@@ -9,10 +9,10 @@ One serving step over a paged cache is a run of three calls:
 (the contracts are those of ctts_op_paged_plan / _append / _attention in
 include/cutetts_b200.h).  The pools k_pages and v_pages are [pages, page_size,
 kv heads, head dim] tensors of float32 or bf16 with any order in memory; one
-pair per layer.  Calls run on the tensors' device, on its current stream
-unless `stream` is given, and can be captured in a CUDA graph.  Arguments of a
-wrong type, shape or device raise ValueError, what the library refuses
-CttsError.
+pair per layer.  For inference: no gradients flow through the calls.  They run
+on the tensors' device, on its current stream unless `stream` is given, and
+can be captured in a CUDA graph.  Arguments of a wrong type, shape or device
+raise ValueError, what the library refuses CttsError.
 """
 from __future__ import annotations
 
