@@ -63,6 +63,8 @@ struct Shape {
   static constexpr int ES = KF ? 4 : 2;
   static constexpr int C = !KF && HD == 64 ? 128 : 64;  // keys per tile: 16 KB of K (float32 of 128 dims: 32), and as much of V
   static constexpr int NB = HD * ES / 128;              // 128-byte blocks of a row
+  // (without the cost of items the CTAs that draw many short ones end last)
+  using Item = AttnItem<R, C, 1, 1, 2>;
   static constexpr uint32_t TILE = NB * C * 128;        // a K or V tile: [block][key][128 B], 16-byte chunks swizzled by key
   static constexpr uint32_t STAGE = 2 * TILE;
   static constexpr int NS = STAGE <= 32768 ? 3 : 2;
@@ -80,6 +82,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
                                                                                        const __grid_constant__ PagedAttnArgs a, int box,
                                                                                        int order) {
   using S = Shape<QF, KF, HD, RH>;
+  using Cursor = AttnCursor<typename S::Item>;
   constexpr int R = S::R, C = S::C, KT = S::KT, NO = HD / 8, KS = HD / 16, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ AttnStart start;
@@ -101,10 +104,10 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
     gave_up = 0;
   }
   grid_dep_enter();
-  attn_find_start<R, C, kNT + 32>(a.line, &start);
+  attn_find_start<typename S::Item, kNT + 32>(a.line, &start);
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   int left;
-  AttnCursor cu = AttnCursor::at<R, C>(a.line, start, &left);
+  Cursor cu = Cursor::at(a.line, start, &left);
   if (left == 0) return;
 
   if (warp == 4) {
@@ -125,10 +128,10 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < C / 8 && kk < cu.len && none);
       const int mine = none ? a.p.kv.n_pages : page;
       if (++kt == end) {
-        left = AttnCursor::behind(left, end - cu.kt);
+        left = cu.behind(left, end - cu.kt);
         more = left > 0;
         if (more) {
-          cu = AttnCursor::next<R, C>(a.line, cu);
+          cu = Cursor::next(a.line, cu);
           kt = 0;
           end = cu.tiles(left);
         }
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
     float* const part = a.acc + (long)slot * a.tile_rows * HD;
     if (!ends && cu.kt == 0 && tid == 0) {
       AttnPart d;
-      d.pieces = attn_pieces(a.line, start, cu.nt - end);
+      d.pieces = attn_pieces<typename S::Item>(a.line, start, cu.nt - end - 1);
       d.row0 = cu.r0; d.packed0 = row_base; d.rows = nrows; d.h = cu.h;
       a.parts[blockIdx.x] = d;
     }
@@ -474,9 +477,9 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         *reinterpret_cast<float2*>(part + (long)r * HD + d) = make_float2(x, y);
       }
     }
-    left = AttnCursor::behind(left, end - cu.kt);
+    left = cu.behind(left, end - cu.kt);
     if (left == 0) break;
-    cu = AttnCursor::next<R, C>(a.line, cu);
+    cu = Cursor::next(a.line, cu);
   }
 }
 
@@ -597,7 +600,7 @@ auto with_shape(const ctts_paged_attn& p, int rows, F f) {
 // ones on the tcgen05 kernel (paged_attn_tc.cu) -- their short requests too: a
 // tile of 128 rows costs a short item as much as a long one, yet two launches
 // after one another took longer (43 decodes and 5 chunks of 200 to 512: 40 us
-// against 35).
+// against 35, and 31 since such items share a CTA's two sub-tiles).
 bool is_short(const ctts_paged_attn& p) { return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) <= 16; }
 int rows_used_of(const ctts_paged_attn& p) { return std::max(1, p.max_new * (p.n_heads / p.kv.n_kv_heads)); }
 

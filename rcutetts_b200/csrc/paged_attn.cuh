@@ -99,11 +99,16 @@ CTTS_DEV int attn_tiles(const AttnReq& r, int m, int group) {
   const int ahead = packed >= r.nn * group ? r.nn : (packed - 1) / group + 1;
   return max(1, (min(r.len, r.len - r.cnt + ahead) + C - 1) / C);
 }
-// To begin and to end an item (queries in, output out) costs about as much as
-// this many key tiles: so much of the line an item takes ahead of its tiles.
-// (Without it the CTAs that draw many short items end last: 43 decodes with 5
-// chunks of 200 to 512 took 39 us instead of 34.)
-constexpr int kItemCost = 2;
+// What an item is made of and what it costs on the line, in units: R packed
+// rows, tiles of C keys, W1 units a tile of an item of up to 128 packed rows,
+// W2 of one with more, and COST ahead of its tiles to begin and end it (queries
+// in, output out).  A CTA has the tiles that begin in its piece.
+template <int R_, int C_, int W1_, int W2_, int COST_>
+struct AttnItem {
+  static constexpr int R = R_, C = C_, W1 = W1_, W2 = W2_, COST = COST_;
+  static CTTS_DEV int weight(int packed) { return packed > 128 ? W2 : W1; }  // of a tile, from the packed rows left in the request
+  static CTTS_DEV int tiles_in(int units, int w) { return w == W1 ? (units + W1 - 1) / W1 : (units + W2 - 1) / W2; }  // that begin there
+};
 
 // The row tiles of a request in order: the rows ahead of each one's end by
 // running quotient and remainder, without a division a tile.
@@ -131,29 +136,29 @@ struct AttnRowWalk {
     }
   }
 };
-template <int R, int C>
+template <class T>
 CTTS_DEV long attn_units(const AttnLine& ln, const AttnReq& r) {
-  const int mt = attn_row_tiles<R>(r, ln.group);
-  AttnRowWalk<R, C> w(r, ln.group);
+  const int mt = attn_row_tiles<T::R>(r, ln.group);
+  AttnRowWalk<T::R, T::C> w(r, ln.group);
   long n = 0;
 #pragma unroll 1
-  for (int m = 0; m < mt; m++, w.next()) n += w.tiles() + kItemCost;
+  for (int m = 0; m < mt; m++, w.next()) n += (long)w.tiles() * T::weight(r.nn * ln.group - m * T::R) + T::COST;
   return n * ln.n_kv;
 }
-// The line is cut into `ctas` pieces of `base` tiles, the first `rest` of them
-// one longer; no more pieces than tiles, so that the pieces of a divided item
+// The line is cut into `ctas` pieces of `base` units, the first `rest` of them
+// one longer; none shorter than a tile, so that the pieces of a divided item
 // lie in neighbouring CTAs.
 struct AttnCut {
   int ctas;
   long base, rest;
-  CTTS_DEV AttnCut(int n, long total) {
-    ctas = total < n ? (int)total : n;
+  CTTS_DEV AttnCut(int n, long total, int tile) {
+    ctas = total < (long)n * tile ? (int)total / tile : n;
     if (ctas == 0) ctas = 1;
     base = total >> 32 ? total / ctas : (long)((unsigned)total / (unsigned)ctas);  // (a 64-bit division is ten times the latency)
     rest = total - base * ctas;
   }
   CTTS_DEV long begin(int c) const { return c < ctas ? c * base + min((long)c, rest) : base * ctas + rest; }
-  CTTS_DEV int owner(long unit) const {  // the CTA that has a tile
+  CTTS_DEV int owner(long unit) const {  // the CTA that has a unit
     const long longer = rest * (base + 1);
     return (int)(unit < longer ? unit / (base + 1) : rest + (unit - longer) / base);
   }
@@ -172,7 +177,7 @@ struct AttnStart {
 // registers when one turn holds the batch).  (Code that runs once a launch is
 // kept small throughout these kernels: what does not fit the instruction cache
 // beside the main loop costs more than a rolled loop.)
-template <int R, int C, int NT>
+template <class T, int NT>
 CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
   constexpr int W = NT / 32;
   __shared__ long wsum[2][W];
@@ -186,7 +191,7 @@ CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
     long u = 0;
     if (b < n) {
       rq = attn_req(ln, b);
-      u = attn_units<R, C>(ln, rq);
+      u = attn_units<T>(ln, rq);
     }
     long inc = u;
 #pragma unroll
@@ -208,7 +213,7 @@ CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
     if (pass == 0) {
       total += all;
       if (base < n) continue;
-      const AttnCut cut(ln.ctas, total);
+      const AttnCut cut(ln.ctas, total, max(T::W1, T::W2));
       u0 = cut.begin(blockIdx.x);
       u1 = cut.begin(blockIdx.x + 1);
       if (tid == 0) {
@@ -235,66 +240,77 @@ CTTS_DEV void attn_find_start(const AttnLine& ln, AttnStart* out) {
   __syncthreads();
 }
 
-// CTAs from this one to the one that holds tile `more` behind this CTA's end.
+// CTAs from this one to the one that has the unit `more` behind this CTA's end.
+template <class T>
 CTTS_DEV int attn_pieces(const AttnLine& ln, const AttnStart& s, int more) {
-  return AttnCut(ln.ctas, s.total).owner(s.end + more - 1) - (int)blockIdx.x + 1;
+  return AttnCut(ln.ctas, s.total, max(T::W1, T::W2)).owner(s.end + more) - (int)blockIdx.x + 1;
 }
 
 // A place on the line: request, row tile, KV head, key tile.  A role walks its
 // CTA's pieces: tiles kt .. of one item, then the next item's from 0.
+template <class T>
 struct AttnCursor {
   int b, m, h, kt, nt, mt;
+  int w;  // units a tile
   int r0, cnt, nn, len;
 
-  CTTS_DEV void set(const AttnLine& ln, int R, const AttnReq& r) {
+  CTTS_DEV void set(const AttnLine& ln, const AttnReq& r) {
     r0 = r.r0; cnt = r.cnt; nn = r.nn; len = r.len;
-    mt = (nn * ln.group + R - 1) / R;
+    mt = attn_row_tiles<T::R>(r, ln.group);
   }
-  template <int R, int C>
-  static __device__ __noinline__ AttnCursor at(AttnLine ln, AttnReq req, int b, long skip) {
+  // `skip` units into request b; kt: units behind the first tile's begin
+  static __device__ __noinline__ AttnCursor seek(AttnLine ln, AttnReq req, int b, long skip) {
     AttnCursor c;
     c.b = b;
-    c.set(ln, R, req);
-    AttnRowWalk<R, C> w(req, ln.group);
+    c.set(ln, req);
+    AttnRowWalk<T::R, T::C> walk(req, ln.group);
 #pragma unroll 1
-    for (c.m = 0;; c.m++, w.next()) {
-      c.nt = w.tiles();
-      const long in = (long)(c.nt + kItemCost) * ln.n_kv;
+    for (c.m = 0;; c.m++, walk.next()) {
+      c.nt = walk.tiles();
+      c.w = T::weight(req.nn * ln.group - c.m * T::R);
+      const long in = (long)(c.nt * c.w + T::COST) * ln.n_kv;
       if (skip < in || c.m + 1 >= c.mt) break;
       skip -= in;
     }
-    const unsigned item = c.nt + kItemCost;  // (skip is inside one row tile's heads: 31 bits)
+    const unsigned item = c.nt * c.w + T::COST;  // (skip is inside one row tile's heads: 31 bits)
     c.h = (unsigned)skip / item;
-    c.kt = (int)((unsigned)skip % item) - kItemCost;
+    c.kt = (int)((unsigned)skip % item) - T::COST;
     return c;
   }
-  // The CTA's first piece; left: what it has of the line (0: nothing to do).
-  template <int R, int C>
+  // The CTA's first piece; left: units from its first tile to the CTA's end
+  // (0: nothing to do).
   static CTTS_DEV AttnCursor at(const AttnLine& ln, const AttnStart& s, int* left) {
     *left = (int)s.units;  // (of one CTA: 31 bits, the host checks)
     AttnCursor c{};
     if (*left > 0) {
-      c = at<R, C>(ln, s.req, s.b, s.skip);
-      if (c.kt < 0) {
-        *left = max(0, *left + c.kt);
-        c.kt = 0;
+      c = seek(ln, s.req, s.b, s.skip);
+      if (T::W1 == 1 && T::W2 == 1) {
+        *left += min(c.kt, 0);
+        c.kt = max(c.kt, 0);
+      } else {
+        const int kt = c.kt > 0 ? T::tiles_in(c.kt, c.w) : 0;
+        *left -= kt * c.w - c.kt;
+        c.kt = kt;
+        if (kt == c.nt) {  // the last tile began ahead of the piece
+          *left -= T::COST;
+          if (*left > 0) c = next(ln, c);
+        }
       }
+      *left = max(*left, 0);
     }
     return c;
   }
   // Tiles of the piece.
-  CTTS_DEV int tiles(int left) const { return min(nt - kt, left); }
-  // What is left of the line behind a piece of n tiles and the cost of the
-  // item that follows (0: it was the last).
-  static CTTS_DEV int behind(int left, int n) { return max(0, left - n - kItemCost); }
+  CTTS_DEV int tiles(int left) const { return min(nt - kt, T::tiles_in(left, w)); }
+  // What is left of the CTA's units at the first tile of the next item, behind
+  // a piece of n tiles (0: there is none).
+  CTTS_DEV int behind(int left, int n) const { return max(0, left - n * w - T::COST); }
   // The next item, from its first tile (never called at the end of the line).
-  template <int R, int C>
   static CTTS_DEV AttnCursor next(const AttnLine& ln, AttnCursor c) {
     c.kt = 0;
     if (++c.h < ln.n_kv) return c;
-    return next_rows<R, C>(ln, c);
+    return next_rows(ln, c);
   }
-  template <int R, int C>
   static __device__ __noinline__ AttnCursor next_rows(AttnLine ln, AttnCursor c) {
     c.h = 0;
     if (++c.m == c.mt) {
@@ -302,10 +318,11 @@ struct AttnCursor {
 #pragma unroll 1
       do {
         c.b++;
-        c.set(ln, R, attn_req(ln, c.b));
+        c.set(ln, attn_req(ln, c.b));
       } while (c.mt == 0 && c.b + 1 < ln.batch);
     }
-    c.nt = attn_tiles<R, C>(AttnReq{c.r0, c.cnt, c.nn, c.len}, c.m, ln.group);
+    c.nt = attn_tiles<T::R, T::C>(AttnReq{c.r0, c.cnt, c.nn, c.len}, c.m, ln.group);
+    c.w = T::weight(c.nn * ln.group - c.m * T::R);
     return c;
   }
   // Packed rows of the item, and the position of the request's first new row.

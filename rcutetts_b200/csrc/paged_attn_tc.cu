@@ -18,7 +18,8 @@
 // multiplies for the other, and P arrives in two halves, so that P.V begins
 // over the second half's exponentials.  One sub-tile (where shared memory or
 // registers hold no second) has two S instead: the scores of tile i + 1 are
-// computed over the softmax of tile i.
+// computed over the softmax of tile i.  bf16 items with rows for one sub-tile
+// only (single tokens among chunks) give every other key tile to the second.
 //
 // bf16: the output is rescaled only when a row's maximum has grown by more
 // than 2^8 since the last time: weights up to 256 lose nothing in floating
@@ -40,8 +41,8 @@
 // rows over 4000 to 6100 tokens, 16 heads over 8 KV heads: 335 to 350 us, 910
 // to 960 TFLOP/s.  float32: three or six products a tile and as many splits;
 // 8 prompts of 190 to 900 rows, 12 heads of 64 over 4, bf16 cache: 38 to 47 us;
-// 2 chunks of 700 to 1500 over float32: 61 to 64 us.  Short calls: some 5 us from the
-// launch to the first scores and as much for each further item, and the join.
+// 2 chunks of 700 to 1500 over float32: 61 to 64 us.  Short calls: some 5 us from
+// the launch to the first scores, 2 to 3 for each further item, and the join.
 //
 // Every wait is bounded; one that gives up raises a flag that ends all roles.
 #include <algorithm>
@@ -77,6 +78,17 @@ struct TcShape {
   // One sub-tile: the scores of tile i + 1 are computed while tile i is in its
   // softmax, into the other of two S.  Two: they take turns instead.
   static constexpr bool PIPE = NSUB == 1;
+  // Two sub-tiles and an item with rows for one: they share its key tiles, the
+  // second takes every other one, and their states merge at the end (bf16: the
+  // output in TMEM is open to the other sub-tile's warps).  Such a tile then
+  // takes 0.9 us instead of 1.4 (64 dims), one of two sub-tiles 1.8.
+  static constexpr bool SHARE = NSUB == 2 && !QF;
+  // Costs on the line, from the clocks of CTAs by least squares over their
+  // tiles and pieces: what equal tiles left uneven.  43 single tokens with 5
+  // chunks of 200 to 512, 64 dims: 35.4 us at equal costs and no sharing, 30.9;
+  // 81 with 9: 59, 51; 40 chunks of 20 to 120, 128 dims: 189, 177.
+  using Item = std::conditional_t<!SHARE, AttnItem<R, KT, 1, 1, 2>,
+                                  std::conditional_t<HD == 64, AttnItem<R, KT, 2, 4, 5>, AttnItem<R, KT, 3, 4, 6>>>;
   // TMEM columns of sub-tile s: S at s * SREG (PIPE: two of KT columns), P over
   // it (bf16) or behind it (three terms of KT / 2), O at OREG + s * OSTEP
   static constexpr uint32_t SREG = QF ? 192 : 128, PCOL = PIPE ? 2 * KT : (QF ? KT : 0);
@@ -157,6 +169,9 @@ CTTS_DEV float2 add2(float2 x, float2 y) {
   return r;
 }
 
+// Warps w and w + 4 meet.
+CTTS_DEV void pair_sync(int w) { asm volatile("bar.sync %0, 64;" ::"r"(w + 1) : "memory"); }
+
 // Byte offsets of packed rows p, p + 4, p + 8, ... (row of q times its stride
 // plus head times width), one division for all of them.
 struct RowWalk {
@@ -190,6 +205,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
                                                                                     const __grid_constant__ CUtensorMap tmV,
                                                                                     const __grid_constant__ PagedAttnArgs a, int box, int order) {
   using S = TcShape<QF, KF, HD>;
+  using Cursor = AttnCursor<typename S::Item>;
   constexpr int KT = S::KT, R = S::R, NS = S::NS, NT = S::NT, NC = S::NC;
   constexpr int W_MMA = 4 * S::NSUB, W_TMA = W_MMA + 1;
   constexpr int KS = KT / 16, HALF = QF ? 0 : KS / 2;  // bf16 calls: P arrives in two halves
@@ -199,6 +215,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t dead_keys[8];  // 8-key groups of a tile whose page does not exist
   __shared__ volatile int gave_up;
+  __shared__ float2 shared_ml[S::SHARE ? 128 : 1];  // maximum and sum of the second sub-tile of a shared item
   const uint32_t sbase = (smem_u32(tc_smem) + 1023u) & ~1023u;
   const uint32_t qs = sbase, ks = qs + S::NSUB * NT * S::QTERM, vs = ks + NS * S::TILE;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -226,14 +243,14 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   grid_dep_enter();
-  attn_find_start<R, KT, S::THREADS>(a.line, &start);
+  attn_find_start<typename S::Item, S::THREADS>(a.line, &start);
   if (tid == 0) a.parts[blockIdx.x].pieces = 0;  // no divided item yet
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   int left;
-  AttnCursor cu = AttnCursor::at<R, KT>(a.line, start, &left);
+  Cursor cu = Cursor::at(a.line, start, &left);
 
   if (!KF && left > 0 && warp == W_TMA) {
     // ---- producer: lane i looks up the page of keys 8i..8i+7 of a tile, the
@@ -252,10 +269,10 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < KT / 8 && kk < cu.len && none);
       const int from = none ? a.p.kv.n_pages : page;  // outside the map: zeros
       if (++kt == end) {
-        left = AttnCursor::behind(left, end - cu.kt);
+        left = cu.behind(left, end - cu.kt);
         more = left > 0;
         if (more) {
-          cu = AttnCursor::next<R, KT>(a.line, cu);
+          cu = Cursor::next(a.line, cu);
           kt = 0;
           end = cu.tiles(left);
         }
@@ -327,10 +344,10 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           fetch(job + 1, buf[(job + 1) & 1]);
         } else {
           if (++kt == end) {
-            left = AttnCursor::behind(left, end - cu.kt);
+            left = cu.behind(left, end - cu.kt);
             more = left > 0;
             if (more) {
-              cu = AttnCursor::next<R, KT>(a.line, cu);
+              cu = Cursor::next(a.line, cu);
               kt = 0;
               end = cu.tiles(left);
             }
@@ -462,6 +479,40 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
             }
           }
         }
+      } else if (S::SHARE && nsub == 1) {
+        // a turn: scores of tile i, then P.V of tile i - 1 for the other sub-tile
+#pragma unroll 1
+        for (int i = 0; i <= n; i++) {
+          if (i < n) {
+            const int s = i & 1;
+            if (i < 2) {
+              mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
+              q_par ^= 1u << s;
+            }
+            mbar_wait_or(&bars.k_full[st], par, &gave_up);
+            scores(s, st, S::SREG * s, &bars.s_full[s]);
+            commit(&bars.k_empty[st]);
+          }
+          if (i > 0) {
+            const int s = (i - 1) & 1;
+            mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+            mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
+            values(s, sp, 0, HALF, i > 2);
+            mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
+            p_par ^= 1u << s;
+            values(s, sp, HALF, KS, 1u);
+            if (i + 1 >= n) commit(&bars.o_full[s]);  // its last tile
+            commit(&bars.v_empty[sp]);
+          }
+          if (i < n) {
+            sp = st;
+            par_p = par;
+            if (++st == NS) {
+              st = 0;
+              par ^= 1;
+            }
+          }
+        }
       } else {
         // a turn: P.V of tile i - 1, scores of tile i
 #pragma unroll 1
@@ -500,9 +551,9 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           }
         }
       }
-      left = __shfl_sync(0xffffffffu, AttnCursor::behind(left, n), 0);
+      left = __shfl_sync(0xffffffffu, cu.behind(left, n), 0);
       if (left == 0) break;
-      cu = AttnCursor::next<R, KT>(a.line, cu);
+      cu = Cursor::next(a.line, cu);
     }
     if (gave_up) {  // MMAs in flight end before TMEM is given back
       commit(&bars.drain);
@@ -531,13 +582,17 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
     // A turn: the queries of the next piece go to shared memory (and its first
     // scores may begin), then the piece before is written out, then the next
     // one's tiles run.
-    AttnCursor nx = cu;
+    Cursor nx = cu;
     int u = 0, end = -1;  // tiles of the pieces before; of the current piece (-1: none yet)
+    int over = 0;         // units by which its last tile reaches past the CTA's end
+    auto shares = [&](const Cursor& c) { return S::SHARE && c.rows(a.line, R) <= 128; };
+    // the sub-tile takes part in a piece of n tiles
+    auto takes_part = [&](const Cursor& c, int n) { return s * 128 < c.rows(a.line, R) || (S::SHARE && n > 1); };
     float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
     while (true) {
-      if (left > 0 && s * 128 < nx.rows(a.line, R)) {
-        const int r0 = s * 128 + (warp & 3) * 32, nrows = nx.rows(a.line, R);  // the warp's first row in the item
+      if (left > 0 && takes_part(nx, nx.tiles(left))) {
+        const int r0 = (shares(nx) ? 0 : s * 128) + (warp & 3) * 32, nrows = nx.rows(a.line, R);  // the warp's first row in the item
         // the warp's 32 queries as bf16 terms: eight lanes read 128 bytes of a
         // row (as bf16), four rows at a time, all loads in flight before the
         // first is used; rows behind the item are zero
@@ -588,32 +643,53 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
         fence_async();
         mbar_arrive(&bars.q_full[s]);
       }
-      if (end >= 0 && s * 128 < cu.rows(a.line, R)) {
-        const int nrows = cu.rows(a.line, R);
-        const bool mine = s * 128 + row < nrows, warp_on = s * 128 + (warp & 3) * 32 < nrows;
+      if (end >= 0 && takes_part(cu, end - cu.kt)) {
+        const int nrows = cu.rows(a.line, R), first_row = shares(cu) ? 0 : s * 128;
+        const bool mine = first_row + row < nrows, warp_on = first_row + (warp & 3) * 32 < nrows;
+        const bool shared = shares(cu) && end - cu.kt > 1;
         // ---- the piece's output, or its partial state
         const bool ends = end == cu.nt, whole = ends && cu.kt == 0;
         const int place = 2 * blockIdx.x + (cu.kt == 0 ? 1 : 0);
         if (!ends && cu.kt == 0 && s == 0 && row == 0) {
           AttnPart d;
-          d.pieces = attn_pieces(a.line, start, cu.nt - end);
+          d.pieces = attn_pieces<typename S::Item>(a.line, start, over + (cu.nt - end - 1) * cu.w);
           d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
           a.parts[blockIdx.x] = d;
         }
         mbar_wait_or(&bars.o_full[s], o_par, &gave_up);
         o_par ^= 1;
-        if (warp_on) {
+        if (shared && s == 1) {
+          // the other sub-tile's warp of the same rows (and TMEM lanes) merges
+          // the states and writes them; O stays until it has
+          if (warp_on) {
+            shared_ml[row] = make_float2(m, l);
+            fence_before();
+            pair_sync(warp & 3);
+            pair_sync(warp & 3);
+            fence_after();
+          }
+        } else if (warp_on) {
+          float f0 = 1.0f, f1 = 0.0f;
+          if (shared) {
+            pair_sync(warp & 3);
+            const float2 other = shared_ml[row];
+            const float mm = fmaxf(m, other.x), mz = mm == -INFINITY ? 0.0f : mm;
+            f0 = exp2_fast(attn_arg(m, mz, c2));
+            f1 = exp2_fast(attn_arg(other.x, mz, c2));
+            m = mm;
+            l = fmaf(other.y, f1, l * f0);
+          }
           fence_after();
           const bool none = l == 0.0f;  // the row saw no key (one that saw any has a weight of 1, or NaN)
           const float inv = whole && !none ? 1.0f / l : 1.0f;
-          if (!whole && mine) a.ml[(long)place * a.tile_rows + s * 128 + row] = make_float2(m, l);
+          if (!whole && mine) a.ml[(long)place * a.tile_rows + first_row + row] = make_float2(m, l);
           if (QF) gather();
           // 32 columns of the warp's 32 rows by way of shared memory: a lane
           // holds a row, eight lanes write 128 bytes of one (four lanes 64
           // bytes in bf16)
           const uint32_t stage = vs + NS * S::TILE + warp * 4096;
           const bool half = whole && !QF;
-          const int r0 = s * 128 + (warp & 3) * 32, left = nrows - r0 - (lane >> 3), es = half ? 2 : 4;
+          const int r0 = first_row + (warp & 3) * 32, left = nrows - r0 - (lane >> 3), es = half ? 2 : 4;
           RowWalk w0(cu.m * R + r0 + (lane >> 3), a.group, a.p.out_ld * es, HD * es);
           uint8_t* dst = static_cast<uint8_t*>(a.p.out) + ((long)cu.r0 * a.p.out_ld + cu.h * a.group * HD) * es;
           if (!whole) {  // rows of the partial state follow one another
@@ -675,12 +751,23 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
             for (int c = 0; c < HD; c += 32) {
               uint32_t o[32];
               tmem_ld32_nowait(tO + c, o);
-              tmem_wait();
-              pin32(o);
+              if (shared) {
+                uint32_t o1[32];
+                tmem_ld32_nowait(tO + S::OSTEP + c, o1);
+                tmem_wait();
+                pin32(o);
+                pin32(o1);
+#pragma unroll
+                for (int j = 0; j < 32; j++) o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), f1, __uint_as_float(o[j]) * f0));
+              } else {
+                tmem_wait();
+                pin32(o);
+              }
               put(c, o);
             }
           }
           fence_before();
+          if (shared) pair_sync(warp & 3);
         }
       }
       if (left == 0) break;
@@ -689,21 +776,29 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
       cu = nx;
       end = cu.kt + cu.tiles(left);
       const int nrows = cu.rows(a.line, R);
-      if (s * 128 < nrows) {  // the sub-tile has rows
-        const bool warp_on = s * 128 + (warp & 3) * 32 < nrows;
-        const int pk = cu.m * R + s * 128 + row;
+      if (takes_part(cu, end - cu.kt)) {
+        const int first_row = shares(cu) ? 0 : s * 128;
+        const int first = cu.kt + (shares(cu) ? s : 0), step = shares(cu) ? 2 : 1;  // its tiles
+        const bool warp_on = first_row + (warp & 3) * 32 < nrows;
+        const int pk = cu.m * R + first_row + row;
         const int pos = cu.pos0() + pk / a.group, pos_lo = cu.pos0() + (pk - lane) / a.group;
         m = -INFINITY;
         l = 0.0f;
 #pragma unroll
         for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] = 0.0f;
 #pragma unroll 1
-        for (int kt = cu.kt; kt < end; kt++) {
+        for (int kt = first; kt < end; kt += step) {
           const int key0 = kt * KT;
-          if (!KF && s == 0 && key0 + KT > cu.len) {
+          const int sb = S::PIPE ? (kt - cu.kt) & 1 : s;
+          const uint32_t tS = tS0 + (S::PIPE ? sb * KT : 0);
+          mbar_wait_or(&bars.s_full[sb], (s_par >> sb) & 1, &gave_up);
+          s_par ^= 1u << sb;
+          if (!KF && (s == 0 || step == 2) && key0 + KT > cu.len) {
             // slots behind the length may hold anything, and 0 * NaN is NaN:
-            // their values become zeros (both sub-tiles' products come after
-            // this sub-tile's arrival at p_half or p_full)
+            // their values become zeros (the products come after this
+            // sub-tile's arrival at p_half or p_full, both sub-tiles' ones).
+            // Behind the scores, as a barrier's parity tells the fill of this
+            // tile from the one before last only once that one is over.
             const int w = u + kt - cu.kt, st = w % NS;
             mbar_wait_or(&bars.v_full[st], (uint32_t)(w / NS) & 1, &gave_up);
             if (row < KT && key0 + row >= cu.len) {
@@ -714,10 +809,6 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
             }
             fence_async();
           }
-          const int sb = S::PIPE ? (kt - cu.kt) & 1 : s;
-          const uint32_t tS = tS0 + (S::PIPE ? sb * KT : 0);
-          mbar_wait_or(&bars.s_full[sb], (s_par >> sb) & 1, &gave_up);
-          s_par ^= 1u << sb;
           if (warp_on) {
             fence_after();
             const uint32_t dead = dead_keys[(u + kt - cu.kt) & 7];
@@ -769,7 +860,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
               l *= f;
 #pragma unroll
               for (int c = 0; c < (QF ? HD : 1); c++) o_row[c] *= f;
-            } else if (kt == cu.kt) {
+            } else if (kt == first) {
               m = mn;  // O is overwritten by the first product
             } else {
               const bool grow = (mn - m) * c2 > 8.0f;
@@ -863,8 +954,9 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           mbar_arrive(&bars.p_full[s]);
         }
       }
-      left = AttnCursor::behind(left, end - cu.kt);
-      if (left > 0) nx = AttnCursor::next<R, KT>(a.line, cu);
+      over = (end - cu.kt) * cu.w - left;
+      left = cu.behind(left, end - cu.kt);
+      if (left > 0) nx = Cursor::next(a.line, cu);
     }
   }
   fence_before();

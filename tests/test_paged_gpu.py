@@ -325,6 +325,32 @@ def test_chunks(q_t, kv_t, heads, kv, hd):
 
 
 @pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("copies", [1, 9, 40])
+def test_short_items_beside_long_ones(q_t, kv_t, hd, copies):
+    """Items of few rows over one to many key tiles beside items of 256 packed rows, divided and whole, pages missing in some."""
+    ctx = [0, 3, 120, 127, 128, 250, 256, 511, 800, 0, 90, 1700] * copies
+    new = [6, 1, 8, 1, 64, 65, 20, 1, 63, 140, 128, 2] * copies
+    c = Case(ctx, new, 4, 2, hd, 16, q_t, kv_t, seed=18 + copies)
+    dead = [(b, col) for b, col in ((2, 7), (5, 0), (7, 8), (8, 3), (11, 40))]
+    for b, col in dead:
+        c.tables[b, col] = -1
+    c.ctx, c.new = ctx[:12] + ctx[-12:], new[:12] + new[-12:]
+    out = c.run(max_new=140)
+    if copies > 1:  # the first and the last twelve requests
+        at = int(c.cu[-13])
+        head, n = int(c.cu[12]), int(c.cu[12])
+        out = torch.cat([out[:head], out[at:]])
+        c.cu = torch.cat([c.cu[:12], c.cu[-13:] - at + n])
+        c.tables, c.lens = torch.cat([c.tables[:12], c.tables[-12:]]), torch.cat([c.lens[:12], c.lens[-12:]])
+        q = torch.cat([c.q[:head], c.q[at: at + head]])
+        c.q = q
+    else:
+        c.ctx, c.new = ctx, new
+    c.check(out, dead)
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
 @pytest.mark.parametrize("p", [8, 16, 32, 64, 128, 256])
 @pytest.mark.parametrize("layout", ["nhd", "hnd"])
 def test_page_sizes_and_layouts(q_t, kv_t, p, layout):
