@@ -484,16 +484,17 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
 }
 
 // Merges the pieces of the items that cuts divide: the blocks (c, *) take the
-// item that leaves CTA c, if there is one.  HD/4 lanes hold a row (four
-// columns each).  Few pieces (chunks; the usual case): each group of lanes
-// takes a row of its own and walks its pieces.  Many (one long request): the
-// block takes a row at a time, its groups share the pieces, and their states
-// merge in shared memory in group order.
+// item that leaves CTA c, if there is one.  HD/8 lanes hold a row (eight
+// columns each: four need twice the blocks, which then run in two waves).  Few
+// pieces (chunks; the usual case): each group of lanes takes a row of its own
+// and walks its pieces.  Many (one long request): the block takes a row at a
+// time, its groups share the pieces, and their states merge in shared memory
+// in group order.
 constexpr int kJoinThreads = 256;
 template <bool BF, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ PagedAttnArgs a) {
-  constexpr int COLS = HD / 4, G = kJoinThreads / COLS, FEW = 8;
-  __shared__ float4 gv[G][COLS];
+  constexpr int COLS = HD / 8, G = kJoinThreads / COLS, FEW = 8;
+  __shared__ float4 gv[G][2 * COLS];
   __shared__ float2 gml[G];
   const int tid = threadIdx.x, c = blockIdx.x, col = tid % COLS, grp = tid / COLS;
   grid_dep_enter();
@@ -505,56 +506,68 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
   for (int base = blockIdx.y * rows_at_once; base < d.rows; base += gridDim.y * rows_at_once) {
     const int r = base + (shared_row ? 0 : grp);
     const bool on = r < d.rows;
-    float m = -INFINITY, l = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.0f, v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.0f;
+    // the state (m2, l2, x, y) joins (m, l, v)
+    auto add = [&](float m2, float l2, const float4& x, const float4& y) {
+      const float mn = fmaxf(m, m2), mz = mn == -INFINITY ? 0.0f : mn;
+      const float f = exp2_fast(attn_arg(m, mz, a.c2)), g = exp2_fast(attn_arg(m2, mz, a.c2));
+      m = mn;
+      l = fmaf(l2, g, l * f);
+      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = fmaf(w[e], g, v[e] * f);
+    };
     if (on) {
 #pragma unroll 4
       for (int i = i0; i < d.pieces; i += di) {
         const long at = (long)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * a.tile_rows + r;
         const float2 ml = a.ml[at];
-        const float4 w = *reinterpret_cast<const float4*>(a.acc + at * HD + 4 * col);
-        const float mn = fmaxf(m, ml.x), mz = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2_fast(attn_arg(m, mz, a.c2)), g = exp2_fast(attn_arg(ml.x, mz, a.c2));
-        m = mn;
-        l = fmaf(ml.y, g, l * f);
-        v.x = fmaf(w.x, g, v.x * f);
-        v.y = fmaf(w.y, g, v.y * f);
-        v.z = fmaf(w.z, g, v.z * f);
-        v.w = fmaf(w.w, g, v.w * f);
+        const float4* w = reinterpret_cast<const float4*>(a.acc + at * HD + 8 * col);
+        add(ml.x, ml.y, w[0], w[1]);
       }
     }
     if (shared_row) {
-      gv[grp][col] = v;
+      gv[grp][2 * col] = make_float4(v[0], v[1], v[2], v[3]);
+      gv[grp][2 * col + 1] = make_float4(v[4], v[5], v[6], v[7]);
       if (col == 0) gml[grp] = make_float2(m, l);
       __syncthreads();
-      if (grp == 0) {
-        float M = -INFINITY;
+      if (tid < HD) {  // a column a thread
+        float M = -INFINITY, x = 0.0f;
 #pragma unroll
         for (int k = 0; k < G; k++) M = fmaxf(M, gml[k].x);
         if (M == -INFINITY) M = 0.0f;
         l = 0.0f;
-        v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < G; k++) {
           const float g = exp2_fast(attn_arg(gml[k].x, M, a.c2));
-          const float4 w = gv[k][col];
           l = fmaf(gml[k].y, g, l);
-          v.x = fmaf(w.x, g, v.x);
-          v.y = fmaf(w.y, g, v.y);
-          v.z = fmaf(w.z, g, v.z);
-          v.w = fmaf(w.w, g, v.w);
+          x = fmaf(reinterpret_cast<const float*>(gv[k])[tid], g, x);
         }
+        const int pk = d.packed0 + r;
+        const long at = (long)(d.row0 + pk / a.group) * a.p.out_ld + (long)(d.h * a.group + pk % a.group) * HD + tid;
+        x *= l == 0.0f ? 0.0f : 1.0f / l;
+        if (BF)
+          static_cast<uint16_t*>(a.p.out)[at] = (uint16_t)pack_bf2(x, 0.0f);
+        else
+          static_cast<float*>(a.p.out)[at] = x;
       }
       __syncthreads();
-    }
-    if (on && (!shared_row || grp == 0)) {
+    } else if (on) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int pk = d.packed0 + r;
-      const long at = (long)(d.row0 + pk / a.group) * a.p.out_ld + (long)(d.h * a.group + pk % a.group) * HD + 4 * col;
-      if (BF)
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.p.out) + at) = make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
-      else
-        *reinterpret_cast<float4*>(static_cast<float*>(a.p.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      const long at = (long)(d.row0 + pk / a.group) * a.p.out_ld + (long)(d.h * a.group + pk % a.group) * HD + 8 * col;
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] *= inv;
+      if (BF) {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.p.out) + at) =
+            make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+      } else {
+        float4* out = reinterpret_cast<float4*>(static_cast<float*>(a.p.out) + at);
+        out[0] = make_float4(v[0], v[1], v[2], v[3]);
+        out[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
     }
   }
 }
@@ -678,7 +691,7 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   } else {
     CTTS_LK(launch_paged_attn_tc(a, s));
   }
-  const dim3 grid(pl.ctas, is_short(p) ? std::min(a.rows_used, 4) : 16), block(kJoinThreads);
+  const dim3 grid(pl.ctas, is_short(p) ? std::min(a.rows_used, 4) : p.kv.head_dim / 8), block(kJoinThreads);
   const bool bf = p.q_dtype == CTTS_BF16;
   if (p.kv.head_dim == 64)
     return bf ? launch_k(paged_attn_join_kernel<true, 64>, grid, block, 0, s, a) : launch_k(paged_attn_join_kernel<false, 64>, grid, block, 0, s, a);
