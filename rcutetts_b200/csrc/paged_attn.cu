@@ -613,7 +613,7 @@ auto with_shape(const ctts_paged_attn& p, int rows, F f) {
 // ones on the tcgen05 kernel (paged_attn_tc.cu) -- their short requests too: a
 // tile of 128 rows costs a short item as much as a long one, yet two launches
 // after one another took longer (43 decodes and 5 chunks of 200 to 512: 40 us
-// against 35, and 31 since such items share a CTA's two sub-tiles).
+// against 35, and 30 since such items share a CTA's two sub-tiles).
 bool is_short(const ctts_paged_attn& p) { return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) <= 16; }
 int rows_used_of(const ctts_paged_attn& p) { return std::max(1, p.max_new * (p.n_heads / p.kv.n_kv_heads)); }
 

@@ -40,8 +40,9 @@
 // (tensor pipe 62 %, special functions 60 % busy); 4 chunks of 1500 to 2048
 // rows over 4000 to 6100 tokens, 16 heads over 8 KV heads: 335 to 350 us, 910
 // to 960 TFLOP/s.  float32: three or six products a tile and as many splits;
-// 8 prompts of 190 to 900 rows, 12 heads of 64 over 4, bf16 cache: 38 to 47 us;
-// 2 chunks of 700 to 1500 over float32: 61 to 64 us.  Short calls: some 5 us from
+// 8 prompts of 190 to 900 rows, 12 heads of 64 over 4, bf16 cache: 36 us;
+// 2 chunks of 700 to 1500 over float32: 59 us (both to a fifth more at the
+// clocks that follow long calls).  Short calls: some 5 us from
 // the launch to the first scores, 2 to 3 for each further item, and the join.
 //
 // Every wait is bounded; one that gives up raises a flag that ends all roles.
