@@ -54,6 +54,9 @@ int check_attn(const ctts_paged_attn* p) {
   CTTS_REQ(p->batch > 0 && p->rows >= 0 && p->max_new >= 0 && p->max_pages > 0, CTTS_ERR_ARG, "bad size");
   CTTS_REQ((int64_t)p->max_pages * p->kv.page_size <= 0x7fffffff, CTTS_ERR_RANGE, "max_pages * page_size must fit 31 bits");
   CTTS_REQ((int64_t)p->rows * (p->n_heads / p->kv.n_kv_heads) <= 0x7fffffff, CTTS_ERR_RANGE, "too many rows");
+  // what the heads of one row tile take of the line is divided in 32 bits (units of a tile: up to 5)
+  CTTS_REQ(5 * ((int64_t)p->max_pages * p->kv.page_size / 64 + 3) * p->kv.n_kv_heads <= 0xffffffff, CTTS_ERR_RANGE,
+           "too many keys and KV heads");
   return CTTS_OK;
 }
 
@@ -129,9 +132,9 @@ extern "C" int ctts_op_paged_attention(const ctts_paged_attn* p, void* stream) {
   const PagedAttnPlan pl = paged_attn_plan(*p);
   CTTS_REQ(pl.ctas > 0, CTTS_ERR_CUDA, "no CUDA device");
   CTTS_REQ(p->workspace_bytes >= pl.ws_bytes, CTTS_ERR_ARG, "workspace too small: " + std::to_string(pl.ws_bytes) + " bytes wanted");
-  // the units of one CTA are counted in 31 bits (a tile is up to 4; a long item has 128 packed rows or more)
+  // the units of one CTA are counted in 31 bits (a tile is up to 5; a long item has 128 packed rows or more)
   const double group = p->n_heads / p->kv.n_kv_heads, tiles = (double)p->max_pages * p->kv.page_size / 64 + 3;
-  CTTS_REQ(4 * tiles * p->kv.n_kv_heads * p->batch * (std::min(p->max_new, p->rows) * group / 128 + 1) <
+  CTTS_REQ(5 * tiles * p->kv.n_kv_heads * p->batch * (std::min(p->max_new, p->rows) * group / 128 + 1) <
                2147483647.0 * pl.ctas,
            CTTS_ERR_RANGE, "too many key tiles");
   CTTS_CK(launch_paged_attn(*p, as_stream(stream, 0)));

@@ -86,13 +86,14 @@ struct TcShape {
   static constexpr bool SHARE = NSUB == 2 && !QF;
   // Costs on the line, from the clocks of CTAs by least squares over their
   // tiles and pieces: what equal tiles left uneven.  43 single tokens with 5
-  // chunks of 200 to 512, 64 dims: 35.4 us at equal costs and no sharing, 30.9;
-  // 81 with 9: 59, 51; 40 chunks of 20 to 120, 128 dims: 189, 177.
+  // chunks of 200 to 512, 64 dims: 35.4 us at equal costs and no sharing, 30;
+  // 81 with 9: 59, 48; 40 chunks of 20 to 120, 128 dims: 189, 177; 43 with 5
+  // there: 101, 79 (costs of 3, 4, 6: 88).
   // float32 queries: with single tokens as above 75 us at equal costs, 69.  (One
   // sub-tile: costs of 1, 3 and 4 tiles an item were no better than 2 in all.)
   using Item = std::conditional_t<
       NSUB == 1, AttnItem<R, KT, 1, 1, 2>,
-      std::conditional_t<QF, AttnItem<R, KT, 3, 4, 4>, std::conditional_t<HD == 64, AttnItem<R, KT, 2, 4, 5>, AttnItem<R, KT, 3, 4, 6>>>>;
+      std::conditional_t<QF, AttnItem<R, KT, 3, 4, 4>, std::conditional_t<HD == 64, AttnItem<R, KT, 2, 4, 5>, AttnItem<R, KT, 3, 5, 8>>>>;
   // TMEM columns of sub-tile s: S at s * SREG (PIPE: two of KT columns), P over
   // it (bf16) or behind it (three terms of KT / 2), O at OREG + s * OSTEP
   static constexpr uint32_t SREG = QF ? 192 : 128, PCOL = PIPE ? 2 * KT : (QF ? KT : 0);

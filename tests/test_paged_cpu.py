@@ -98,6 +98,13 @@ def test_attention_refuses_a_scale_whose_factor_vanishes_or_overflows(scale):
     assert call("ctts_op_paged_attention", pack("attention", scale=scale))[0] == _lib.ERR_ARG
 
 
+def test_attention_refuses_keys_and_heads_past_32_bits():
+    over = dict(pages=1 << 26, tld=1 << 26, h=64, heads=64, qld=64 * 64, old=64 * 64)
+    assert call("ctts_op_paged_attention", pack("attention", **over))[0] == _lib.ERR_RANGE
+    over.update(rows=0, h=32, heads=32, qld=32 * 64, old=32 * 64)  # half as many fit
+    assert call("ctts_op_paged_attention", pack("attention", **over))[0] == 0
+
+
 def test_nothing_to_do_is_no_error():
     assert call("ctts_op_paged_append", pack("append", rows=0))[0] == 0
     assert call("ctts_op_paged_attention", pack("attention", rows=0))[0] == 0
