@@ -797,3 +797,47 @@ def test_another_stream_owns_what_it_uses():
         assert step.state.tolist() == [2, 3, 2, 1]
     with pytest.raises((TypeError, AttributeError)):
         c.run(stream="no stream")
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_two_calls_at_once(q_t, kv_t, hd):
+    """Chunks and single tokens on two streams at once, and two calls of each kind: every one gives what it gives alone."""
+    cases = [Case([900, 0, 300], [200, 70, 1], 4, 2, hd, 16, q_t, kv_t, seed=19), Case([50, 4000, 700], [40, 130, 128], 4, 2, hd, 16, q_t, kv_t, seed=20),
+             Case([300, 5000, 12], [1] * 3, 4, 2, hd, 16, q_t, kv_t, seed=21), Case([90] * 70, [1] * 70, 4, 2, hd, 16, q_t, kv_t, seed=22)]
+    want = [c.run() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for turn in range(12):
+        for k, s in enumerate(streams):
+            i = (turn // (3 * k + 1) + k) % 4
+            with torch.cuda.stream(s):
+                got.append((i, cases[i].run()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i]) for i, out in got)
+
+
+def test_captured_runs_on_two_streams():
+    """Two captured steps with workspaces of their own, replayed at once."""
+    cases = [Case([900, 0, 300], [200, 70, 1], 4, 2, 128, 16, BF16, BF16, seed=23), Case([50, 4000], [1, 1], 4, 2, 64, 16, F32, BF16, seed=24)]
+    want = [c.run() for c in cases]
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in cases], [], []
+    for c, s in zip(cases, streams):
+        out = torch.empty_like(c.q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(3):
+                c.run(out=out)
+        graphs.append(g)
+        outs.append(out)
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
