@@ -465,8 +465,9 @@ typedef struct {
   float scale; /* 1e-20 .. 1e20 */
 } ctts_paged_attn;
 CTTS_API int ctts_op_paged_attention(const ctts_paged_attn* p, void* stream);
-/* Workspace bytes a call with these sizes needs on the current device (the
- * data pointers are not looked at). */
+/* Workspace bytes that serve calls with these types and heads and up to
+ * max_new new rows a request on the current device (the data pointers are not
+ * looked at; batch, rows and max_pages do not matter). */
 CTTS_API int ctts_op_paged_attention_workspace(const ctts_paged_attn* p, size_t* bytes);
 
 #ifdef __cplusplus

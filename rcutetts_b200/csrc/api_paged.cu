@@ -110,9 +110,8 @@ extern "C" int ctts_op_paged_attention_workspace(const ctts_paged_attn* p, size_
   CTTS_REQ(bytes, CTTS_ERR_ARG, "null argument");
   const int rc = check_attn(p);
   if (rc != CTTS_OK) return rc;
-  const PagedAttnPlan pl = paged_attn_plan(*p);
-  CTTS_REQ(pl.ctas > 0, CTTS_ERR_CUDA, "no CUDA device");
-  *bytes = pl.ws_bytes;
+  CTTS_REQ(paged_attn_plan(*p).ctas > 0, CTTS_ERR_CUDA, "no CUDA device");
+  *bytes = paged_attn_ws_bytes(*p);
   return CTTS_OK;
 }
 

@@ -18,9 +18,10 @@ cudaError_t launch_paged_append(const ctts_paged_append& p, cudaStream_t s);
 struct PagedAttnPlan {
   int ctas = 0;       // persistent CTAs
   int tile_rows = 0;  // packed rows (token-major, query heads of a KV head inside) per work item
-  size_t ws_bytes = 0;
+  size_t ws_bytes = 0;  // of this call
 };
 PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p);
+size_t paged_attn_ws_bytes(const ctts_paged_attn& p);  // that serve calls with up to p.max_new new rows
 cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s);
 
 }  // namespace ctts

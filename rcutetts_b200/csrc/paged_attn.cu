@@ -661,6 +661,15 @@ PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
   return pl;
 }
 
+// Fewer rows can want more: short items of few rows leave an SM room for more
+// blocks, each with partial states of its own.
+size_t paged_attn_ws_bytes(const ctts_paged_attn& p) {
+  ctts_paged_attn q = p;
+  size_t most = paged_attn_plan(p).ws_bytes;
+  for (q.max_new = 0; q.max_new < p.max_new && is_short(q); q.max_new++) most = std::max(most, paged_attn_plan(q).ws_bytes);
+  return most;
+}
+
 cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   if (p.rows == 0 || p.max_new == 0) return cudaSuccess;
   const PagedAttnPlan pl = paged_attn_plan(p);
