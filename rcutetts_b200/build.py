@@ -1,5 +1,7 @@
 """Build libcutetts_b200.so (sm_100a) in-tree with nvcc, and the torch binding
-of the paged operators beside it.
+of the paged operators beside it.  The library needs the CUDA toolkit alone;
+where torch with CUDA, or Python's headers, are missing it is built without
+the binding.
 
 Each source compiles to an object under rcutetts_b200/_build/ (in parallel,
 skipped when up to date), then one shared library is linked next to this
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -82,16 +85,25 @@ def build(verbose: bool = False) -> str:
     return LIB
 
 
-def build_ext() -> str:
-    """_paged_ext.so against the installed torch, linked to the library beside it."""
+def _no_ext(why: str) -> None:
+    print(f"the torch binding of the paged operators is not built: {why}", file=sys.stderr)
+
+
+def build_ext() -> str | None:
+    """_paged_ext.so against the installed torch, linked to the library beside it.  None, and a word on stderr, where there is no
+    torch to build it against."""
     newest = max(os.path.getmtime(p) for p in (EXT_SRC, os.path.join(ROOT, "include", "cutetts_b200.h")))
     if os.path.exists(EXT) and os.path.getmtime(EXT) >= newest:
         return EXT
-    import sysconfig
-
-    import torch
-
+    try:
+        import torch
+    except ImportError as e:
+        return _no_ext(str(e))
     troot = os.path.dirname(torch.__file__)
+    for p in (os.path.join(troot, "lib", "libtorch_cuda.so"), os.path.join(troot, "include", "ATen", "ATen.h"),
+              os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        if not os.path.exists(p):
+            return _no_ext(f"{p} is missing")
     inc = [os.path.join(troot, "include"), os.path.join(troot, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
