@@ -90,15 +90,18 @@ def _no_ext(why: str) -> None:
 
 
 def build_ext() -> str | None:
-    """_paged_ext.so against the installed torch, linked to the library beside it.  None, and a word on stderr, where there is no
-    torch to build it against."""
-    newest = max(os.path.getmtime(p) for p in (EXT_SRC, os.path.join(ROOT, "include", "cutetts_b200.h")))
-    if os.path.exists(EXT) and os.path.getmtime(EXT) >= newest:
-        return EXT
+    """_paged_ext.so against the installed torch, linked to the library beside it; again when its source, torch or Python is another.
+    None, and a word on stderr, where there is no torch to build it against."""
     try:
         import torch
     except ImportError as e:
         return _no_ext(str(e))
+    newest = max(os.path.getmtime(p) for p in (EXT_SRC, os.path.join(ROOT, "include", "cutetts_b200.h")))
+    made_for, stamp = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}", os.path.join(BUILD, "paged_ext.made_for")
+    if os.path.exists(EXT) and os.path.getmtime(EXT) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == made_for:
+                return EXT
     troot = os.path.dirname(torch.__file__)
     for p in (os.path.join(troot, "lib", "libtorch_cuda.so"), os.path.join(troot, "include", "ATen", "ATen.h"),
               os.path.join(sysconfig.get_paths()["include"], "Python.h")):
@@ -107,12 +110,16 @@ def build_ext() -> str | None:
     inc = [os.path.join(troot, "include"), os.path.join(troot, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"), sysconfig.get_paths()["include"]]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{p}" for p in inc] + [
-           EXT_SRC, "-o", EXT, f"-L{HERE}", "-l:libcutetts_b200.so", f"-L{os.path.join(troot, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DPAGED_EXT_TORCH="{torch.__version__}"']
+    cmd += [f"-I{p}" for p in inc] + [EXT_SRC, "-o", EXT + ".new", f"-L{HERE}", "-l:libcutetts_b200.so", f"-L{os.path.join(troot, 'lib')}",
+                                      "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    os.makedirs(BUILD, exist_ok=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {EXT_SRC}:\n{r.stderr[-4000:]}")
+    os.replace(EXT + ".new", EXT)  # (a process may have the old one mapped)
+    with open(stamp, "w") as f:
+        f.write(made_for)
     return EXT
 
 

@@ -360,6 +360,18 @@ PyMethodDef kMethods[] = {
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_paged_ext", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
+// Whether torch is the one this was built for: the layout of its classes goes
+// with the version.
+bool same_torch() {
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* version = torch ? PyObject_GetAttrString(torch, "__version__") : nullptr;
+  const bool same = version && PyUnicode_Check(version) && PyUnicode_CompareWithASCIIString(version, PAGED_EXT_TORCH) == 0;
+  if (version && !same) PyErr_Format(PyExc_ImportError, "_paged_ext.so was built for torch " PAGED_EXT_TORCH ", this is %S", version);
+  Py_XDECREF(version);
+  Py_XDECREF(torch);
+  return same;
+}
+
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_ext(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__paged_ext(void) { return same_torch() ? PyModule_Create(&kModule) : nullptr; }

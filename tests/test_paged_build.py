@@ -24,3 +24,51 @@ def test_library_builds_without_torch(built, monkeypatch, tmp_path, capsys):
     assert build.build() == build.LIB
     assert not os.path.exists(build.EXT)
     assert "torch" in capsys.readouterr().err
+
+
+def fake_compiler(monkeypatch):
+    """The compiler calls of build_ext(): each is noted and leaves its output."""
+    import subprocess
+
+    calls = []
+
+    def run(cmd, **kw):
+        calls.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build.subprocess, "run", run)
+    return calls
+
+
+@pytest.mark.parametrize("what", ["torch", "python"])
+def test_binding_is_built_again_for_another_torch_or_python(built, monkeypatch, tmp_path, what):
+    import sysconfig
+
+    import torch
+
+    monkeypatch.setattr(build, "EXT", str(tmp_path / "_paged_ext.so"))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path))
+    calls = fake_compiler(monkeypatch)
+    build.build_ext()
+    build.build_ext()
+    assert len(calls) == 1  # up to date
+    if what == "torch":
+        monkeypatch.setattr(torch, "__version__", "0.0.1")
+    else:
+        old = sysconfig.get_config_var
+        monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "cpython-39-none" if name == "SOABI" else old(name))
+    build.build_ext()
+    assert len(calls) == 2
+    build.build_ext()
+    assert len(calls) == 2
+
+
+def test_binding_of_another_torch_is_refused(monkeypatch):
+    """It uses torch's C++ classes, whose layout goes with the version: import says so instead of running on it."""
+    import subprocess
+    import sys
+
+    code = "import torch; torch.__version__ = '0.0.1'; from rcutetts_b200 import paged"
+    r = subprocess.run([sys.executable, "-c", code], cwd=build.ROOT, capture_output=True, text=True)
+    assert r.returncode and "ImportError" in r.stderr and "0.0.1" in r.stderr and "python -m rcutetts_b200.build" in r.stderr
