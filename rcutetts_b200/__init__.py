@@ -5,6 +5,9 @@ of include/cutetts_b200.h); this package is the host-side mirror of the
 reference crate's model API (see rcutetts_b200.model) and of the paged KV-cache
 operators (rcutetts_b200.paged).
 """
+import importlib.util as _util
+import os as _os
+
 from .config import DiTConfig, FrameConfig, LMConfig, VAEConfig  # noqa: F401
 
 _MODEL_NAMES = {
@@ -15,7 +18,10 @@ _MODEL_NAMES = {
 
 _PAGED_NAMES = {"PagedStep", "paged_plan", "paged_append", "paged_attention", "paged_attention_workspace"}
 
-__all__ = ["LMConfig", "DiTConfig", "VAEConfig", "FrameConfig"] + sorted(_MODEL_NAMES | _PAGED_NAMES)
+# the paged operators need torch and their binding, the rest does not
+_HAS_PAGED = _os.path.exists(_os.path.join(_os.path.dirname(__file__), "_paged_ext.so")) and _util.find_spec("torch") is not None
+
+__all__ = ["LMConfig", "DiTConfig", "VAEConfig", "FrameConfig"] + sorted(_MODEL_NAMES | (_PAGED_NAMES if _HAS_PAGED else set()))
 
 
 def __getattr__(name):

@@ -72,3 +72,22 @@ def test_binding_of_another_torch_is_refused(monkeypatch):
     code = "import torch; torch.__version__ = '0.0.1'; from rcutetts_b200 import paged"
     r = subprocess.run([sys.executable, "-c", code], cwd=build.ROOT, capture_output=True, text=True)
     assert r.returncode and "ImportError" in r.stderr and "0.0.1" in r.stderr and "python -m rcutetts_b200.build" in r.stderr
+
+
+@pytest.mark.parametrize("gone", ["torch", "binding"])
+def test_star_import_without_the_binding(gone):
+    """`from rcutetts_b200 import *` needs neither torch nor the binding: then it comes without the paged operators."""
+    import subprocess
+    import sys
+
+    hide = {"torch": "sys.modules['torch'] = None", "binding": "import os.path; e = os.path.exists; "
+            "os.path.exists = lambda p: '_paged_ext' not in str(p) and e(p); sys.modules['rcutetts_b200._paged_ext'] = None"}[gone]
+    code = f"import sys; {hide}\nfrom rcutetts_b200 import *\nLMConfig(); FrameEngine; assert 'paged_plan' not in globals()"
+    r = subprocess.run([sys.executable, "-c", code], cwd=build.ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+
+def test_star_import_has_the_paged_operators():
+    names = {}
+    exec("from rcutetts_b200 import *", names)
+    assert {"LMConfig", "QwenW", "PagedStep", "paged_plan", "paged_append", "paged_attention", "paged_attention_workspace"} <= set(names)
