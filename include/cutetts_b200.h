@@ -445,8 +445,8 @@ CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
  * max_new is an upper bound of the requests' new rows (rows beyond it are
  * left as they were); a length above max_pages*page_size is cut to that.
  * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
- * n_heads / n_kv_heads <= 16; max_pages * page_size < 2^31, and times n_kv_heads
- * below 5 * 10^10.  Scores, softmax and sums are float32.  With
+ * n_heads / n_kv_heads <= 16; max_pages * page_size <= 2^31 - 128, and times
+ * n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.  With
  * bf16 queries the softmax weights enter the product with V in bf16; with
  * float32 queries every operand carries 24 bits.
  * The result depends on the split of the work over the GPU, which follows

@@ -1,0 +1,19 @@
+"""Sizes at the edge of what the paged KV-cache operators take: refused by the host, before anything is launched."""
+import ctypes as C
+
+import pytest
+
+from rcutetts_b200 import _lib
+from test_paged_cpu import call, pack
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64])
+def test_attention_refuses_lengths_whose_last_tile_passes_31_bits(page):
+    """Keys go by in tiles of up to 128: a length's last tile has to end below 2^31, or the count of tiles wraps round."""
+    most = (2**31 - 128) // page
+    over = dict(h=1, heads=4, qld=4 * 64, old=4 * 64, n=100, p=page)
+    for pages in (most + 1, (2**31 - 1) // page):
+        args = pack("attention", pages=pages, tld=pages, **over)
+        assert call("ctts_op_paged_attention", args)[0] == _lib.ERR_RANGE
+        assert _lib.load().ctts_op_paged_attention_workspace(args, C.byref(C.c_size_t())) == _lib.ERR_RANGE
+    assert call("ctts_op_paged_attention", pack("attention", pages=most, tld=most, rows=0, **over))[0] == 0
