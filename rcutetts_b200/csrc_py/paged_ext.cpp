@@ -141,6 +141,11 @@ at::Tensor part(const at::Tensor& t, int64_t first, int64_t n) {
   return at::Tensor(std::move(impl));
 }
 
+// A call has written to t: what autograd has saved of it is another version.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A negative status as CttsError(code, message).
 void done(int rc) {
   if (rc == CTTS_OK) return;
@@ -202,6 +207,8 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.positions = p.state + 4;
     p.slots = p.positions + r;
     done(ctts_op_paged_plan(&p, on.stream));
+    written(tab);
+    written(free);
     PyObject* t = PyTuple_New(5);
     if (!t) throw python_error();
     const int64_t first[5] = {0, b, 2 * b + 5, 2 * b + 5 + r, 2 * b + 1}, len[5] = {b, b + 1, r, r, 4};
@@ -256,7 +263,10 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.q_ld = rows_ld(out, rows, p.n_heads, hd, "out must be a [rows, n_heads, head dim] tensor with whole rows");
     p.q = out.data_ptr();
     done(ctts_op_paged_append(&p, on.stream));
+    written(k);
+    written(v);
     if (a[11] != Py_None) {
+      written(out);
       Py_INCREF(a[11]);
       return a[11];
     }
@@ -322,6 +332,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.workspace = ws.data_ptr();
     done(ctts_op_paged_attention(&p, on.stream));
     if (a[8] != Py_None) {
+      written(out);
       Py_INCREF(a[8]);
       return a[8];
     }
