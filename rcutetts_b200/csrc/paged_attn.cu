@@ -49,9 +49,12 @@ CTTS_DEV void ldsm4_t(uint32_t addr, uint32_t* r) {
 // and unread).  Bound by the cache's bytes: what there is to compute per key
 // (mma.sync m16n8k16, two products of 16 rows) is far below what the tensor
 // core's legacy path gives, so the tiles go by in a ring that one producer
-// warp fills by TMA, and two blocks an SM overlap their latencies.
-// 30 requests of 2000 to 32000 tokens, 8 KV heads of 128, bf16: 181 us, 6.5
-// TB/s (plain cp.async loads by the computing warps: 272 us).
+// warp fills by TMA; where shared memory holds two blocks an SM they overlap
+// their latencies.
+// 30 requests of 2000 to 32000 tokens, 16 heads on 8 KV heads of 128, bf16:
+// 181 us, 6.5 TB/s (plain cp.async loads by the computing warps: 272 us).
+// With float32 queries an SM holds one block there: 273 us, 4.4 TB/s; over a
+// float32 cache, twice the bytes, 565 us, 4.3 TB/s.
 template <bool QF, bool KF, int HD, int RH>
 struct Shape {
   static constexpr int R = 8 * RH;
@@ -72,8 +75,19 @@ struct Shape {
   static constexpr int KT = C / 32;  // 8-key column tiles per warp and key tile
   // query fragments stay in registers where they are few
   static constexpr bool QREG = NQ * (HD / 16) * 2 * RH <= 16;
-  static constexpr int CTAS = STAGE <= 32768 ? 2 : 1;  // an SM holds at least this many blocks
-  static size_t smem(int rows_used) { return 1024 + (size_t)NS * STAGE + QBYTES + (size_t)4 * rows_used * (HD + 2) * 4; }
+  static constexpr size_t smem(int rows_used) { return 1024 + (size_t)NS * STAGE + QBYTES + (size_t)4 * rows_used * (HD + 2) * 4; }
+  // Blocks that an SM's shared memory holds: 228 KB, of which each takes 1 KB
+  // and its static variables beside its own.  Two of 16 KB tiles while their
+  // rows are few: 64 dims up to 8 rows and more, 128 dims up to 5 (float32
+  // queries: a single one); else one.
+  static constexpr int blocks(int rows_used) {
+    const int n = (int)(228 * 1024 / (smem(rows_used) + 1024 + 512));
+    return n < 1 ? 1 : (n > 4 ? 4 : n);
+  }
+  // What the registers have to leave room for: as many as with the fewest rows.
+  // (Room for two where one fits made float32 queries over 128 dims spill: 64
+  // single tokens of 150 to 1200, 16 heads on one 16.7 us, 15.9 without.)
+  static constexpr int CTAS = blocks(RH == 1 ? 1 : 9);
 };
 
 template <bool QF, bool KF, int HD, int RH>
@@ -575,9 +589,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
 template <bool QF, bool KF, int HD, int RH>
 int attn_ctas(int rows_used) {
   using S = Shape<QF, KF, HD, RH>;
-  // shared memory: 228 KB an SM, of which each block takes 1 KB beside its own
-  const int occ = std::max(1, std::min(4, (int)(228 * 1024 / (S::smem(rows_used) + 1024 + 512))));
-  return device_sms() * occ;
+  return device_sms() * S::blocks(rows_used);
 }
 
 template <bool QF, bool KF, int HD, int RH>
