@@ -60,7 +60,10 @@ CTTS_API const char* ctts_last_error(void);
  * producer writes; every poll gives up after `spin_limit` tries (0 = the
  * default, about four million).  The kernel records the timeout and runs to
  * its end; the host call that reads the DiT error word returns
- * CTTS_ERR_TIMEOUT and clears it, and the device stays usable.
+ * CTTS_ERR_TIMEOUT and clears it, and the device stays usable.  Launches of
+ * paged attention run with CTA 0 never handing a stage of its key tiles back,
+ * so its copies wait for a stage that stays full; a wait there gives up after
+ * `spin_limit` tries of about 1.5 us (0 = the default, 2^24).
  * Process-wide, off by default; frames already captured in a CUDA graph
  * keep the setting they were captured with. */
 CTTS_API int ctts_debug_inject_wait_fault(int skip, unsigned spin_limit);

@@ -8,16 +8,22 @@
 #include <cstdlib>
 
 #include "api_common.h"
+#include "launch_state.h"
 #include "model.h"
 
 using namespace ctts;
 
-namespace {
+namespace ctts {
 
-// Injected wait fault of the small-batch DiT grid loop (error-path tests;
-// ctts_debug_inject_wait_fault), read when a launch is enqueued.
+// Injected wait fault of the small-batch DiT grid loop and of paged attention
+// (error-path tests; ctts_debug_inject_wait_fault), read when a launch is
+// enqueued.
 std::atomic<int> g_fault_skip{0};
 std::atomic<uint32_t> g_fault_spin_limit{0};
+
+}  // namespace ctts
+
+namespace {
 
 int dit_ws_ensure(ctts_dit* d, DitWs& w, int rows, int steps) {
   if (w.rows >= rows && w.steps >= steps) return CTTS_OK;

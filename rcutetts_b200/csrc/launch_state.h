@@ -11,11 +11,17 @@
 
 #include <atomic>
 #include <cstddef>
+#include <cstdint>
 #include <mutex>
 
 namespace ctts {
 
 constexpr int kMaxDevices = 64;
+
+// ctts_debug_inject_wait_fault (api_dit.cu): whether launches run with a fault,
+// and the tries of a wait (0: the kernel's own).
+extern std::atomic<int> g_fault_skip;
+extern std::atomic<uint32_t> g_fault_spin_limit;
 
 inline int current_device() {
   int d = -1;

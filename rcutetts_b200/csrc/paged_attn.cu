@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
   __shared__ AttnStart start;
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ uint32_t dead_keys[NS];  // 8-key groups of a stage whose page does not exist
-  __shared__ volatile int gave_up;
+  __shared__ volatile uint32_t tries;  // of a wait; 0: one gave up
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (sbase - smem_u32(smem_raw));
   const uint32_t qbase = sbase + NS * S::STAGE;
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
       mbar_init(&empty[i], 4);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    gave_up = 0;
+    tries = a.tries;
   }
   grid_dep_enter();
   attn_find_start<typename S::Item, kNT + 32>(a.line, &start);
@@ -133,10 +133,10 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
       const int kk = kt * C + 8 * lane;
       return lane < C / 8 && kk < cu.len ? a.p.block_tables[(long)cu.b * a.p.table_ld + (kk >> a.shift)] : -1;
     };
-    int page = page_of(), st = 0;
+    int page = page_of(), st = 0, u = 0;
     uint32_t par = 0;
 #pragma unroll 1
-    for (int u = 0, more = 1; more && !gave_up; u++) {
+    for (bool more = true; more && tries; u++) {
       const int kk = kt * C + 8 * lane, h = cu.h;
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < C / 8 && kk < cu.len && none);
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         }
       }
       if (more) page = page_of();  // of the next tile, over the wait
-      if (u >= NS) mbar_wait_or(&empty[st], par ^ 1, &gave_up);
+      if (u >= NS) mbar_wait_or(&empty[st], par ^ 1, &tries);
       if (lane == 0) {
         dead_keys[st] = dead;
         mbar_expect_tx(&full[st], S::STAGE);
@@ -171,11 +171,8 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         par ^= 1;
       }
     }
-    if (gave_up)  // copies in flight land before the block may leave
-      for (int i = 0; i < NS; i++) {
-        mbar_wait(&full[i], 0);
-        mbar_wait(&full[i], 1);
-      }
+    // copies in flight land before the block may leave, whoever gave up
+    for (int w = max(0, u - NS); w < u; w++) mbar_wait(&full[w % NS], (uint32_t)(w / NS) & 1);
     return;
   }
   auto sync_rows = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // the four computing warps
@@ -255,7 +252,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
 #pragma unroll 1
     for (int kt = cu.kt; kt < end; kt++) {
       const int key0 = kt * C + wkey;
-      mbar_wait_or(&full[buf], par, &gave_up);
+      mbar_wait_or(&full[buf], par, &tries);
       if (key0 <= plast) {
         const uint32_t kt_s = sbase + buf * S::STAGE, vt_s = kt_s + S::TILE;
         const uint8_t* const kt_p = smem + buf * S::STAGE;
@@ -427,7 +424,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[buf]);  // the stage is consumed
+      if (lane == 0 && !(a.keep_cta0 && blockIdx.x == 0)) mbar_arrive(&empty[buf]);  // the stage is consumed
       if (++buf == NS) {
         buf = 0;
         par ^= 1;
@@ -701,6 +698,8 @@ cudaError_t launch_paged_attn(const ctts_paged_attn& p, cudaStream_t s) {
   ln.ctas = pl.ctas;
   a.tile_rows = pl.tile_rows;
   a.c2 = (float)((double)p.scale * 1.4426950408889634);
+  a.keep_cta0 = g_fault_skip.load(std::memory_order_relaxed);
+  if (const uint32_t n = g_fault_spin_limit.load(std::memory_order_relaxed)) a.tries = n;
   a.parts = static_cast<AttnPart*>(p.workspace);
   a.acc = reinterpret_cast<float*>(a.parts + pl.ctas);
   a.ml = reinterpret_cast<float2*>(a.acc + (size_t)2 * pl.ctas * pl.tile_rows * p.kv.head_dim);

@@ -38,6 +38,8 @@ struct PagedAttnArgs {
   int rows_used = 0;             // packed rows a short item can have
   float c2 = 0;                  // scale * log2(e): scores to powers of two
   AttnPart* parts = nullptr;     // [ctas]
+  uint32_t tries = kWaitLimit;   // of a wait
+  int keep_cta0 = 0;             // error-path testing (ctts_debug_inject_wait_fault): CTA 0 never hands a stage back
   float2* ml = nullptr;          // [2 * ctas][tile_rows]: maximum of q . k, sum
   float* acc = nullptr;          // [2 * ctas][tile_rows][hd]: unnormalised output
 };
@@ -355,14 +357,14 @@ CTTS_DEV bool mbar_try(uint64_t* bar, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-// Bounded wait, and a flag for all roles when it gives up: nobody waits after
-// that, the block runs to its end.
-CTTS_DEV void mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+// Wait of *tries tries, which all roles of a block share.  The one that gives
+// up sets them to zero: nobody waits after that, the block runs to its end.
+CTTS_DEV void mbar_wait_or(uint64_t* bar, uint32_t parity, volatile uint32_t* tries) {
   if (mbar_try(bar, parity)) return;
 #pragma unroll 1
-  for (uint32_t it = 0; it < kWaitLimit && !*gave_up; ++it)
+  for (uint32_t it = 0; it < *tries; ++it)
     if (mbar_try(bar, parity)) return;
-  *gave_up = 1;
+  *tries = 0;
 }
 CTTS_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");

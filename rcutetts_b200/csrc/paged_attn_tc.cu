@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
   __shared__ __align__(8) TcBars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t dead_keys[8];  // 8-key groups of a tile whose page does not exist
-  __shared__ volatile int gave_up;
+  __shared__ volatile uint32_t tries;  // of a wait; 0: one gave up
   __shared__ float2 shared_ml[S::SHARE ? 128 : 1];  // maximum and sum of the second sub-tile of a shared item
   const uint32_t sbase = (smem_u32(tc_smem) + 1023u) & ~1023u;
   const uint32_t qs = sbase, ks = qs + S::NSUB * NT * S::QTERM, vs = ks + NS * S::TILE;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
     }
     mbar_init(&bars.drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    gave_up = 0;
+    tries = a.tries;
   }
   if (warp == W_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
     int page = page_of(), st = 0, u = 0;
     uint32_t par = 0;
 #pragma unroll 1
-    for (bool more = true; more && !gave_up; u++) {
+    for (bool more = true; more && tries; u++) {
       const int kk = kt * KT + 8 * lane, h = cu.h, slot = kk & (a.p.kv.page_size - 1);
       const bool none = (unsigned)page >= (unsigned)a.p.kv.n_pages;
       const uint32_t dead = __ballot_sync(0xffffffffu, lane < KT / 8 && kk < cu.len && none);
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
 #pragma unroll 1
       for (int kv = 0; kv < 2; kv++) {
         uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-        if (u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &gave_up);
+        if (u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &tries);
         if (lane == 0) {
           if (kv == 0) dead_keys[u & 7] = dead;  // read behind the scores' barrier; the copies are at most 6 tiles ahead
           mbar_expect_tx(full, S::TILE);
@@ -304,11 +304,12 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
         par ^= 1;
       }
     }
-    if (gave_up)  // copies in flight land before the block may leave
-      for (int w = max(0, u - NS); w < u; w++) {
-        mbar_wait(&bars.k_full[w % NS], (uint32_t)(w / NS) & 1);
-        mbar_wait(&bars.v_full[w % NS], (uint32_t)(w / NS) & 1);
-      }
+    // copies in flight land before the block may leave, whoever gave up
+#pragma unroll 1
+    for (int w = max(0, u - NS); w < u; w++) {
+      mbar_wait(&bars.k_full[w % NS], (uint32_t)(w / NS) & 1);
+      mbar_wait(&bars.v_full[w % NS], (uint32_t)(w / NS) & 1);
+    }
   } else if (KF && left > 0 && warp > W_MMA) {
     // ---- producers of a float32 cache: keys and values come in by plain
     // loads (16 threads a row of 64 dims), 64 dims of 64 keys ahead of the
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
         }
         const int kv = job / NC, c = job % NC;
         uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-        if (c == 0 && u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &gave_up);
+        if (c == 0 && u >= NS) mbar_wait_or(kv ? &bars.v_empty[st] : &bars.k_empty[st], par ^ 1, &tries);
         const uint32_t dst = (kv ? vs : ks) + st * S::TILE + c * KT * 128;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
@@ -449,6 +450,10 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
       if (leader) umma_commit(bar);
       __syncwarp();
     };
+    const bool keeps = a.keep_cta0 && blockIdx.x == 0;
+    auto release = [&](uint64_t* bar) {  // a stage back to the producer
+      if (!keeps) commit(bar);
+    };
     uint32_t q_par = 0, p_par = 0;  // one bit per sub-tile
     uint32_t par = 0, par_p = 0;    // of the fills of stages st (tile i) and sp (tile i - 1)
     int st = 0, sp = 0;
@@ -458,22 +463,22 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
       const int nsub = __shfl_sync(0xffffffffu, cu.rows(a.line, R) > 128 ? 2 : 1, 0);
       if (S::PIPE) {
         // a turn: scores of tile i, then P.V of tile i - 1
-        mbar_wait_or(&bars.q_full[0], q_par, &gave_up);
+        mbar_wait_or(&bars.q_full[0], q_par, &tries);
         q_par ^= 1;
 #pragma unroll 1
         for (int i = 0; i <= n; i++) {
           if (i < n) {
-            mbar_wait_or(&bars.k_full[st], par, &gave_up);
+            mbar_wait_or(&bars.k_full[st], par, &tries);
             scores(0, st, (i & 1) * KT, &bars.s_full[i & 1]);
-            commit(&bars.k_empty[st]);
+            release(&bars.k_empty[st]);
           }
           if (i > 0) {
-            mbar_wait_or(&bars.p_full[0], p_par, &gave_up);
+            mbar_wait_or(&bars.p_full[0], p_par, &tries);
             p_par ^= 1;
-            mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+            mbar_wait_or(&bars.v_full[sp], par_p, &tries);
             values(0, sp, 0, KS, 0);
             commit(&bars.o_full[0]);
-            commit(&bars.v_empty[sp]);
+            release(&bars.v_empty[sp]);
           }
           if (i < n) {
             sp = st;
@@ -491,23 +496,23 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           if (i < n) {
             const int s = i & 1;
             if (i < 2) {
-              mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
+              mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &tries);
               q_par ^= 1u << s;
             }
-            mbar_wait_or(&bars.k_full[st], par, &gave_up);
+            mbar_wait_or(&bars.k_full[st], par, &tries);
             scores(s, st, S::SREG * s, &bars.s_full[s]);
-            commit(&bars.k_empty[st]);
+            release(&bars.k_empty[st]);
           }
           if (i > 0) {
             const int s = (i - 1) & 1;
-            mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
-            mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
+            mbar_wait_or(&bars.v_full[sp], par_p, &tries);
+            mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &tries);
             values(s, sp, 0, HALF, i > 2);
-            mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
+            mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &tries);
             p_par ^= 1u << s;
             values(s, sp, HALF, KS, 1u);
             if (i + 1 >= n) commit(&bars.o_full[s]);  // its last tile
-            commit(&bars.v_empty[sp]);
+            release(&bars.v_empty[sp]);
           }
           if (i < n) {
             sp = st;
@@ -522,31 +527,31 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
         // a turn: P.V of tile i - 1, scores of tile i
 #pragma unroll 1
         for (int i = 0; i <= n; i++) {
-          if (i > 0) mbar_wait_or(&bars.v_full[sp], par_p, &gave_up);
+          if (i > 0) mbar_wait_or(&bars.v_full[sp], par_p, &tries);
 #pragma unroll 1
           for (int s = 0; s < nsub; s++) {
             if (i > 0) {
               if (HALF) {
-                mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &gave_up);
+                mbar_wait_or(&bars.p_half[s], (p_par >> s) & 1, &tries);
                 values(s, sp, 0, HALF, i > 1);
               }
-              mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &gave_up);
+              mbar_wait_or(&bars.p_full[s], (p_par >> s) & 1, &tries);
               p_par ^= 1u << s;
               values(s, sp, HALF, KS, HALF ? 1u : 0u);
               if (i == n) commit(&bars.o_full[s]);
             }
             if (i < n) {
               if (i == 0) {
-                mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &gave_up);
+                mbar_wait_or(&bars.q_full[s], (q_par >> s) & 1, &tries);
                 q_par ^= 1u << s;
               }
-              if (s == 0) mbar_wait_or(&bars.k_full[st], par, &gave_up);
+              if (s == 0) mbar_wait_or(&bars.k_full[st], par, &tries);
               scores(s, st, S::SREG * s, &bars.s_full[s]);
             }
           }
-          if (i > 0) commit(&bars.v_empty[sp]);
+          if (i > 0) release(&bars.v_empty[sp]);
           if (i < n) {
-            commit(&bars.k_empty[st]);
+            release(&bars.k_empty[st]);
             sp = st;
             par_p = par;
             if (++st == NS) {
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
       if (left == 0) break;
       cu = Cursor::next(a.line, cu);
     }
-    if (gave_up) {  // MMAs in flight end before TMEM is given back
+    if (tries == 0) {  // MMAs in flight end before TMEM is given back
       commit(&bars.drain);
       mbar_wait(&bars.drain, 0);
     }
@@ -661,7 +666,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           d.row0 = cu.r0; d.packed0 = cu.m * R; d.rows = nrows; d.h = cu.h;
           a.parts[blockIdx.x] = d;
         }
-        mbar_wait_or(&bars.o_full[s], o_par, &gave_up);
+        mbar_wait_or(&bars.o_full[s], o_par, &tries);
         o_par ^= 1;
         if (shared && s == 1) {
           // the other sub-tile's warp of the same rows (and TMEM lanes) merges
@@ -796,7 +801,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           const int key0 = kt * KT;
           const int sb = S::PIPE ? (kt - cu.kt) & 1 : s;
           const uint32_t tS = tS0 + (S::PIPE ? sb * KT : 0);
-          mbar_wait_or(&bars.s_full[sb], (s_par >> sb) & 1, &gave_up);
+          mbar_wait_or(&bars.s_full[sb], (s_par >> sb) & 1, &tries);
           s_par ^= 1u << sb;
           if (!KF && (s == 0 || step == 2) && key0 + KT > cu.len) {
             // slots behind the length may hold anything, and 0 * NaN is NaN:
@@ -805,7 +810,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
             // Behind the scores, as a barrier's parity tells the fill of this
             // tile from the one before last only once that one is over.
             const int w = u + kt - cu.kt, st = w % NS;
-            mbar_wait_or(&bars.v_full[st], (uint32_t)(w / NS) & 1, &gave_up);
+            mbar_wait_or(&bars.v_full[st], (uint32_t)(w / NS) & 1, &tries);
             if (row < KT && key0 + row >= cu.len) {
 #pragma unroll 1
               for (int c = 0; c < NC * 8; c++)
@@ -854,7 +859,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
             if (QF) {
               if (kt > cu.kt) {
                 if (S::PIPE) {  // (two sub-tiles: the scores were issued behind it)
-                  mbar_wait_or(&bars.o_full[0], o_par, &gave_up);
+                  mbar_wait_or(&bars.o_full[0], o_par, &tries);
                   o_par ^= 1;
                   fence_after();
                 }
@@ -953,7 +958,7 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           } else if (S::PIPE && kt > cu.kt) {
             // a warp without rows keeps step: its arrival for this tile must
             // not count for the one before
-            mbar_wait_or(&bars.o_full[0], o_par, &gave_up);
+            mbar_wait_or(&bars.o_full[0], o_par, &tries);
             o_par ^= 1;
           }
           mbar_arrive(&bars.p_full[s]);
