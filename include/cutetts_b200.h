@@ -63,7 +63,8 @@ CTTS_API const char* ctts_last_error(void);
  * CTTS_ERR_TIMEOUT and clears it, and the device stays usable.  Launches of
  * paged attention run with CTA 0 never handing a stage of its key tiles back,
  * so its copies wait for a stage that stays full; a wait there gives up after
- * `spin_limit` tries of about 1.5 us (0 = the default, 2^24).
+ * `spin_limit` tries of about 1.5 us (0 = the default, 2^24), and the rows
+ * that CTA had still to write are NaN.
  * Process-wide, off by default; frames already captured in a CUDA graph
  * keep the setting they were captured with. */
 CTTS_API int ctts_debug_inject_wait_fault(int skip, unsigned spin_limit);
@@ -362,8 +363,9 @@ CTTS_API int ctts_op_embed_gather(const float* table, int vocab, int H, const in
  * and can be captured in a CUDA graph.  Arguments the host can see are checked
  * (CTTS_ERR_ARG, CTTS_ERR_RANGE); lengths, offsets and page numbers live on
  * the device and are clamped there, so a bad one never reads or writes out of
- * range.  Waits inside a kernel are bounded; one that gives up, which no valid
- * call reaches, ends the kernel without a code, as in ctts_op_linear_noalloc. */
+ * range.  Waits inside a kernel are bounded (25 s); when one gives up, which
+ * no valid call reaches, the rows that its block had still to write are NaN:
+ * the calls are asynchronous and have no code for it. */
 
 /* K and V pools of n_pages pages of page_size token slots (a power of two,
  * 8..256).  Element d of KV head h of slot t of page p lies at

@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         *reinterpret_cast<float2*>(w + 2 + 8 * t + 2 * tq) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
     }
     sync_rows();
+    const bool lost = tries == 0;  // a wait gave up: what was computed since may be anything
     for (int i = tid; i < nrows * (HD / 2); i += kNT) {
       const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
       const float* w = wst + r * (HD + 2);
@@ -475,6 +476,7 @@ __global__ void __launch_bounds__(kNT + 32, Shape<QF, KF, HD, RH>::CTAS) paged_a
         x = fmaf(w[k * ws + 2 + d], g, x);
         y = fmaf(w[k * ws + 3 + d], g, y);
       }
+      if (lost) x = y = __int_as_float(0x7fffffff);
       if (whole) {
         const int pk = row_base + r;
         const long at = (long)(cu.r0 + pk / a.group) * a.p.out_ld + (long)(cu.h * a.group + pk % a.group) * HD + d;

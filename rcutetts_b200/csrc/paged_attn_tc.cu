@@ -45,7 +45,8 @@
 // clocks that follow long calls).  Short calls: some 5 us from
 // the launch to the first scores, 2 to 3 for each further item, and the join.
 //
-// Every wait is bounded; one that gives up raises a flag that ends all roles.
+// Every wait is bounded; after one that gives up no role waits any more, and
+// what the block still writes is NaN.
 #include <algorithm>
 
 #include "common.cuh"
@@ -691,7 +692,8 @@ __global__ void __launch_bounds__(TcShape<QF, KF, HD>::THREADS, 1) paged_attn_tc
           }
           fence_after();
           const bool none = l == 0.0f;  // the row saw no key (one that saw any has a weight of 1, or NaN)
-          const float inv = whole && !none ? 1.0f / l : 1.0f;
+          float inv = whole && !none ? 1.0f / l : 1.0f;
+          if (tries == 0) inv = __int_as_float(0x7fffffff);  // a wait gave up: what was computed since may be anything
           if (!whole && mine) a.ml[(long)place * a.tile_rows + first_row + row] = make_float2(m, l);
           if (QF) gather();
           // 32 columns of the warp's 32 rows by way of shared memory: a lane

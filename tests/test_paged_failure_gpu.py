@@ -41,3 +41,18 @@ def test_a_wait_that_runs_out_ends_the_call(q_t, kv_t, hd, new):
     _, took = faulty(c)
     assert took < 2.0
     assert torch.equal(c.run(), want)
+
+
+@pytest.mark.parametrize("q_t, kv_t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+def test_what_a_wait_that_runs_out_leaves_is_nan(q_t, kv_t, hd, new):
+    """A row is what it is without the fault, or NaN: never what happened to lie in a stage, and never what the output held."""
+    c = long_requests(new, hd, q_t, kv_t)
+    want = c.run()
+    out, _ = faulty(c)
+    lost = torch.isnan(out)
+    assert lost[:new].any()  # the first CTA begins with the first request
+    assert torch.equal(out[~lost], want[~lost]) and not lost[-new:].any()
+    rows = lost.view(out.shape[0], -1, hd)
+    assert torch.equal(rows.any(-1), rows.all(-1))  # a head's row as a whole
