@@ -400,8 +400,10 @@ typedef struct {
  * pushed entries of free_pages; nothing else.  The inputs are not changed, so
  * a repeated call gives the same step; the next step passes seq_lens as its
  * ctx_lens and state as its free_count, with other buffers for its outputs
- * (an output that is an input too is CTTS_ERR_ARG).  batch <= 4096.  A
- * negative context counts as 0. */
+ * (an output that is an input too is CTTS_ERR_ARG; no others of the buffers
+ * may overlap either).  batch is 1 to 4096.  A negative context counts as 0.
+ * free_pages has an entry for every page of the pool: pages given back beyond
+ * free_capacity are lost. */
 typedef struct {
   const int *ctx_lens, *new_lens, *free_count;
   int *block_tables, *free_pages;
@@ -446,14 +448,24 @@ CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
  * cu_rows[batch] are left as they were.  Slots at and behind a request's
  * length never reach a result, whatever they hold.  (Of the keys ahead of a
  * row that are its request's own later rows only finite ones are without
- * effect: weight 0 times an infinite or NaN value is NaN.)  out may be q.
+ * effect: weight 0 times an infinite or NaN value is NaN.)  What a row does
+ * see is taken to be finite: infinities among its query, keys and values, and
+ * float32 ones above 3.38e38, may give NaN where the formula gives an infinity
+ * or leaves them out.  out may be q; otherwise it overlaps no input.
  * max_new is an upper bound of the requests' new rows (rows beyond it are
  * left as they were); a length above max_pages*page_size is cut to that.
+ * max_new also chooses the kernel: above 16 packed rows (max_new times
+ * n_heads / n_kv_heads) all requests, single tokens too, go by tiles of 128
+ * rows.  30 single tokens of 2000 to 32000, 12 heads on 4 of 64, with max_new 1
+ * and 512: bf16 62 and 72 us, float32 queries over bf16 62 and 234, over
+ * float32 130 and 318.  So pass the step's own bound, and capture steps of
+ * single tokens apart from those with chunks.
  * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
- * n_heads / n_kv_heads <= 16; max_pages * page_size <= 2^31 - 128, and times
- * n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.  With
- * bf16 queries the softmax weights enter the product with V in bf16; with
- * float32 queries every operand carries 24 bits.
+ * batch >= 1; n_heads / n_kv_heads <= 16; max_pages * page_size <= 2^31 - 128,
+ * and times n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.
+ * With bf16 queries the softmax weights enter the product with V in bf16 (relative
+ * error of the output 0.0020 to 0.0023, 0.0017 of it its own rounding); with
+ * float32 queries every operand carries 24 bits (2 to 3 * 10^-7).
  * The result depends on the split of the work over the GPU, which follows
  * from the lengths: the same call gives the same bits.
  * workspace: ctts_op_paged_attention_workspace bytes, 16-byte aligned, no

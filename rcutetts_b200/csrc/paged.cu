@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const ctts_pag
 // waited for between warps.  Few rows (a decode step): several warps a row.
 // 16381 rows, 16 + 2 x 8 heads of 128, bf16: 55 us, 4.9 TB/s (one row a block
 // and its angles through shared memory: 89 us; four passes in flight at fewer
-// warps: 58 us, eight: 64 us).  4001 rows, 12 + 2 x 4 heads of 64, float32:
+// warps: 58 us, eight: 64 us; slots a page after the other, as plan gives
+// them, instead of scattered ones: 54.9 us).  4001 rows, 12 + 2 x 4 heads of 64, float32:
 // 9.5 us, 4.3 TB/s.
 constexpr int kAppWarps = 4;   // a block
 constexpr int kAppAhead = 2;   // loads in flight: passes of a warp

@@ -622,9 +622,12 @@ auto with_shape(const ctts_paged_attn& p, int rows, F f) {
 
 // Items of up to 16 packed rows run on this file's kernel, calls with longer
 // ones on the tcgen05 kernel (paged_attn_tc.cu) -- their short requests too: a
-// tile of 128 rows costs a short item as much as a long one, yet two launches
-// after one another took longer (43 decodes and 5 chunks of 200 to 512: 40 us
-// against 35, and 30 since such items share a CTA's two sub-tiles).
+// tile of 128 rows costs a short item as much as a long one, yet in bf16 two
+// launches after one another took longer (43 decodes and 5 chunks of 200 to
+// 512: 40 us against 35, and 30 since such items share a CTA's two sub-tiles).
+// With float32 queries they do not share, and two launches were not tried: 30
+// single tokens of 2000 to 32000 take 62 us there on this file's kernel, 234
+// beside a chunk of 20 rows (over a float32 cache 130 and 319; bf16 62 and 73).
 bool is_short(const ctts_paged_attn& p) { return (long)p.max_new * (p.n_heads / p.kv.n_kv_heads) <= 16; }
 int rows_used_of(const ctts_paged_attn& p) { return std::max(1, p.max_new * (p.n_heads / p.kv.n_kv_heads)); }
 

@@ -24,7 +24,10 @@
 // bf16: the output is rescaled only when a row's maximum has grown by more
 // than 2^8 since the last time: weights up to 256 lose nothing in floating
 // point, and the pass over O in TMEM becomes rare.  The scores stay in
-// registers between the maximum and the exponentials.
+// registers between the maximum and the exponentials.  The weights are rounded
+// to bf16 (2^-8 of each at most), as the tensor core takes one type for both
+// operands of P . V: the output's relative error is 0.0020 to 0.0023 where its
+// own rounding to bf16 makes 0.0017.
 //
 // float32 queries: queries and weights enter as three bf16 terms (24 bits),
 // and so do keys and values of a float32 cache; of the products those below

@@ -9,10 +9,11 @@ One serving step over a paged cache is a run of three calls:
 (the contracts are those of ctts_op_paged_plan / _append / _attention in
 include/cutetts_b200.h).  The pools k_pages and v_pages are [pages, page_size,
 kv heads, head dim] tensors of float32 or bf16 with any order in memory; one
-pair per layer.  For inference: no gradients flow through the calls.  They run
-on the tensors' device, on its current stream unless `stream` is given, and
-can be captured in a CUDA graph.  Arguments of a wrong type, shape or device
-raise ValueError, what the library refuses CttsError.
+pair per layer.  For inference: no gradients flow through the calls (what they
+write in place counts as a new version of its tensor).  They run on the tensors'
+device, on its current stream unless `stream` is given, and can be captured in a
+CUDA graph.  Arguments of a wrong type, shape or device raise ValueError, what
+the library refuses CttsError: a step without requests, for one.
 """
 from __future__ import annotations
 
@@ -65,7 +66,8 @@ def paged_append(x, k_pages, v_pages, positions, slots, n_heads: int, q_norm=Non
 
 def paged_attention(q, k_pages, v_pages, block_tables, cu_rows, seq_lens, max_new: int, scale: Optional[float] = None, out=None,
                     workspace=None, stream=None) -> torch.Tensor:
-    """Causal attention of the rows q [rows, heads, head dim] over the pages of their requests; max_new bounds a request's rows.
+    """Causal attention of the rows q [rows, heads, head dim] over the pages of their requests; max_new bounds a request's rows
+    (pass the step's own bound: a generous one costs time, see ctts_op_paged_attention).
 
     Returns [rows, heads, head dim] in q's type (`out`, whose rows behind the last request are left as they were, or a new tensor).
     workspace: a tensor of paged_attention_workspace bytes or more to use instead of one from torch's allocator; calls that may
