@@ -401,7 +401,8 @@ typedef struct {
  * a repeated call gives the same step; the next step passes seq_lens as its
  * ctx_lens and state as its free_count, with other buffers for its outputs
  * (an output that is an input too is CTTS_ERR_ARG; no others of the buffers
- * may overlap either).  batch is 1 to 4096.  A negative context counts as 0.
+ * may overlap either).  batch is 1 to 4096, max_rows and free_capacity are at
+ * most 2^30.  A negative context counts as 0.
  * free_pages has an entry for every page of the pool: pages given back beyond
  * free_capacity are lost. */
 typedef struct {

@@ -70,6 +70,8 @@ extern "C" int ctts_op_paged_plan(const ctts_paged_plan* p, void* stream) {
   CTTS_REQ(p->batch > 0 && p->max_pages > 0 && p->max_rows >= 0 && p->free_capacity >= 0 && p->table_ld >= p->max_pages,
            CTTS_ERR_ARG, "bad size");
   CTTS_REQ(p->batch <= kPlanMaxBatch, CTTS_ERR_RANGE, "at most 4096 requests in one plan");
+  // (the kernel's counters go on by the grid's threads)
+  CTTS_REQ(p->max_rows <= 1 << 30 && p->free_capacity <= 1 << 30, CTTS_ERR_RANGE, "at most 2^30 rows and free pages");
   CTTS_REQ(p->page_size >= 8 && p->page_size <= 256 && (p->page_size & (p->page_size - 1)) == 0, CTTS_ERR_ARG,
            "page_size must be a power of two, 8 to 256");
   CTTS_REQ((int64_t)p->max_pages * p->page_size <= 0x7fffffff, CTTS_ERR_RANGE, "max_pages * page_size must fit 31 bits");
