@@ -462,8 +462,8 @@ CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
  * float32 130 and 318.  So pass the step's own bound, and capture steps of
  * single tokens apart from those with chunks.
  * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
- * batch >= 1; n_heads / n_kv_heads <= 16; max_pages * page_size <= 2^31 - 128,
- * and times n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.
+ * batch is 1 to 2^30; n_heads / n_kv_heads <= 16; max_pages * page_size <=
+ * 2^31 - 128, and times n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.
  * With bf16 queries the softmax weights enter the product with V in bf16 (relative
  * error of the output 0.0020 to 0.0023, 0.0017 of it its own rounding); with
  * float32 queries every operand carries 24 bits (2 to 3 * 10^-7).

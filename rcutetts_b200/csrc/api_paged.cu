@@ -52,6 +52,7 @@ int check_attn(const ctts_paged_attn* p) {
   CTTS_REQ(p->q_dtype == CTTS_F32 || (p->q_dtype == CTTS_BF16 && p->kv.dtype == CTTS_BF16), CTTS_ERR_ARG,
            "queries are float32, or bf16 over a bf16 cache");
   CTTS_REQ(p->batch > 0 && p->rows >= 0 && p->max_new >= 0 && p->max_pages > 0, CTTS_ERR_ARG, "bad size");
+  CTTS_REQ(p->batch <= 1 << 30, CTTS_ERR_RANGE, "too many requests");  // (counted in strides of a block's threads)
   // (the last tile of keys, of 128 at most, ends below 2^31)
   CTTS_REQ((int64_t)p->max_pages * p->kv.page_size <= 0x7fffffff - 127, CTTS_ERR_RANGE, "max_pages * page_size must not exceed 2^31 - 128");
   CTTS_REQ((int64_t)p->rows * (p->n_heads / p->kv.n_kv_heads) <= 0x7fffffff, CTTS_ERR_RANGE, "too many rows");

@@ -24,3 +24,11 @@ def test_plan_refuses_lists_whose_loops_pass_31_bits(over):
     """The lists are filled in strides of the grid (some 75 thousand entries): a counter near 2^31 would wrap round to negative entries."""
     far = dict(pos=1 << 40, slots=1 << 41, free=1 << 42)  # lists that overlap nothing
     assert call("ctts_op_paged_plan", pack("plan", **far, **over))[0] == _lib.ERR_RANGE
+
+
+@pytest.mark.parametrize("batch", [2**30 + 1, 2**31 - 1])
+def test_attention_refuses_batches_whose_scan_passes_31_bits(batch):
+    """Each block scans the requests in strides of its threads: near 2^31 that counter would wrap round and never end."""
+    args = pack("attention", batch=batch, pages=1, tld=1)
+    assert call("ctts_op_paged_attention", args)[0] == _lib.ERR_RANGE
+    assert _lib.load().ctts_op_paged_attention_workspace(args, C.byref(C.c_size_t())) == _lib.ERR_RANGE
