@@ -463,10 +463,11 @@ CTTS_API int ctts_op_paged_append(const ctts_paged_append* p, void* stream);
  * single tokens apart from those with chunks.
  * Types: q and out bf16 over a bf16 cache, or q and out float32 over either;
  * batch is 1 to 2^30; n_heads / n_kv_heads <= 16; max_pages * page_size <=
- * 2^31 - 128, and times n_kv_heads below 5 * 10^10.  Scores, softmax and sums are float32.
- * With bf16 queries the softmax weights enter the product with V in bf16 (relative
- * error of the output 0.0020 to 0.0023, 0.0017 of it its own rounding); with
- * float32 queries every operand carries 24 bits (2 to 3 * 10^-7).
+ * 2^31 - 128, and times n_kv_heads below 5 * 10^10.  Scores, softmax and sums
+ * are float32.  With bf16 queries the softmax weights enter the product with V
+ * in bf16 (relative error of the output 0.0020 to 0.0023, 0.0017 of it its own
+ * rounding); with float32 queries every operand carries 24 bits (2 to
+ * 3 * 10^-7).
  * The result depends on the split of the work over the GPU, which follows
  * from the lengths: the same call gives the same bits.
  * workspace: ctts_op_paged_attention_workspace bytes, 16-byte aligned, no

@@ -94,7 +94,7 @@ def build_ext() -> str | None:
     None, and a word on stderr, where there is no torch to build it against."""
     try:
         import torch
-    except ImportError as e:
+    except (ImportError, OSError) as e:  # (OSError: one of its libraries is missing)
         return _no_ext(str(e))
     newest = max(os.path.getmtime(p) for p in (EXT_SRC, os.path.join(ROOT, "include", "cutetts_b200.h")))
     made_for, stamp = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}", os.path.join(BUILD, "paged_ext.made_for")

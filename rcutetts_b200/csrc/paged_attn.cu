@@ -586,12 +586,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __g
 }
 
 template <bool QF, bool KF, int HD, int RH>
-int attn_ctas(int rows_used) {
-  using S = Shape<QF, KF, HD, RH>;
-  return device_sms() * S::blocks(rows_used);
-}
-
-template <bool QF, bool KF, int HD, int RH>
 cudaError_t launch_attn(const PagedAttnArgs& a, cudaStream_t s) {
   using S = Shape<QF, KF, HD, RH>;
   static SmemOptIn opt;
@@ -656,31 +650,35 @@ bool paged_pool_map(CUtensorMap* m, const void* base, const ctts_paged_kv& kv, i
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) {
+static PagedAttnPlan plan_for(const ctts_paged_attn& p, int sms) {
   PagedAttnPlan pl;
   if (is_short(p)) {
     const int rows = rows_used_of(p);
     with_shape(p, rows, [&](auto q, auto k, auto hd, auto rh) {
       constexpr bool QF = decltype(q)::value, KF = decltype(k)::value;
       constexpr int HD = decltype(hd)::value, RH = decltype(rh)::value;
-      pl.ctas = attn_ctas<QF, KF, HD, RH>(rows);
-      pl.tile_rows = Shape<QF, KF, HD, RH>::R;
+      using S = Shape<QF, KF, HD, RH>;
+      pl.ctas = sms * S::blocks(rows);
+      pl.tile_rows = S::R;
       return 0;
     });
   } else {
-    pl.ctas = device_sms();
+    pl.ctas = sms;
     pl.tile_rows = paged_attn_tc_rows(p);
   }
   pl.ws_bytes = pl.ctas * (sizeof(AttnPart) + (size_t)2 * pl.tile_rows * (p.kv.head_dim + 2) * sizeof(float));
   return pl;
 }
 
+PagedAttnPlan paged_attn_plan(const ctts_paged_attn& p) { return plan_for(p, device_sms()); }
+
 // Fewer rows can want more: short items of few rows leave an SM room for more
 // blocks, each with partial states of its own.
 size_t paged_attn_ws_bytes(const ctts_paged_attn& p) {
+  const int sms = device_sms();
   ctts_paged_attn q = p;
-  size_t most = paged_attn_plan(p).ws_bytes;
-  for (q.max_new = 0; q.max_new < p.max_new && is_short(q); q.max_new++) most = std::max(most, paged_attn_plan(q).ws_bytes);
+  size_t most = plan_for(p, sms).ws_bytes;
+  for (q.max_new = 0; q.max_new < p.max_new && is_short(q); q.max_new++) most = std::max(most, plan_for(q, sms).ws_bytes);
   return most;
 }
 
