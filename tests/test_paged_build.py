@@ -5,12 +5,13 @@ import pytest
 
 from rcutetts_b200 import build
 
+if not (os.path.exists(build.LIB) and os.path.exists(build.EXT)):
+    build.build()
+
 
 @pytest.fixture
 def built(monkeypatch):
     """A library that is up to date, so that build() gets to the binding at once."""
-    if not os.path.exists(build.LIB):
-        build.build()
     monkeypatch.setattr(build, "_compile", lambda src, hdr, verbose: build.LIB)
 
 
